@@ -27,6 +27,8 @@ from .capi import (  # noqa: F401
     debug_attention_slices,
     debug_gemm_form,
     debug_gemv_form,
+    kv4_attention_workspace_bytes,
+    kv4_cache_bytes,
     library_path,
     linear_static_scratch,
     load_library,

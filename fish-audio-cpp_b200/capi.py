@@ -101,6 +101,15 @@ def load_library() -> C.CDLL:
         "w8a8_paged_attention_decode": (I, [P, P, P, P, P, P, P, I, I, I, I, F, I, I, I, I, P, P, I, P]),
         "w8a8_qkv_attention_decode": (I, [P, P, P, P, F, P, P, P, P, P, P, P, I, I, I, I, F, I, I, I, I, P, P, I, P]),
         "w8a8_qkv_attention_decode_ahead": (I, [P, P, P, P, F, P, P, P, P, P, P, P, I, I, I, I, F, I, I, I, I, P, P, I, P]),
+        "w8a8_plan_blocks": (I, [P, P, P, I, P, I, P, I, P, P, P, P, P, P, I, P, P]),
+        "w8a8_kv4_cache_bytes": (Z, [I, I, I, I, I]),
+        "w8a8_kv4_write": (I, [P, P, P, P, F, P, P, P, P, I, I, I, I, I, I, I, I, P, P]),
+        "w8a8_kv4_read": (I, [P, P, I, P, I, I, I, I, I, I, P, P, P]),
+        "w8a8_kv4_attention_workspace_bytes": (Z, [I, I]),
+        "w8a8_kv4_attention_decode": (I, [P, P, P, I, P, P, P, I, I, I, I, F, I, I, I, I, I, P, P, P]),
+        "w8a8_linear4_q": (I, [P, P, P, I, P, P, P, I, I, I, I, P, P]),
+        "w8a8_quantize_weight4": (I, [P, P, I, I, I, P, P, P]),
+        "w8a8_unpack_weight4": (I, [P, P, I, I, P, P]),
         "w8a8_tp_create": (I, [P, I, I, I, I, P]),
         "w8a8_tp_connect": (I, [P, P]),
         "w8a8_tp_allreduce_rmsnorm_quantize": (I, [P, P, P, P, F, P, P, I, I, I, I, P, P, P, P]),
@@ -133,7 +142,9 @@ EXPORTS = [
     "w8a8_decode_stack_workspace_bytes", "w8a8_decode_stack_step",
     "w8a8_decode_stack_timeline",
     "w8a8_pack_gate_up", "w8a8_qknorm_rope_kvwrite", "w8a8_paged_attention_decode", "w8a8_qkv_attention_decode",
-    "w8a8_qkv_attention_decode_ahead", "w8a8_tp_create", "w8a8_tp_connect",
+    "w8a8_qkv_attention_decode_ahead", "w8a8_plan_blocks", "w8a8_kv4_cache_bytes", "w8a8_kv4_write", "w8a8_kv4_read",
+    "w8a8_kv4_attention_workspace_bytes", "w8a8_kv4_attention_decode", "w8a8_linear4_q", "w8a8_quantize_weight4", "w8a8_unpack_weight4",
+    "w8a8_tp_create", "w8a8_tp_connect",
     "w8a8_tp_linear_q", "w8a8_tp_allreduce_rmsnorm_quantize", "w8a8_packed_weight_bytes", "w8a8_pack_weight", "w8a8_register_packed_weight",
     "w8a8_static_scratch_bytes", "w8a8_linear_static_scratch", "w8a8_static_scratch_check_status",
 ]
@@ -235,6 +246,15 @@ def debug_gemv_form(M, N, K, group_size, sms=148, kernel=KERNEL_GEMV_PACKED):
 def debug_attention_slices(batch, n_kv, max_blocks, sms, room):
     """Context slices of the paged attention where none are asked for; room: {S: clusters of S CTAs that run at once}."""
     return load_library().w8a8_debug_attention_slices(batch, n_kv, max_blocks, sms, (C.c_int * 9)(*(room.get(s, 0) for s in range(9))))
+
+
+def kv4_cache_bytes(n_blocks, n_layers, n_kv, head_dim, group) -> int:
+    """Bytes of a paged cache in 4 bits; 0 where the arguments describe none."""
+    return load_library().w8a8_kv4_cache_bytes(n_blocks, n_layers, n_kv, head_dim, group)
+
+
+def kv4_attention_workspace_bytes(n_heads, n_kv) -> int:
+    return load_library().w8a8_kv4_attention_workspace_bytes(n_heads, n_kv)
 
 
 class Context:
@@ -391,6 +411,42 @@ class Context:
                                             _ptr(positions), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), _ptr(seq_lens),
                                             _ptr(out), batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers, n_kv,
                                             quant_group_size, _ptr(Xq), _ptr(Xs), context_splits, _stream(stream)), name)
+
+    def plan_blocks(self, cached_lens, new_lens, batch, block_table, max_blocks, free_blocks, free_capacity, free_count, slots, positions,
+                    seq_lens, first_token, max_tokens, info, free_count_out=None, stream=None):
+        """Block tables, slots and positions of a step from the requests' lengths. free_count_out None: free_count is updated in place."""
+        self._check(self.lib.w8a8_plan_blocks(self.handle, _ptr(cached_lens), _ptr(new_lens), batch, _ptr(block_table), max_blocks,
+                                              _ptr(free_blocks), free_capacity, _ptr(free_count),
+                                              _ptr(free_count if free_count_out is None else free_count_out), _ptr(slots), _ptr(positions),
+                                              _ptr(seq_lens), _ptr(first_token), max_tokens, _ptr(info), _stream(stream)), "w8a8_plan_blocks")
+
+    def kv4_write(self, qkv, slots, cache, n_blocks, layer, n_layers, tokens, n_q, n_kv, head_dim, group, q_norm_w=None, k_norm_w=None,
+                  eps=0.0, freqs=None, positions=None, q_out=None, stream=None):
+        self._check(self.lib.w8a8_kv4_write(self.handle, _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), eps, _ptr(freqs), _ptr(positions),
+                                            _ptr(slots), _ptr(cache), n_blocks, layer, n_layers, tokens, n_q, n_kv, head_dim, group,
+                                            _ptr(q_out), _stream(stream)), "w8a8_kv4_write")
+
+    def kv4_read(self, cache, n_blocks, slots, layer, n_layers, tokens, n_kv, head_dim, group, k_out, v_out, stream=None):
+        self._check(self.lib.w8a8_kv4_read(self.handle, _ptr(cache), n_blocks, _ptr(slots), layer, n_layers, tokens, n_kv, head_dim, group,
+                                           _ptr(k_out), _ptr(v_out), _stream(stream)), "w8a8_kv4_read")
+
+    def kv4_attention_decode(self, q, cache, n_blocks, block_table, seq_lens, out, batch, n_heads, head_dim, max_blocks, sm_scale, layer,
+                             n_layers, n_kv, group, quant_group_size=0, Xq=None, Xs=None, stream=None):
+        self._check(self.lib.w8a8_kv4_attention_decode(self.handle, _ptr(q), _ptr(cache), n_blocks, _ptr(block_table), _ptr(seq_lens),
+                                                       _ptr(out), batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers, n_kv,
+                                                       group, quant_group_size, _ptr(Xq), _ptr(Xs), _stream(stream)),
+                    "w8a8_kv4_attention_decode")
+
+    def linear4_q(self, W4, w_scale, group_size, Xq, Xs, Y, M, N, K, epilogue=EPI_NONE, residual=None, stream=None):
+        self._check(self.lib.w8a8_linear4_q(self.handle, _ptr(W4), _ptr(w_scale), group_size, _ptr(Xq), _ptr(Xs), _ptr(Y), M, N, K, epilogue,
+                                            _ptr(residual), _stream(stream)), "w8a8_linear4_q")
+
+    def quantize_weight4(self, W, N, K, group_size, W4, w_scale, stream=None):
+        self._check(self.lib.w8a8_quantize_weight4(self.handle, _ptr(W), N, K, group_size, _ptr(W4), _ptr(w_scale), _stream(stream)),
+                    "w8a8_quantize_weight4")
+
+    def unpack_weight4(self, W4, N, K, W, stream=None):
+        self._check(self.lib.w8a8_unpack_weight4(self.handle, _ptr(W4), N, K, _ptr(W), _stream(stream)), "w8a8_unpack_weight4")
 
     def tp_create(self, rank, world, max_tokens, dim) -> bytes:
         """Allocates this rank's exchange buffer; returns its 64-byte IPC handle."""

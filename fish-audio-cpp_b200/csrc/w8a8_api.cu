@@ -22,7 +22,7 @@ struct w8a8_ctx {
     std::unordered_map<const void*, PackedEntry> packed;
     std::mutex packed_mu;
     short gemm_bt = 0, gemm_splits = 0;  // w8a8_debug_force_gemm_form
-    int* tail_counters = nullptr;     // arrival counters of the decode kernel's tails, zero between launches
+    int* tail_counters = nullptr;     // arrival counters of the decode kernel's tails, then of the 4-bit attention; zero between launches
     w8a8::TpState* tp = nullptr;  // tensor-parallel exchange, when w8a8_tp_create was called
 };
 
@@ -198,8 +198,8 @@ int w8a8_create(w8a8_ctx** out, int device, size_t workspace_bytes) {
     e = cudaMalloc(&c->workspace, c->workspace_bytes);
     if (e == cudaSuccess) e = cudaMalloc(&c->device_status, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(c->device_status, 0, sizeof(int));
-    if (e == cudaSuccess) e = cudaMalloc(&c->tail_counters, kTailCounterInts * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(c->tail_counters, 0, kTailCounterInts * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&c->tail_counters, (kTailCounterInts + kKv4Tickets) * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(c->tail_counters, 0, (kTailCounterInts + kKv4Tickets) * sizeof(int));
     cudaSetDevice(prev);
     if (e != cudaSuccess) {
         cudaFree(c->workspace);
@@ -240,7 +240,7 @@ int w8a8_check_device_status(w8a8_ctx* ctx, void* stream) {
     if (host != 0) {
         cudaMemsetAsync(ctx->device_status, 0, sizeof(int), s);
         // a kernel that gave up may have left arrival counters half-counted
-        cudaMemsetAsync(ctx->tail_counters, 0, kTailCounterInts * sizeof(int), s);
+        cudaMemsetAsync(ctx->tail_counters, 0, (kTailCounterInts + kKv4Tickets) * sizeof(int), s);
         return fail(W8A8_ERR_TIMEOUT, "a kernel gave up a bounded wait (code %d)", host);
     }
     return W8A8_OK;
@@ -530,6 +530,144 @@ int w8a8_qkv_attention_decode_ahead(w8a8_ctx* ctx, const void* qkv, const void* 
     return qkv_attention(ctx, qkv, q_norm_w, k_norm_w, eps, freqs, positions, k_cache, v_cache, block_table, seq_lens, out, batch,
                          n_heads, head_dim, max_blocks_per_seq, sm_scale, layer, n_layers, n_kv_heads, quant_group_size, Xq, Xs,
                          context_splits, true, stream);
+}
+
+// ---- the decode step in 4 bits ----
+// Last of the checks (what is wrong with the arguments is said before the context is looked into): a launch goes to the current device.
+static int check_device(const w8a8_ctx* ctx, const char* what) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != ctx->device)
+        return fail(W8A8_ERR_INVALID_ARG, "%s: the current device is %d, the context's is %d", what, dev, ctx->device);
+    return W8A8_OK;
+}
+
+static int check_kv4(const w8a8_ctx* ctx, const char* what, const void* cache, int n_blocks, int layer, int n_layers, int rows, int n_q, int n_kv,
+                     int head_dim, int group) {
+    if (!ctx) return fail(W8A8_ERR_INVALID_ARG, "null context");
+    if (head_dim != 128) return fail(W8A8_ERR_UNSUPPORTED, "%s: head_dim %d (only 128 is built)", what, head_dim);
+    if (kv4_page_bytes(group) == 0) return fail(W8A8_ERR_UNSUPPORTED, "%s: group size %d (32, 64 and 128 are built)", what, group);
+    if (rows < 0 || n_blocks < 0 || n_layers <= 0 || layer < 0 || layer >= n_layers || n_q < 0 || n_kv <= 0 || n_kv > 65536 || n_q > 65536)
+        return fail(W8A8_ERR_INVALID_ARG, "%s: bad sizes (rows %d, blocks %d, layer %d of %d, heads %d / %d)", what, rows, n_blocks, layer, n_layers,
+                    n_q, n_kv);
+    if (rows > 0 && n_blocks == 0) return fail(W8A8_ERR_INVALID_ARG, "%s: a cache of no blocks", what);
+    if (rows > 0 && (!cache || (reinterpret_cast<uintptr_t>(cache) & 15u)))
+        return fail(W8A8_ERR_INVALID_ARG, "%s: the cache must be there and 16-byte aligned", what);
+    return W8A8_OK;
+}
+
+size_t w8a8_kv4_cache_bytes(int n_blocks, int n_layers, int n_kv_heads, int head_dim, int group_size) {
+    if (n_blocks <= 0 || n_layers <= 0 || n_kv_heads <= 0 || head_dim != 128) return 0;
+    return static_cast<size_t>(n_blocks) * n_layers * n_kv_heads * kv4_page_bytes(group_size);
+}
+
+int w8a8_plan_blocks(w8a8_ctx* ctx, const int* cached_lens, const int* new_lens, int batch, int* block_table, int max_blocks_per_seq,
+                     int* free_blocks, int free_capacity, const int* free_count, int* free_count_out, int64_t* slots, int* positions,
+                     int* seq_lens, int* first_token, int max_tokens, int* info, void* stream) {
+    if (!ctx) return fail(W8A8_ERR_INVALID_ARG, "null context");
+    if (batch < 0 || max_blocks_per_seq <= 0 || free_capacity < 0 || max_tokens < 0)
+        return fail(W8A8_ERR_INVALID_ARG, "plan_blocks: bad sizes (batch %d, table width %d, capacity %d, tokens %d)", batch, max_blocks_per_seq,
+                    free_capacity, max_tokens);
+    if (batch > plan_max_batch()) return fail(W8A8_ERR_UNSUPPORTED, "plan_blocks: batch %d (at most %d)", batch, plan_max_batch());
+    if (!free_count || !free_count_out || !first_token || !info || (free_capacity > 0 && !free_blocks) ||
+        (batch > 0 && (!cached_lens || !new_lens || !block_table || !seq_lens)) || (max_tokens > 0 && (!slots || !positions)))
+        return fail(W8A8_ERR_INVALID_ARG, "plan_blocks: null pointer");
+    if (int rc = check_device(ctx, "plan_blocks")) return rc;
+    return launch_plan_blocks(cached_lens, new_lens, batch, block_table, max_blocks_per_seq, free_blocks, free_capacity, free_count, free_count_out,
+                              reinterpret_cast<long long*>(slots), positions, seq_lens, first_token, max_tokens, info,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int w8a8_kv4_write(w8a8_ctx* ctx, const void* qkv, const void* q_norm_w, const void* k_norm_w, float eps, const float* freqs,
+                   const int* positions, const int64_t* slots, void* cache, int n_blocks, int layer, int n_layers, int tokens, int n_q_heads,
+                   int n_kv_heads, int head_dim, int group_size, void* q_out, void* stream) {
+    if (int rc = check_kv4(ctx, "kv4_write", cache, n_blocks, layer, n_layers, tokens, n_q_heads, n_kv_heads, head_dim, group_size)) return rc;
+    if (tokens > 0 && (!qkv || !slots)) return fail(W8A8_ERR_INVALID_ARG, "kv4_write: null pointer");
+    if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(W8A8_ERR_INVALID_ARG, "kv4_write: q_norm_w and k_norm_w go together");
+    if ((freqs == nullptr) != (positions == nullptr)) return fail(W8A8_ERR_INVALID_ARG, "kv4_write: freqs and positions go together");
+    if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w) |
+         reinterpret_cast<uintptr_t>(q_out)) & 7u)
+        return fail(W8A8_ERR_INVALID_ARG, "kv4_write: qkv, the norm weights and q_out must be 8-byte aligned");
+    if (int rc = check_device(ctx, "kv4_write")) return rc;
+    return launch_kv4_write(static_cast<const __half*>(qkv), static_cast<const __half*>(q_norm_w), static_cast<const __half*>(k_norm_w), eps, freqs,
+                            positions, reinterpret_cast<const long long*>(slots), cache, n_blocks, layer, n_layers, tokens, n_q_heads, n_kv_heads,
+                            group_size, static_cast<__half*>(q_out), static_cast<cudaStream_t>(stream));
+}
+
+int w8a8_kv4_read(w8a8_ctx* ctx, const void* cache, int n_blocks, const int64_t* slots, int layer, int n_layers, int tokens, int n_kv_heads,
+                  int head_dim, int group_size, void* k_out, void* v_out, void* stream) {
+    if (int rc = check_kv4(ctx, "kv4_read", cache, n_blocks, layer, n_layers, tokens, 0, n_kv_heads, head_dim, group_size)) return rc;
+    if (tokens > 0 && (!slots || (!k_out && !v_out))) return fail(W8A8_ERR_INVALID_ARG, "kv4_read: null pointer");
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 7u)
+        return fail(W8A8_ERR_INVALID_ARG, "kv4_read: k_out and v_out must be 8-byte aligned");
+    if (int rc = check_device(ctx, "kv4_read")) return rc;
+    return launch_kv4_read(cache, n_blocks, reinterpret_cast<const long long*>(slots), layer, n_layers, tokens, n_kv_heads, group_size,
+                           static_cast<__half*>(k_out), static_cast<__half*>(v_out), static_cast<cudaStream_t>(stream));
+}
+
+size_t w8a8_kv4_attention_workspace_bytes(int n_heads, int n_kv_heads) {
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8) return 0;
+    return kv4_attention_scratch(n_heads, n_kv_heads);
+}
+
+int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table, const int* seq_lens,
+                              void* out, int batch, int n_heads, int head_dim, int max_blocks_per_seq, float sm_scale, int layer, int n_layers,
+                              int n_kv_heads, int group_size, int quant_group_size, void* Xq, void* Xs, void* stream) {
+    if (int rc = check_kv4(ctx, "kv4_attention_decode", cache, n_blocks, layer, n_layers, batch, n_heads, n_kv_heads, head_dim, group_size)) return rc;
+    if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8)
+        return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: %d query heads over %d kv heads (1 to 8 each are built)", n_heads, n_kv_heads);
+    if (max_blocks_per_seq <= 0 || max_blocks_per_seq > (1 << 27) / n_kv_heads || (batch > 0 && max_blocks_per_seq > (1 << 30) / batch))
+        return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: a table of %d x %d blocks", batch, max_blocks_per_seq);
+    if (batch > kv4_max_batch()) return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: batch %d (at most %d)", batch, kv4_max_batch());
+    if (batch > 0 && (!q || !block_table || !seq_lens || (!out && !Xq))) return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: null pointer");
+    if ((Xq == nullptr) != (Xs == nullptr)) return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: Xq and Xs go together");
+    const int row = n_heads / n_kv_heads * head_dim;
+    if (Xq && (quant_group_size < 4 || (quant_group_size & (quant_group_size - 1)) || row % quant_group_size != 0))
+        return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: output codes in groups of %d (a power of two, 4 or more, dividing %d)", quant_group_size, row);
+    if ((reinterpret_cast<uintptr_t>(q) & 15u) || (reinterpret_cast<uintptr_t>(out) & 7u) || (reinterpret_cast<uintptr_t>(Xq) & 3u))
+        return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: q must be 16-byte, out 8-byte and Xq 4-byte aligned");
+    if (int rc = check_device(ctx, "kv4_attention_decode")) return rc;
+    const size_t need = kv4_attention_scratch(n_heads, n_kv_heads);
+    if (need > ctx->workspace_bytes) return fail(W8A8_ERR_WORKSPACE, "need %zu bytes of scratch, context has %zu", need, ctx->workspace_bytes);
+    return launch_kv4_attention(static_cast<const __half*>(q), cache, n_blocks, block_table, seq_lens, static_cast<__half*>(out), batch, n_heads,
+                                n_kv_heads, max_blocks_per_seq, sm_scale, layer, n_layers, group_size, quant_group_size, static_cast<int8_t*>(Xq),
+                                static_cast<float*>(Xs), reinterpret_cast<float*>(ctx->workspace), ctx->tail_counters + kTailCounterInts,
+                                ctx->device_status, static_cast<cudaStream_t>(stream));
+}
+
+static int check_weight4(const w8a8_ctx* ctx, const char* what, int N, int K, int group_size) {
+    if (!ctx) return fail(W8A8_ERR_INVALID_ARG, "null context");
+    if (N <= 0 || K <= 0) return fail(W8A8_ERR_INVALID_ARG, "%s: bad shape N=%d K=%d", what, N, K);
+    if (K % 2 != 0 || K > (1 << 20) || (norm_group(K, group_size) % 2 != 0))
+        return fail(W8A8_ERR_UNSUPPORTED, "%s: K=%d in groups of %d (both even, K at most 2^20)", what, K, norm_group(K, group_size));
+    return W8A8_OK;
+}
+
+int w8a8_linear4_q(w8a8_ctx* ctx, const void* W4, const void* w_scale, int group_size, const void* Xq, const void* Xs, void* Y, int M, int N,
+                   int K, int epilogue, const void* residual, void* stream) {
+    if (int rc = check_weight4(ctx, "linear4_q", N, K, group_size)) return rc;
+    if (M < 0) return fail(W8A8_ERR_INVALID_ARG, "linear4_q: bad shape M=%d", M);
+    if (epilogue < W8A8_EPI_NONE || epilogue > W8A8_EPI_SWIGLU) return fail(W8A8_ERR_INVALID_ARG, "unknown epilogue %d", epilogue);
+    if ((epilogue == W8A8_EPI_RESIDUAL) != (residual != nullptr) && M > 0)
+        return fail(W8A8_ERR_INVALID_ARG, "linear4_q: W8A8_EPI_RESIDUAL and a residual go together");
+    if (epilogue == W8A8_EPI_SWIGLU && N % 16 != 0) return fail(W8A8_ERR_INVALID_ARG, "W8A8_EPI_SWIGLU needs N %% 16 == 0 (got %d)", N);
+    if (M > 0 && (!W4 || !w_scale || !Xq || !Xs || !Y)) return fail(W8A8_ERR_INVALID_ARG, "linear4_q: null pointer");
+    if (int rc = check_device(ctx, "linear4_q")) return rc;
+    return launch_linear4(W4, static_cast<const __half*>(w_scale), group_size, static_cast<const int8_t*>(Xq), static_cast<const float*>(Xs),
+                          static_cast<__half*>(Y), static_cast<const __half*>(residual), M, N, K, epilogue, static_cast<cudaStream_t>(stream));
+}
+
+int w8a8_quantize_weight4(w8a8_ctx* ctx, const void* W, int N, int K, int group_size, void* W4, void* w_scale, void* stream) {
+    if (int rc = check_weight4(ctx, "quantize_weight4", N, K, group_size)) return rc;
+    if (!W || !W4 || !w_scale) return fail(W8A8_ERR_INVALID_ARG, "quantize_weight4: null pointer");
+    if (int rc = check_device(ctx, "quantize_weight4")) return rc;
+    return launch_quantize_weight4(static_cast<const __half*>(W), N, K, group_size, W4, static_cast<__half*>(w_scale), static_cast<cudaStream_t>(stream));
+}
+
+int w8a8_unpack_weight4(w8a8_ctx* ctx, const void* W4, int N, int K, void* W, void* stream) {
+    if (int rc = check_weight4(ctx, "unpack_weight4", N, K, 0)) return rc;
+    if (!W || !W4 || (reinterpret_cast<uintptr_t>(W) & 1u)) return fail(W8A8_ERR_INVALID_ARG, "unpack_weight4: W4 and W must be there, W 2-byte aligned");
+    if (int rc = check_device(ctx, "unpack_weight4")) return rc;
+    return launch_unpack_weight4(W4, N, K, W, static_cast<cudaStream_t>(stream));
 }
 
 size_t w8a8_decode_stack_workspace_bytes(const w8a8_decode_stack* stack) {

@@ -166,6 +166,30 @@ int launch_qkv_attention_decode(const __half* qkv, const __half* q_norm_w, const
                                 const int* block_table, const int* seq_lens, int B, int n_q, int n_kv, int max_blocks,
                                 float sm_scale, int layer, int n_layers, __half* out, int g, int8_t* Xq, float* Xs,
                                 int splits, bool ahead, int* status, cudaStream_t stream);
+// w8a8_plan.cu : block tables, slot maps and positions from request lengths.
+int plan_max_batch();
+int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* table, int max_blocks, int* free_blocks, int capacity,
+                       const int* free_count, int* free_count_out, long long* slots, int* positions, int* seq_lens, int* first_token,
+                       int max_tokens, int* info, cudaStream_t stream);
+// w8a8_kv4_store.cu : rows of the qkv projection into the 4-bit cache, and back.
+size_t kv4_page_bytes(int group);  // 0: no such group size
+int launch_kv4_write(const __half* qkv, const __half* q_norm_w, const __half* k_norm_w, float eps, const float* freqs, const int* positions,
+                     const long long* slots, void* cache, int n_blocks, int layer, int n_layers, int tokens, int n_q, int n_kv, int group,
+                     __half* q_out, cudaStream_t stream);
+int launch_kv4_read(const void* cache, int n_blocks, const long long* slots, int layer, int n_layers, int tokens, int n_kv, int group,
+                    __half* k_out, __half* v_out, cudaStream_t stream);
+// w8a8_kv4_attn.cu : decode attention over the 4-bit cache.
+constexpr int kKv4Tickets = 512;  // one per CTA
+int kv4_max_batch();
+size_t kv4_attention_scratch(int n_q, int n_kv);
+int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const int* table, const int* lens, __half* out, int batch, int n_q,
+                         int n_kv, int max_blocks, float sm_scale, int layer, int n_layers, int group, int g, int8_t* Xq, float* Xs,
+                         float* scratch, int* tickets, int* status, cudaStream_t stream);
+// w8a8_linear4.cu : few rows of activation codes times 4-bit weights.
+int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t* Xq, const float* Xs, __half* Y, const __half* residual, int M, int N,
+                   int K, int epilogue, cudaStream_t stream);
+int launch_quantize_weight4(const __half* W, int N, int K, int group, void* codes, __half* scale, cudaStream_t stream);
+int launch_unpack_weight4(const void* codes, int N, int K, void* W, cudaStream_t stream);
 // w8a8_decode_stack.cu : a whole decode step as one persistent cooperative kernel.
 size_t decode_stack_workspace_bytes(const w8a8_decode_stack& d);
 int launch_decode_stack(const w8a8_decode_stack& d, unsigned char* workspace, size_t workspace_bytes, int* status, cudaStream_t stream);

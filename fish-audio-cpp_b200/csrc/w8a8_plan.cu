@@ -1,0 +1,242 @@
+// The step plan: block tables, slot maps and positions of a ragged batch, made on the GPU from the requests' lengths, with the
+// paged cache's blocks taken from and given back to a stack of free block numbers. Takes the place of the reference's host free list and
+// block-table upload (src/engine/block_manager.cc, src/engine/scheduler.cc), and of the host copy of the table in its decode step
+// (src/engine/dual_ar_engine.cc:568-571).
+//
+// With have_b = ceil(cached_b / 16), over requests in order:
+//   ended (new_b < 0): its have_b blocks go on the stack, give_b = have_b
+//   others: take_b = ceil((cached_b + new_b) / 16) - have_b blocks come from the stack's top (after all that was given back)
+//   token i of request b has the position cached_b + i and the slot 16 * table[b][position / 16] + position % 16
+// Three exclusive prefix sums (tokens, blocks taken, blocks given) make every one of these independent of the others.
+//
+// Bound: latency at decode sizes (one round trip for the lengths, one for block numbers), 12 bytes written per token for prompts. One
+// launch: a CTA, or a cluster of eight for many tokens, whose CTAs all make the same sums and share the tokens; the barriers of the
+// cluster separate "read the old lengths, push" from "pop, write". All or nothing: where the blocks, the table's width, the token
+// count or a length do not fit, no request gets anything, and `info` says why.
+#include "sm100_ptx.cuh"
+#include "w8a8_internal.h"
+
+namespace w8a8 {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBlock = 16;
+constexpr int kPlanMaxBatch = 4096;
+
+struct PlanParams {
+    const int* cached;
+    const int* fresh;
+    int batch;
+    int* table;
+    int max_blocks;
+    int* free_blocks;
+    int capacity;
+    const int* free_count;
+    int* free_count_out;
+    long long* slots;
+    int* positions;
+    int* seq_lens;
+    int* first_token;
+    int max_tokens;
+    int* info;
+    int vector_stores;  // slots and positions are 16-byte aligned
+};
+
+struct Sums {
+    long long tokens, take, give;
+};
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.tokens + b.tokens, a.take + b.take, a.give + b.give}; }
+__device__ __forceinline__ Sums shfl_up(Sums v, int d) {
+    return {__shfl_up_sync(0xffffffffu, v.tokens, d), __shfl_up_sync(0xffffffffu, v.take, d), __shfl_up_sync(0xffffffffu, v.give, d)};
+}
+
+__device__ __forceinline__ void plan_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanParams p) {
+    extern __shared__ int plan_smem[];
+    int* first_s = plan_smem;                      // [batch + 1] tokens ahead of request b
+    int* take_s = first_s + p.batch + 1;           // [batch] blocks taken ahead of it
+    int* give_s = take_s + p.batch;                // [batch] blocks given back ahead of it
+    int* cached_s = give_s + p.batch;              // [batch]; minus one minus the length where the request ended
+    __shared__ Sums warp_s[kPlanThreads / 32];
+    __shared__ Sums run_s;
+    __shared__ int bad_s;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = blockIdx.x, parts = gridDim.x;
+    ptx::pdl_wait();
+    ptx::pdl_launch_dependents();
+    const long long count = *p.free_count;
+    if (tid == 0) {
+        run_s = {0, 0, 0};
+        bad_s = 8;  // the lowest status found (5 comes before all); 8: none
+    }
+    __syncthreads();
+    for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+        const int b = b0 + tid;
+        Sums mine = {0, 0, 0};
+        int cached = 0;
+        bool ended = false;
+        if (b < p.batch) {
+            cached = p.cached[b];
+            const int fresh = p.fresh[b];
+            ended = fresh < 0;
+            if (cached < 0) {
+                atomicMin(&bad_s, 4);
+                cached = 0;
+            }
+            const long long have = (static_cast<long long>(cached) + kPlanBlock - 1) / kPlanBlock;
+            const long long all = ended ? have : (static_cast<long long>(cached) + fresh + kPlanBlock - 1) / kPlanBlock;
+            if (all > p.max_blocks) atomicMin(&bad_s, 2);
+            mine = {ended ? 0 : fresh, all - have, ended ? have : 0};
+        }
+        Sums inc = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const Sums o = shfl_up(inc, d);
+            if (lane >= d) inc = inc + o;
+        }
+        if (lane == 31) warp_s[warp] = inc;
+        __syncthreads();
+        const Sums base = run_s;
+        if (warp == 0) {
+            Sums w = warp_s[lane];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const Sums o = shfl_up(w, d);
+                if (lane >= d) w = w + o;
+            }
+            warp_s[lane] = w;
+        }
+        __syncthreads();
+        Sums at = base + inc;
+        if (warp > 0) at = at + warp_s[warp - 1];
+        if (b < p.batch) {  // (numbers that do not fit 32 bits belong to a plan that is refused below)
+            first_s[b + 1] = static_cast<int>(at.tokens);
+            take_s[b] = static_cast<int>(at.take - mine.take);
+            give_s[b] = static_cast<int>(at.give - mine.give);
+            cached_s[b] = ended ? -1 - cached : cached;
+        }
+        if (tid == 0) run_s = base + warp_s[kPlanThreads / 32 - 1];
+        __syncthreads();
+    }
+    if (tid == 0) first_s[0] = 0;
+    const Sums all = run_s;
+    const long long top = count + all.give;
+    int status = bad_s;
+    if (all.tokens > p.max_tokens) status = min(status, 3);
+    if (all.take > top) status = min(status, 1);
+    if (count < 0 || top > p.capacity) status = 5;
+    const bool ok = status == 8;
+
+    // blocks of requests that ended go on the stack; a warp a request
+    if (ok && all.give > 0)
+        for (int b = part * (kPlanThreads / 32) + warp; b < p.batch; b += parts * (kPlanThreads / 32)) {
+            const int cached = -1 - cached_s[b];
+            if (cached < 0) continue;
+            const int have = (cached + kPlanBlock - 1) / kPlanBlock;
+            for (int j = lane; j < have; j += 32)
+                p.free_blocks[count + give_s[b] + j] = p.table[static_cast<size_t>(b) * p.max_blocks + j];
+        }
+    // all inputs that an output may replace are read, all pushes are there
+    __syncthreads();
+    plan_cluster_sync();
+
+    const int threads = parts * kPlanThreads, me = part * kPlanThreads + tid;
+    for (int b = part * (kPlanThreads / 32) + warp; b < p.batch; b += parts * (kPlanThreads / 32)) {
+        const int cached = cached_s[b];
+        const int fresh = first_s[b + 1] - first_s[b];
+        if (lane == 0) {
+            p.seq_lens[b] = !ok ? max(0, cached < 0 ? -1 - cached : cached) : cached < 0 ? 0 : cached + fresh;
+            p.first_token[b + 1] = ok ? first_s[b + 1] : 0;
+        }
+        if (ok && cached >= 0) {
+            const int have = (cached + kPlanBlock - 1) / kPlanBlock, end = (cached + fresh + kPlanBlock - 1) / kPlanBlock;
+            for (int j = have + lane; j < end; j += 32)
+                p.table[static_cast<size_t>(b) * p.max_blocks + j] = __ldcg(p.free_blocks + (top - 1 - (take_s[b] + j - have)));
+        }
+    }
+    if (me == 0) {
+        p.first_token[0] = 0;
+        p.info[0] = ok ? 0 : status;
+        p.info[1] = ok ? static_cast<int>(all.tokens) : 0;
+        p.info[2] = ok ? static_cast<int>(all.take) : 0;
+        p.info[3] = static_cast<int>(ok ? top - all.take : count);
+        *p.free_count_out = static_cast<int>(ok ? top - all.take : count);
+    }
+    // four tokens a thread: one search, then forward
+    const int tokens = ok ? static_cast<int>(all.tokens) : 0;
+    for (long long t0 = 4ll * me; t0 < p.max_tokens; t0 += 4ll * threads) {
+        long long slot[4] = {-1, -1, -1, -1};
+        int pos[4] = {0, 0, 0, 0};
+        if (t0 < tokens) {
+            int lo = 0, hi = p.batch - 1;  // the last request whose first token is not behind t0
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (first_s[mid] <= t0) lo = mid; else hi = mid - 1;
+            }
+            int b = lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = static_cast<int>(t0) + e;
+                if (t < tokens) {
+                    while (first_s[b + 1] <= t) ++b;
+                    const int cached = cached_s[b], have = (cached + kPlanBlock - 1) / kPlanBlock;
+                    pos[e] = cached + t - first_s[b];
+                    const int blk = pos[e] / kPlanBlock;
+                    const int phys = blk >= have ? __ldcg(p.free_blocks + (top - 1 - (take_s[b] + blk - have)))
+                                                 : __ldcg(p.table + static_cast<size_t>(b) * p.max_blocks + blk);
+                    slot[e] = phys < 0 ? -1 : static_cast<long long>(phys) * kPlanBlock + pos[e] % kPlanBlock;
+                }
+            }
+        }
+        if (p.vector_stores && t0 + 4 <= p.max_tokens) {
+            reinterpret_cast<longlong2*>(p.slots + t0)[0] = make_longlong2(slot[0], slot[1]);
+            reinterpret_cast<longlong2*>(p.slots + t0)[1] = make_longlong2(slot[2], slot[3]);
+            *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+            for (int e = 0; e < 4 && t0 + e < p.max_tokens; ++e) {
+                p.slots[t0 + e] = slot[e];
+                p.positions[t0 + e] = pos[e];
+            }
+        }
+    }
+}
+
+SmemAttribute plan_attribute;
+constexpr int kPlanSmem = (4 * kPlanMaxBatch + 1) * 4;
+
+}  // namespace
+
+int plan_max_batch() { return kPlanMaxBatch; }
+
+int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* table, int max_blocks, int* free_blocks, int capacity,
+                       const int* free_count, int* free_count_out, long long* slots, int* positions, int* seq_lens, int* first_token,
+                       int max_tokens, int* info, cudaStream_t stream) {
+    PlanParams p = {cached, fresh, batch, table, max_blocks, free_blocks, capacity, free_count, free_count_out, slots, positions,
+                    seq_lens, first_token, max_tokens, info,
+                    ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) & 15u) == 0};
+    const int parts = max_tokens > 4 * kPlanThreads || batch > kPlanThreads ? 8 : 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(parts, 1, 1);
+    cfg.blockDim = dim3(kPlanThreads, 1, 1);
+    cfg.dynamicSmemBytes = (4 * batch + 1) * 4;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled(kPdlRow) ? 2 : 1;
+    const cudaError_t e = launch_with_smem(plan_attribute, kPlanSmem, cfg, plan_blocks_kernel, p);
+    if (e != cudaSuccess) return fail(W8A8_ERR_CUDA, "plan_blocks launch: %s", cudaGetErrorString(e));
+    return W8A8_OK;
+}
+
+}  // namespace w8a8

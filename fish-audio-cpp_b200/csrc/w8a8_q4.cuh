@@ -1,0 +1,60 @@
+// What a 4-bit group is, shared by the KV cache and the weights, and the layout of a page of the 4-bit cache.
+//
+// A group is g consecutive fp16 values x. e is the one of largest magnitude (the positive one where +e and -e are both there),
+// s = fp16(e / -8), code = rint(x / s) held to [-8, 7] (half to even; 0 where s is 0), the value it stands for is code * s. The sixteen
+// codes are all used, and e itself is held exactly (e / -8 is exact but where it is subnormal). A group that holds an infinity or a NaN
+// has the scale NaN and codes 0: it reads as NaN throughout, nothing that is not a number turns into one.
+//
+// x has 11 significant bits and (k + 1/2) s at most 15, so x / s is either a tie exactly or at least 2^-16 away from one, relatively: any
+// quotient that is exact at ties and within 2^-20 elsewhere gives the same codes as 64 bits do.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace w8a8 {
+namespace q4 {
+
+// The extremes of a group travel as (max x, max -x): both are maxima that propagate NaN.
+__device__ __forceinline__ __half2 extremes(__half a, __half b) {
+    const __half2 v = __halves2half2(a, b), n = __hneg2(v);
+    return __halves2half2(__hmax_nan(__low2half(v), __high2half(v)), __hmax_nan(__low2half(n), __high2half(n)));
+}
+
+struct Scale {
+    __half s;      // as stored
+    float f, inv;  // s, and 1 / s to within a few ulp; 0 where every code is 0
+    __device__ __forceinline__ explicit Scale(__half2 mx) {
+        const float hi = __low2float(mx), neg_lo = __high2float(mx);
+        s = __float2half_rn((hi >= neg_lo ? hi : -neg_lo) * -0.125f);
+        if (!(fmaxf(fabsf(hi), fabsf(neg_lo)) < INFINITY) || isnan(hi) || isnan(neg_lo)) s = __ushort_as_half(0x7fffu);
+        f = __half2float(s);
+        inv = (f == 0.0f || isnan(f)) ? 0.0f : __frcp_rn(f);
+    }
+    // One correction by the residual: exact where the quotient is a number of few bits, a tie above all (q * f has 24 bits at most there).
+    __device__ __forceinline__ int code(__half x) const {
+        if (inv == 0.0f) return 0;
+        const float v = __half2float(x), q = v * inv;
+        return max(-8, min(7, __float2int_rn(fmaf(fmaf(-q, f, v), inv, q))));
+    }
+};
+
+// ---- a page of the cache: 16 tokens of one (layer, kv head), 128 channels ----
+//   [0, 1024)       K codes: token t at 64 t; in it 16 bytes for each quarter j of eight channels of every 32-channel run: the word
+//                   16 j + 4 run holds channels 32 run + 8 j + n as nibbles n = 0 .. 7 (low first)
+//   [1024, 2048)    V codes: pair of tokens p at 128 p; unit r = 0 .. 7 of 16 bytes; the word 8 half + 4 high of it holds channels
+//                   64 high + 16 n + 8 half + r, n = 0 .. 3, of token 2 p as nibbles 0 .. 3 and of token 2 p + 1 as nibbles 4 .. 7
+//   [2048, + 32 G)  K scales fp16, G = 128 / group: [pair of tokens][group][token of the pair]
+//   [.., + 32 G)    V scales, the same
+// Codes are stored plus 8. The orders are those in which a lane's 16-byte read holds what it feeds to the matrix instructions, with no
+// exchange between lanes: eight channels of one token for q K^T, four channels by two tokens for P V (the contraction runs over tokens).
+constexpr int kTokens = 16, kDim = 128;
+constexpr int kVOff = kTokens * kDim / 2, kScaleOff = 2 * kVOff;
+__host__ __device__ constexpr int page_bytes(int groups) { return kScaleOff + 4 * kTokens * groups; }
+__host__ __device__ __forceinline__ constexpr int scale_off(int groups, int is_v, int token, int group) {
+    return kScaleOff + is_v * 2 * kTokens * groups + (((token >> 1) * groups + group) * 2 + (token & 1)) * 2;
+}
+
+}  // namespace q4
+}  // namespace w8a8

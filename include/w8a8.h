@@ -299,6 +299,83 @@ W8A8_API int w8a8_qkv_attention_decode_ahead(w8a8_ctx* ctx, const void* qkv, con
                                     float sm_scale, int layer, int n_layers, int n_kv_heads, int quant_group_size,
                                     void* Xq, void* Xs, int context_splits, void* stream);
 
+/* ---- the decode step in 4 bits, over ragged batches (no counterpart in the reference) -------------------- */
+
+/* A 4-bit GROUP is g consecutive fp16 values x. e is the one of largest magnitude (the positive one where +e and -e are both
+ * there); the scale is s = fp16(e / -8); a code is rint(x / s) held to [-8, 7], half to even (0 where s is 0); the value that it
+ * stands for is code * s. A group that holds an infinity or a NaN reads as NaN throughout. */
+
+/* The plan of a step: what the reference does with a free list on the host and an upload of the block table (src/engine/
+ * block_manager.cc, src/engine/scheduler.cc, src/engine/dual_ar_engine.cc:568-571), made on the GPU from the requests' lengths.
+ *   cached_lens int32 [batch]  tokens that a request has in the cache
+ *   new_lens    int32 [batch]  tokens that this step adds to it (0: none); negative: the request has ended
+ *   block_table int32 [batch, max_blocks_per_seq]  in: the blocks of the cached tokens; the blocks taken are added behind them
+ *   free_blocks int32 [free_capacity]  a stack of free block numbers, free_count (on the device) of them; blocks of ended requests
+ *               are pushed in request order, then blocks are taken from the top in request order. free_count_out receives what is left
+ *               (it may be free_count itself)
+ *   slots       int64 [max_tokens]  of every new token, requests in order: 16 * block + place in the block; -1 behind the last
+ *   positions   int32 [max_tokens]  of every new token; 0 behind the last
+ *   seq_lens    int32 [batch]  cached + new, 0 where ended (it may be cached_lens itself)
+ *   first_token int32 [batch + 1]  index of a request's first new token
+ *   info        int32 [4]  {status, new tokens, blocks taken, blocks left}
+ * All or nothing. Where status is not 0, no table row and no free block has changed, every slot is -1, first_token is 0 and seq_lens holds
+ * the cached lengths (an ended request's too): 5 free_count out of range (with what is given back); else the lowest of 1 not enough free
+ * blocks, 2 a request longer than its table row, 3 more than max_tokens new tokens, 4 a negative cached length (taken as 0). Rows of ended requests are left as they were.
+ * batch <= 4096. One launch. */
+W8A8_API int w8a8_plan_blocks(w8a8_ctx* ctx, const int* cached_lens, const int* new_lens, int batch, int* block_table,
+                     int max_blocks_per_seq, int* free_blocks, int free_capacity, const int* free_count, int* free_count_out,
+                     int64_t* slots, int* positions, int* seq_lens, int* first_token, int max_tokens, int* info,
+                     void* stream);
+
+/* The paged cache in 4 bits: pages [blocks, n_layers, n_kv] of 16 tokens of one kv head, K and V with their scales in one page:
+ * 2048 + 64 * (128 / group) bytes, group = 32, 64 or 128 channels (the fp16 cache's are 8192). Layout of a page, codes plus 8:
+ *   [0, 1024)     K: token t at 64 t; the 32-bit word 4 j + run of it holds channels 32 run + 8 j + n as nibbles n = 0 .. 7, low first
+ *   [1024, 2048)  V: tokens 2 p and 2 p + 1 at 128 p; the word 4 r + 2 half + high holds channels 64 high + 16 n + 8 half + r,
+ *                 n = 0 .. 3, of token 2 p as nibbles 0 .. 3 and of token 2 p + 1 as nibbles 4 .. 7
+ *   then fp16 scales of K [8 pairs of tokens][128 / group][2], and of V the same
+ * The buffer is 16-byte aligned and w8a8_kv4_cache_bytes long (0: bad arguments); it needs no initialisation. */
+W8A8_API size_t w8a8_kv4_cache_bytes(int n_blocks, int n_layers, int n_kv_heads, int head_dim, int group_size);
+
+/* w8a8_qknorm_rope_kvwrite for this cache, tokens named by slots (w8a8_plan_blocks): a prompt's rows as well as a decode step's. qkv
+ * fp16 [tokens, (n_q + 2 n_kv) * head_dim]; q_norm_w and k_norm_w both or neither; freqs and positions both or neither (no
+ * rotation). q_out fp16 [tokens, n_q, head_dim] or NULL; the fp16 q, k and v are bit-identical to that call's, k and v are then held
+ * in 4 bits. A token whose slot is negative or outside the cache (n_blocks * 16 slots) is left out, its row of q_out too. Two tokens of one call must
+ * not have the same slot. */
+W8A8_API int w8a8_kv4_write(w8a8_ctx* ctx, const void* qkv, const void* q_norm_w, const void* k_norm_w, float eps,
+                   const float* freqs, const int* positions, const int64_t* slots, void* cache, int n_blocks, int layer,
+                   int n_layers, int tokens, int n_q_heads, int n_kv_heads, int head_dim, int group_size, void* q_out,
+                   void* stream);
+
+/* The values that listed slots stand for, rounded to fp16: k_out, v_out [tokens, n_kv, head_dim] (one of them may be NULL), e.g. for a prompt that
+ * continues a cached prefix. Rows whose slot is negative or outside the cache are left as they were. */
+W8A8_API int w8a8_kv4_read(w8a8_ctx* ctx, const void* cache, int n_blocks, const int64_t* slots, int layer, int n_layers,
+                  int tokens, int n_kv_heads, int head_dim, int group_size, void* k_out, void* v_out, void* stream);
+
+/* w8a8_paged_attention_decode over this cache: q fp16 [batch, n_heads, head_dim], 1 to 8 query heads per kv head, batch <= 4096, any
+ * mix of lengths (a row of length 0 gives zeros). Lengths are cut at 16 * max_blocks_per_seq; a block number outside the cache reads
+ * block 0. out fp16 [batch, n_heads, head_dim] and / or its codes Xq and scales Xs as there, quant_group_size a power of two from 4 up
+ * that divides (n_heads / n_kv_heads) * head_dim. Sums are fp32; softmax weights and code * scale of V are rounded to fp16. Results do
+ * not depend on timing. Needs w8a8_kv4_attention_workspace_bytes of the context's workspace. */
+W8A8_API size_t w8a8_kv4_attention_workspace_bytes(int n_heads, int n_kv_heads);
+W8A8_API int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table,
+                              const int* seq_lens, void* out, int batch, int n_heads, int head_dim,
+                              int max_blocks_per_seq, float sm_scale, int layer, int n_layers, int n_kv_heads,
+                              int group_size, int quant_group_size, void* Xq, void* Xs, void* stream);
+
+/* w8a8_linear_q over 4-bit weights: W4 uint8 [N, K / 2], row-major, two codes a byte as two's complement, the even k in the low four
+ * bits; w_scale fp16 [N, G] (4-bit groups along K); Xq, Xs as there. Per group an exact int32 sum, promoted with both scales in
+ * fp32. epilogue W8A8_EPI_*, residual fp16 [M, N] with W8A8_EPI_RESIDUAL only (may alias Y); for W8A8_EPI_SWIGLU the rows are interleaved
+ * by w8a8_pack_gate_up, called with K / 2 in place of K. K and the group size are even. Built for a few rows: the weights are streamed
+ * once per 32 rows; longer prompts run w8a8_linear_q over what w8a8_unpack_weight4 makes, with the same scales. The fast kernel takes
+ * K and group sizes that are multiples of 32 with W4 and Xq 16-byte aligned, everything else a generic one. */
+W8A8_API int w8a8_linear4_q(w8a8_ctx* ctx, const void* W4, const void* w_scale, int group_size, const void* Xq, const void* Xs,
+                   void* Y, int M, int N, int K, int epilogue, const void* residual, void* stream);
+/* Loader side: fp16 weights [N, K] to W4 and w_scale; and W4 to int8 codes [N, K], which with the same scales are a weight of
+ * w8a8_linear_q, w8a8_pack_weight and the rest. */
+W8A8_API int w8a8_quantize_weight4(w8a8_ctx* ctx, const void* W, int N, int K, int group_size, void* W4, void* w_scale,
+                          void* stream);
+W8A8_API int w8a8_unpack_weight4(w8a8_ctx* ctx, const void* W4, int N, int K, void* W, void* stream);
+
 /* ---- one decode step of the whole stack as one launch ------------------------------------------ */
 
 typedef struct w8a8_decode_layer {
