@@ -549,6 +549,8 @@ static int check_kv4(const w8a8_ctx* ctx, const char* what, const void* cache, i
     if (rows < 0 || n_blocks < 0 || n_layers <= 0 || layer < 0 || layer >= n_layers || n_q < 0 || n_kv <= 0 || n_kv > 65536 || n_q > 65536)
         return fail(W8A8_ERR_INVALID_ARG, "%s: bad sizes (rows %d, blocks %d, layer %d of %d, heads %d / %d)", what, rows, n_blocks, layer, n_layers,
                     n_q, n_kv);
+    if (rows > 0 && static_cast<long long>(n_blocks) * n_layers > 0x7fffffffll / n_kv)
+        return fail(W8A8_ERR_UNSUPPORTED, "%s: %d x %d x %d pages (fewer than 2^31 are built)", what, n_blocks, n_layers, n_kv);
     if (rows > 0 && n_blocks == 0) return fail(W8A8_ERR_INVALID_ARG, "%s: a cache of no blocks", what);
     if (rows > 0 && (!cache || (reinterpret_cast<uintptr_t>(cache) & 15u)))
         return fail(W8A8_ERR_INVALID_ARG, "%s: the cache must be there and 16-byte aligned", what);
@@ -615,7 +617,7 @@ int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, i
     if (int rc = check_kv4(ctx, "kv4_attention_decode", cache, n_blocks, layer, n_layers, batch, n_heads, n_kv_heads, head_dim, group_size)) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8)
         return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: %d query heads over %d kv heads (1 to 8 each are built)", n_heads, n_kv_heads);
-    if (max_blocks_per_seq <= 0 || max_blocks_per_seq > (1 << 27) / n_kv_heads || (batch > 0 && max_blocks_per_seq > (1 << 30) / batch))
+    if (max_blocks_per_seq <= 0 || max_blocks_per_seq > (1 << 26) / n_kv_heads || (batch > 0 && max_blocks_per_seq > (1 << 30) / batch))
         return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: a table of %d x %d blocks", batch, max_blocks_per_seq);
     if (batch > kv4_max_batch()) return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: batch %d (at most %d)", batch, kv4_max_batch());
     if (batch > 0 && (!q || !block_table || !seq_lens || (!out && !Xq))) return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: null pointer");

@@ -16,10 +16,12 @@
 // A warp streams its run through a ring of its own: one bulk copy per page, issued by a lane kStages ahead, across the borders of
 // pairs; nothing in the steady state synchronises warps.
 //
-// Arithmetic. Codes become fp16 numbers by placing the four bits in the significand of 1024 (or, four bits further up, of 1024 in
-// sixteenths) and taking that off: two values per instruction, exact. Scores: q (fp16) times codes, fp32 sums per group, times the
-// group's scale in fp32. P V: p is rounded to fp16 (2^-11 relative; the denominator sums the rounded values), code * scale is rounded
-// to fp16 (2^-11 relative, the values that w8a8_kv4_read returns), products are summed in fp32.
+// Arithmetic. Scores: a masked nibble is, as the bits of an fp16 number, the subnormal code * 2^-24 (or, four bits up, code * 2^-20, which
+// meets a q that was divided by 16), exact as a matrix operand: one instruction for two codes. The 8 that stored codes carry leaves with the
+// accumulator's start, -8 * sum of q over the group. Sums are fp32 per group, times the group's scale in fp32. P V: codes as fp16 numbers
+// (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p is rounded to fp16 (2^-11
+// relative, and the denominator sums the rounded values); products are summed in fp32. The reference of the exponentials is a score of the
+// row that others exceed by at most 2^kLag, so that it moves, and the sums with it, a few times per row only.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 #include "w8a8_q4.cuh"
@@ -32,6 +34,7 @@ using q4::kTokens;
 
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
+constexpr float kLag = 8.0f;  // p is at most 2^8: it keeps its precision in fp16
 
 struct Kv4Params {
     const __half* q;  // [batch, n_q, 128]
@@ -43,7 +46,7 @@ struct Kv4Params {
     float* Xs;    // [batch, n_q * 128 / g]
     int g;
     int batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers;
-    float scale_log2;  // sm_scale * log2(e)
+    float scale_log2;  // sm_scale * log2(e) * 2^24: the scores' codes come as 2^-24 of themselves
     int min_units;     // pages a warp takes at least
     float* scratch;    // [CTAs][2] pieces
     int* tickets;      // [CTAs], zero between launches
@@ -59,7 +62,15 @@ __device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
-// The eight biased codes of a word as four fp16 pairs: nibbles (0, 4), (1, 5), (2, 6), (3, 7).
+// The eight stored codes (code + 8) of a word as fp16 pairs, nibbles (0, 4), (1, 5), (2, 6), (3, 7): times 2^-24, 2^-20, 2^-24, 2^-20.
+__device__ __forceinline__ void unpack8_tiny(uint32_t w, uint32_t (&h)[4]) {
+    const uint32_t up = w >> 8;
+    h[0] = w & 0x000f000fu;
+    h[1] = w & 0x00f000f0u;
+    h[2] = up & 0x000f000fu;
+    h[3] = up & 0x00f000f0u;
+}
+// The eight codes themselves.
 __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&h)[4]) {
     const __half2 off = as_half2(0x64086408u);                                        // 1024 + 8
     const __half2 sixteenth = as_half2(0x2c002c00u), off16 = as_half2(0xd480d480u);  // 1 / 16; -(64 + 8)
@@ -75,6 +86,18 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same into d from c, which stays.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// Element (row, col) of an 8 x 8 matrix of 16-bit numbers goes to (col, row): lane 4 row + j holds columns 2 j, 2 j + 1.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
@@ -99,7 +122,7 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
 // A piece: the state of a softmax over part of a pair's pages. Numerators [heads][128], then maxima and denominators.
 __host__ __device__ constexpr int piece_floats(int heads) { return heads * kDim + 2 * heads; }
 
-// Merges the pieces first, first + 1, ... of which at(i) is the address; lane l holds channels 4 l .. of every head.
+// Adds the pieces base[i], i in `which`, in order; lane l holds channels 4 l .. of every head.
 template <int R>
 struct Merged {
     float4 acc[R];
@@ -121,17 +144,6 @@ struct Merged {
         l[h] = l[h] * x + la * y;
         m[h] = top;
     }
-    template <bool GLOBAL>
-    __device__ __forceinline__ void add_piece(const float* piece, int lane) {
-#pragma unroll
-        for (int h = 0; h < R; ++h) {
-            const float4* a = reinterpret_cast<const float4*>(piece + h * kDim) + lane;
-            if constexpr (GLOBAL)
-                add(h, __ldcg(a), __ldcg(piece + R * kDim + h), __ldcg(piece + R * kDim + R + h));
-            else
-                add(h, *a, piece[R * kDim + h], piece[R * kDim + R + h]);
-        }
-    }
     __device__ __forceinline__ void store(float* piece, int lane) const {
 #pragma unroll
         for (int h = 0; h < R; ++h) {
@@ -146,16 +158,15 @@ struct Merged {
 
 // The pair's rows of the output, and their int8 codes (int8_gemm.cu:147-211) where asked for. heads <= R are real.
 template <int R>
-__device__ __noinline__ void finish(const Kv4Params& p, const Merged<R>& s, int b, int kvh, int heads, int lane) {
+__device__ __forceinline__ void finish(const Kv4Params& p, const Merged<R>& s, int b, int kvh, int heads, int lane) {
     const int K = p.n_q * kDim;
     const size_t row = static_cast<size_t>(b) * K + static_cast<size_t>(kvh) * heads * kDim;
     float2 v[R][2];
 #pragma unroll
     for (int h = 0; h < R; ++h) {
-        if (h >= heads) break;
         const float inv = s.l[h] != 0.0f ? 1.0f / s.l[h] : 0.0f;
         const __half2 a = __floats2half2_rn(s.acc[h].x * inv, s.acc[h].y * inv), c = __floats2half2_rn(s.acc[h].z * inv, s.acc[h].w * inv);
-        if (p.out) *reinterpret_cast<uint2*>(p.out + row + h * kDim + 4 * lane) = {as_u32(a), as_u32(c)};
+        if (p.out && h < heads) *reinterpret_cast<uint2*>(p.out + row + h * kDim + 4 * lane) = {as_u32(a), as_u32(c)};
         v[h][0] = __half22float2(a);
         v[h][1] = __half22float2(c);
     }
@@ -163,8 +174,8 @@ __device__ __noinline__ void finish(const Kv4Params& p, const Merged<R>& s, int 
     float amax[R];
 #pragma unroll
     for (int h = 0; h < R; ++h) {
-        if (h >= heads) break;
         amax[h] = fmaxf(fmaxf(fabsf(v[h][0].x), fabsf(v[h][0].y)), fmaxf(fabsf(v[h][1].x), fabsf(v[h][1].y)));
+#pragma unroll 1
         for (int d = 1; d < 32 && 4 * d < p.g; d <<= 1) amax[h] = fmaxf(amax[h], __shfl_xor_sync(0xffffffffu, amax[h], d));
     }
 #pragma unroll
@@ -172,11 +183,10 @@ __device__ __noinline__ void finish(const Kv4Params& p, const Merged<R>& s, int 
         if (d * kDim < p.g) {
 #pragma unroll
             for (int h = 0; h < R; ++h)
-                if (!(h & d) && (h | d) < heads) amax[h] = amax[h | d] = fmaxf(amax[h], amax[h | d]);
+                if (!(h & d)) amax[h] = amax[h | d] = fmaxf(amax[h], amax[h | d]);
         }
 #pragma unroll
     for (int h = 0; h < R; ++h) {
-        if (h >= heads) break;
         float scale = amax[h] / 127.0f;
         if (scale < 1e-8f) scale = 1e-8f;
         const float inv = 1.0f / scale;
@@ -185,9 +195,29 @@ __device__ __noinline__ void finish(const Kv4Params& p, const Merged<R>& s, int 
 #pragma unroll
         for (int e = 0; e < 4; ++e) packed |= static_cast<uint32_t>(max(-127, min(127, __float2int_rn(x[e] * inv))) & 255) << (8 * e);
         const size_t ch = row + h * kDim + 4 * lane;
-        *reinterpret_cast<uint32_t*>(p.Xq + ch) = packed;
-        if (ch % p.g == 0) p.Xs[ch / p.g] = scale;
+        if (h < heads) {
+            *reinterpret_cast<uint32_t*>(p.Xq + ch) = packed;
+            if (ch % p.g == 0) p.Xs[ch / p.g] = scale;
+        }
     }
+}
+
+// Pieces base[i] (in shared memory), i in `which`, added in order: to `to`, or finished. One copy of this code: it runs cold.
+template <int R>
+__device__ __noinline__ void merge_pieces(const Kv4Params& p, const float* base, uint32_t which, float* to, int b, int kvh) {
+    const int lane = threadIdx.x & 31;
+    Merged<R> s;
+    s.clear();
+#pragma unroll 1
+    for (; which; which &= which - 1) {
+        const float* piece = base + (__ffs(which) - 1) * piece_floats(R);
+#pragma unroll
+        for (int h = 0; h < R; ++h) s.add(h, reinterpret_cast<const float4*>(piece + h * kDim)[lane], piece[R * kDim + h], piece[R * kDim + R + h]);
+    }
+    if (to)
+        s.store(to, lane);
+    else
+        finish<R>(p, s, b, kvh, p.n_q / p.n_kv, lane);
 }
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
@@ -204,22 +234,21 @@ constexpr int kv4_smem(int batch) {
 }
 
 template <int G, int R>
-__global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) kv4_attention_kernel(const Kv4Params p) {
+__global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
     constexpr int W = Shape<R>::kWarps, D = Shape<R>::kStages, kPage = q4::page_bytes(G), kPiece = piece_floats(R);
+    static_assert((D & (D - 1)) == 0 && D <= 32, "a stage is the low bits of a unit's number");
     extern __shared__ __align__(128) unsigned char kv4_smem_raw[];
-    unsigned char* const ring_all = kv4_smem_raw;                                          // [W][D][kPage]
-    float* const pieces = reinterpret_cast<float*>(kv4_smem_raw + W * D * kPage);          // [W][2][kPiece]
-    int* const first_s = reinterpret_cast<int*>(pieces + W * 2 * kPiece);                  // [batch + 1]: table entries in use ahead of a sequence
+    unsigned char* const ring_all = kv4_smem_raw;                                  // [W][D][kPage]
+    float* const pieces = reinterpret_cast<float*>(kv4_smem_raw + W * D * kPage);  // [W][2][kPiece]
+    int* const first_s = reinterpret_cast<int*>(pieces + W * 2 * kPiece);          // [batch + 1]: table entries in use ahead of a sequence
     __shared__ __align__(8) uint64_t full_bar[W][D];
     __shared__ int scan_s[W + 1];
     __shared__ long long piece_pair[2 * W];  // the pair of a piece, or -1
     __shared__ int last_s;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
-    const int heads = p.n_q / p.n_kv;
-    if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < D; ++i) ptx::mbar_init(&full_bar[warp][i], 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (lane < D) {
+        ptx::mbar_init(&full_bar[warp][lane], 1);
         ptx::fence_barrier_init();
         ptx::fence_proxy_async();
     }
@@ -229,50 +258,52 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
 
     // ---- table entries in use ahead of every sequence; each is n_kv units ----
     const int cap = p.max_blocks * kTokens;
-    {
+    auto entries_of = [&](int b) { return (min(max(p.lens[b], 0), cap) + kTokens - 1) / kTokens; };
+    if (p.batch <= 32) {
+        if (warp == 0) {
+            const int n = lane < p.batch ? entries_of(lane) : 0;
+            int inc = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, inc, d);
+                if (lane >= d) inc += o;
+            }
+            if (lane < p.batch) first_s[lane + 1] = inc;
+            if (lane == 0) first_s[0] = 0;
+        }
+    } else {
         const int each = (p.batch + W * 32 - 1) / (W * 32), b0 = tid * each, b1 = min(p.batch, b0 + each);
         int sum = 0;
-        for (int b = b0; b < b1; ++b) sum += (min(max(p.lens[b], 0), cap) + kTokens - 1) / kTokens;
+        for (int b = b0; b < b1; ++b) sum += entries_of(b);
         int inc = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, inc, d);
             if (lane >= d) inc += o;
         }
-        if (lane == 31) scan_s[warp + 1] = inc;
-        if (tid == 0) scan_s[0] = 0;
+        if (lane == 31) scan_s[warp] = inc;
         __syncthreads();
         int at = inc - sum;
-        for (int w = 0; w <= warp; ++w) at += scan_s[w];
-        for (int b = b0; b < b1; ++b) {
-            first_s[b] = at;
-            at += (min(max(p.lens[b], 0), cap) + kTokens - 1) / kTokens;
-        }
-        if (b1 == p.batch && (b0 < b1 || p.batch == 0)) first_s[p.batch] = at;
-        __syncthreads();
+        for (int w = 0; w < warp; ++w) at += scan_s[w];
+        if (tid == 0) first_s[0] = 0;
+        for (int b = b0; b < b1; ++b) first_s[b + 1] = at += entries_of(b);
     }
+    __syncthreads();
     const long long units = static_cast<long long>(first_s[p.batch]) * p.n_kv;
-    // rows of no tokens: zeros
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
-        if (first_s[b] == first_s[b + 1])
-            for (int h = warp; h < p.n_kv; h += W) {
-                Merged<R> none;
-                none.clear();
-                finish<R>(p, none, b, h, heads, lane);
-            }
 
     // ---- this warp's run ----
     const long long warps = static_cast<long long>(gridDim.x) * W;
     long long per = (units + warps - 1) / warps;
     if (per < p.min_units) per = p.min_units;
     const long long cta_units = per * W, cta_lo = min(units, blockIdx.x * cta_units), cta_hi = min(units, cta_lo + cta_units);
-    const long long lo = min(cta_hi, cta_lo + warp * per), hi = min(cta_hi, lo + per);
-    const int n_mine = static_cast<int>(hi - lo);
+    const long long lo = min(cta_hi, cta_lo + warp * per);
+    const int n_mine = static_cast<int>(min(cta_hi, lo + per) - lo);
 
     // the sequence of a unit
     auto sequence_of = [&](long long u) {
         const int entry = static_cast<int>(u / p.n_kv);  // (a sequence's units are those of its entries, whatever their order in it)
         int a = 0, z = p.batch - 1;
+#pragma unroll 1
         while (a < z) {
             const int mid = (a + z + 1) >> 1;
             if (first_s[mid] <= entry) a = mid; else z = mid - 1;
@@ -280,7 +311,7 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
         return a;  // (the last of those that start at or before u: empty ones in front of it start there too)
     };
     const uint32_t ring = ptx::smem_u32(ring_all) + warp * (D * kPage);
-    long long page_of = 0;  // of unit lo + (i & ~31) + lane: its page's number in the cache
+    int page_of = 0;  // the page's number in the cache of unit (i & ~31) + lane of the run
     auto look_up = [&](int i0) {
         const int i = i0 + lane;
         if (i < n_mine) {
@@ -290,164 +321,202 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
             const int rest = static_cast<int>(u - static_cast<long long>(first_s[b]) * p.n_kv), h = rest / blocks, blk = rest - h * blocks;
             int phys = p.table[static_cast<size_t>(b) * p.max_blocks + blk];
             if (phys < 0 || phys >= p.n_blocks) phys = 0;  // (the caller's mistake; reads stay inside the cache)
-            page_of = (static_cast<long long>(phys) * p.n_layers + p.layer) * p.n_kv + h;
+            page_of = (phys * p.n_layers + p.layer) * p.n_kv + h;
         }
     };
-    auto issue = [&](int i) {  // the copy of unit i of the run
-        const int from = i & 31;
-        const long long page = __shfl_sync(0xffffffffu, page_of, from);
-        if (lane == 0) {
-            uint64_t* bar = &full_bar[warp][i % D];
+    auto issue = [&](int i) {  // the copy of unit i of the run, by the lane that knows where it is
+        if (lane == (i & 31)) {
+            uint64_t* bar = &full_bar[warp][i & (D - 1)];
             ptx::mbar_arrive_expect_tx(bar, kPage);
-            bulk_load(ring + (i % D) * kPage, p.cache + page * kPage, kPage, bar);
+            bulk_load(ring + (i & (D - 1)) * kPage, p.cache + static_cast<size_t>(static_cast<uint32_t>(page_of)) * kPage, kPage, bar);
         }
     };
-    int issued = 0;
     if (n_mine > 0) {
         look_up(0);
-        for (; issued < min(n_mine, D); ++issued) issue(issued);
+        for (int i = 0; i < min(n_mine, D); ++i) issue(i);
     }
 
-    float* const my_head = pieces + (2 * warp) * kPiece;      // the piece of a pair that began in front of this run
-    float* const my_tail = pieces + (2 * warp + 1) * kPiece;  // the piece of a pair that begins in it
+    // rows of no tokens: zeros
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
+        if (first_s[b] == first_s[b + 1])
+            for (int h = warp; h < p.n_kv; h += W) merge_pieces<R>(p, pieces, 0u, nullptr, b, h);
+
+    const int g8 = lane >> 2, j4 = lane & 3;
     bool failed = false;
-    int i = 0;
     int b = n_mine > 0 ? sequence_of(lo) : 0;
-    while (i < n_mine) {
+    for (int i = 0; i < n_mine;) {
         // ---- the next pair of the run ----
         const long long u0 = lo + i;
         while (static_cast<long long>(first_s[b + 1]) * p.n_kv <= u0) ++b;
         const int blocks = first_s[b + 1] - first_s[b];
         const int rest = static_cast<int>(u0 - static_cast<long long>(first_s[b]) * p.n_kv), kvh = rest / blocks, blk0 = rest - kvh * blocks;
-        const int n_here = min(n_mine - i, blocks - blk0);
-        const int len = min(max(p.lens[b], 0), cap);
+        const int i_end = min(n_mine, i + blocks - blk0);
+        int tokens = min(max(p.lens[b], 0), cap) - blk0 * kTokens;  // from the page's first on
 
-        // q: of head g8 (rows 8 .. 15 of the tile are zero), the channels in the order of the K words
-        uint32_t qa[4][4];  // [run][a0, a2 of the first step; a0, a2 of the second]
+        // q of head g8 (nothing in columns without a head), the channels in the order of the K words; the start of the sums
+        uint32_t qb[4][4];  // [run][channels 0, 4; 1, 5; 2, 6; 3, 7 of the lane's eight]; the odd ones over 16
+        float start[G][4];  // of heads 2 j4, 2 j4 + 1, for the tokens of either half
+        {
+            const int heads = p.n_q / p.n_kv;
+            float sum[G];
 #pragma unroll
-        for (int run = 0; run < 4; ++run) {
-            uint4 w = {0, 0, 0, 0};
-            if (g8 < heads) w = ptx::ld_result_v4(p.q + (static_cast<size_t>(b) * p.n_q + kvh * heads + g8) * kDim + 32 * run + 8 * j4);
-            qa[run][0] = __byte_perm(w.x, w.z, 0x5410);  // channels 0, 4
-            qa[run][1] = __byte_perm(w.x, w.z, 0x7632);  // 1, 5
-            qa[run][2] = __byte_perm(w.y, w.w, 0x5410);  // 2, 6
-            qa[run][3] = __byte_perm(w.y, w.w, 0x7632);  // 3, 7
+            for (int x = 0; x < G; ++x) sum[x] = 0.0f;
+#pragma unroll
+            for (int run = 0; run < 4; ++run) {
+                uint4 w = {0, 0, 0, 0};
+                if (g8 < heads) w = ptx::ld_result_v4(p.q + (static_cast<size_t>(b) * p.n_q + kvh * heads + g8) * kDim + 32 * run + 8 * j4);
+                const __half2 over16 = as_half2(0x2c002c00u);
+                qb[run][0] = __byte_perm(w.x, w.z, 0x5410);
+                qb[run][1] = as_u32(__hmul2(as_half2(__byte_perm(w.x, w.z, 0x7632)), over16));
+                qb[run][2] = __byte_perm(w.y, w.w, 0x5410);
+                qb[run][3] = as_u32(__hmul2(as_half2(__byte_perm(w.y, w.w, 0x7632)), over16));
+                float even = 0.0f, odd = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float2 f = __half22float2(as_half2(qb[run][x]));
+                    (x & 1 ? odd : even) += f.x + f.y;
+                }
+                sum[run * G / 4] += fmaf(16.0f, odd, even) * -0x1p-21f;  // -8 2^-24
+            }
+#pragma unroll
+            for (int x = 0; x < G; ++x) {
+                sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
+                sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
+                const float s0 = __shfl_sync(0xffffffffu, sum[x], 8 * j4), s1 = __shfl_sync(0xffffffffu, sum[x], 8 * j4 + 4);
+                // (registers of their own, next to one another, as the multiply wants them: no copies per page)
+                asm volatile("mov.b32 %0, %4;\n mov.b32 %1, %5;\n mov.b32 %2, %4;\n mov.b32 %3, %5;"
+                             : "=f"(start[x][0]), "=f"(start[x][1]), "=f"(start[x][2]), "=f"(start[x][3]) : "f"(s0), "f"(s1));
+            }
         }
-        float m_run = kNoScore, l_run = 0.0f;
+        float m_run[2] = {kNoScore, kNoScore}, l_run[2] = {0.0f, 0.0f};  // of heads 2 j4, 2 j4 + 1
         float o[8][4];  // channels 16 n + g8 (+ 8) of heads 2 j4, 2 j4 + 1
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
 
-        for (int k = 0; k < n_here; ++k, ++i) {
-            const int st = i % D;
-            if (!failed && !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&full_bar[warp][st], (i / D) & 1))) {
-                if (lane == 0) atomicExch(p.status, 900 + st);
+#pragma unroll 1
+        for (; i < i_end; ++i, tokens -= kTokens) {
+            if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&full_bar[warp][i & (D - 1)], (i / D) & 1)) && !failed &&
+                !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&full_bar[warp][i & (D - 1)], (i / D) & 1))) {
+                atomicExch(p.status, 900);
                 failed = true;  // (the numbers are void from here on; counters and barriers still run their course)
             }
-            const uint32_t page = ring + st * kPage;
-            const int tokens = min(kTokens, len - (blk0 + k) * kTokens);
+            const uint32_t page = ring + (i & (D - 1)) * kPage;
 
-            // ---- scores: tokens 2 j4, 2 j4 + 1 (and + 8) of head g8 ----
-            float sc[2][2];
-            uint32_t ks[2][G];
+            // ---- scores: tokens g8, g8 + 8 of heads 2 j4, 2 j4 + 1 ----
+            float sc[4];  // raw: times scale_log2 they are in powers of two
+            {
+                uint32_t k0[4], k1[4], s0[G], s1[G];
+                lds_words<4>(k0, page + g8 * 64 + j4 * 16);
+                lds_words<4>(k1, page + (g8 + 8) * 64 + j4 * 16);
+                lds_words<G>(s0, page + q4::kScaleOff + (g8 >> 1) * 4 * G);
+                lds_words<G>(s1, page + q4::kScaleOff + (4 + (g8 >> 1)) * 4 * G);
+                const uint32_t pick = g8 & 1 ? 0x7632 : 0x5410;  // the token's half of two groups' words
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                uint32_t kw[4];
-                lds_words<4>(kw, page + (g8 + 8 * t) * 64 + j4 * 16);
-                lds_words<G>(ks[t], page + q4::kScaleOff + (j4 + 4 * t) * 4 * G);
-                sc[t][0] = sc[t][1] = 0.0f;
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int x = 0; x < G; ++x) {
+                    float d[4];
 #pragma unroll
-                for (int run = 0; run < 4; ++run) {
-                    uint32_t h[4];
-                    unpack8(kw[run], h);
-                    mma_f16(acc, qa[run][0], 0u, qa[run][1], 0u, h[0], h[1]);
-                    mma_f16(acc, qa[run][2], 0u, qa[run][3], 0u, h[2], h[3]);
-                    if ((run + 1) % (4 / G) == 0) {
-                        const float2 s = __half22float2(as_half2(ks[t][run / (4 / G)]));
-                        sc[t][0] = fmaf(acc[0], s.x, sc[t][0]);
-                        sc[t][1] = fmaf(acc[1], s.y, sc[t][1]);
-                        acc[0] = acc[1] = 0.0f;
+                    for (int run = x * 4 / G; run < (x + 1) * 4 / G; ++run) {
+                        uint32_t h0[4], h1[4];
+                        unpack8_tiny(k0[run], h0);
+                        unpack8_tiny(k1[run], h1);
+                        if (run == x * 4 / G)
+                            mma_f16(d, h0[0], h1[0], h0[1], h1[1], qb[run][0], qb[run][1], start[x]);
+                        else
+                            mma_f16(d, h0[0], h1[0], h0[1], h1[1], qb[run][0], qb[run][1]);
+                        mma_f16(d, h0[2], h1[2], h0[3], h1[3], qb[run][2], qb[run][3]);
                     }
+                    const int other = G > 1 ? x ^ 1 : x;
+                    const float2 t0 = __half22float2(as_half2(__byte_perm(s0[x & ~1], s0[other | x], pick)));
+                    const float2 t1 = __half22float2(as_half2(__byte_perm(s1[x & ~1], s1[other | x], pick)));
+                    const float f0 = x & 1 ? t0.y : t0.x, f1 = x & 1 ? t1.y : t1.x;
+                    sc[0] = x ? fmaf(d[0], f0, sc[0]) : d[0] * f0;
+                    sc[1] = x ? fmaf(d[1], f0, sc[1]) : d[1] * f0;
+                    sc[2] = x ? fmaf(d[2], f1, sc[2]) : d[2] * f1;
+                    sc[3] = x ? fmaf(d[3], f1, sc[3]) : d[3] * f1;
                 }
             }
-            float mx = kNoScore;
+            uint32_t v0[4], v1[4], vs0[G], vs1[G];  // V of token pairs j4 and 4 + j4
+            lds_words<4>(v0, page + q4::kVOff + j4 * 128 + g8 * 16);
+            lds_words<4>(v1, page + q4::kVOff + (4 + j4) * 128 + g8 * 16);
+            lds_words<G>(vs0, page + q4::kScaleOff + 2 * kTokens * G + j4 * 4 * G);
+            lds_words<G>(vs1, page + q4::kScaleOff + 2 * kTokens * G + (4 + j4) * 4 * G);
+            if (tokens < kTokens) {  // what lies behind the sequence's end may not be a number: its scale becomes zero
+                auto keep = [&](int left) { return left >= 2 ? 0xffffffffu : left == 1 ? 0x0000ffffu : 0u; };
+                const uint32_t keep0 = keep(tokens - 2 * j4), keep1 = keep(tokens - 8 - 2 * j4);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int x = 0; x < G; ++x) {
+                    vs0[x] &= keep0;
+                    vs1[x] &= keep1;
+                }
+            }
+            // relative to the reference; what lies behind the sequence's end weighs nothing
+            float y[4];
+            auto relative = [&] {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = g8 + 4 * (e & 2) < tokens ? fmaf(sc[e], p.scale_log2, -m_run[e & 1]) : -INFINITY;
+            };
+            relative();
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kLag)) {
+                const float before[2] = {m_run[0], m_run[1]};
+                m_run[0] = m_run[1] = 0.0f;
+                relative();
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    sc[t][e] = 8 * t + 2 * j4 + e < tokens ? sc[t][e] * p.scale_log2 : kNoScore;
-                    mx = fmaxf(mx, sc[t][e]);
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (__any_sync(0xffffffffu, mx > m_run)) {
-                const float top = fmaxf(m_run, mx), corr = exp2_fast(m_run - top);
-                m_run = top;
-                l_run *= corr;
-                const float c0 = __shfl_sync(0xffffffffu, corr, 8 * j4), c1 = __shfl_sync(0xffffffffu, corr, 8 * j4 + 4);
+                    float mx = fmaxf(y[e], y[2 + e]);
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    o[n][0] *= c0;
-                    o[n][1] *= c1;
-                    o[n][2] *= c0;
-                    o[n][3] *= c1;
+                    for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                    m_run[e] = fmaxf(before[e], mx);
+                    const float corr = exp2_fast(before[e] - m_run[e]);
+                    l_run[e] *= corr;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        o[n][e] *= corr;
+                        o[n][2 + e] *= corr;
+                    }
                 }
+                relative();
             }
-            const __half2 p0 = __floats2half2_rn(exp2_fast(sc[0][0] - m_run), exp2_fast(sc[0][1] - m_run));
-            const __half2 p1 = __floats2half2_rn(exp2_fast(sc[1][0] - m_run), exp2_fast(sc[1][1] - m_run));
+            const __half2 p0 = __floats2half2_rn(exp2_fast(y[0]), exp2_fast(y[1])), p1 = __floats2half2_rn(exp2_fast(y[2]), exp2_fast(y[3]));
             const float2 f0 = __half22float2(p0), f1 = __half22float2(p1);
-            l_run += (f0.x + f0.y) + (f1.x + f1.y);
+            l_run[0] += f0.x + f1.x;
+            l_run[1] += f0.y + f1.y;
 
             // ---- out^T += V^T P^T: rows are channels, columns heads, the contraction runs over tokens ----
-            uint32_t vw[2][4], vs[2][G];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                lds_words<4>(vw[t], page + q4::kVOff + (j4 + 4 * t) * 128 + g8 * 16);
-                lds_words<G>(vs[t], page + q4::kScaleOff + 2 * kTokens * G + (j4 + 4 * t) * 4 * G);
-            }
-            if (tokens < kTokens)  // what lies behind the sequence's end may not be a number: its scale becomes zero
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int left = tokens - (8 * t + 2 * j4);
-                    const uint32_t keep = left >= 2 ? 0xffffffffu : left == 1 ? 0x0000ffffu : 0u;
-#pragma unroll
-                    for (int x = 0; x < G; ++x) vs[t][x] &= keep;
-                }
+            const uint32_t pb0 = transposed(as_u32(p0)), pb1 = transposed(as_u32(p1));
 #pragma unroll
             for (int high = 0; high < 2; ++high) {
                 uint32_t a0[4], a1[4], a2[4], a3[4];
-                unpack8(vw[0][high], a0);
-                unpack8(vw[0][2 + high], a1);
-                unpack8(vw[1][high], a2);
-                unpack8(vw[1][2 + high], a3);
+                unpack8(v0[high], a0);
+                unpack8(v0[2 + high], a1);
+                unpack8(v1[high], a2);
+                unpack8(v1[2 + high], a3);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    const int x = (4 * high + n) * G / 8;
-                    const __half2 s0 = as_half2(vs[0][x]), s1 = as_half2(vs[1][x]);
+                    const __half2 s0 = as_half2(vs0[(4 * high + n) * G / 8]), s1 = as_half2(vs1[(4 * high + n) * G / 8]);
                     mma_f16(o[4 * high + n], as_u32(__hmul2(as_half2(a0[n]), s0)), as_u32(__hmul2(as_half2(a1[n]), s0)),
-                            as_u32(__hmul2(as_half2(a2[n]), s1)), as_u32(__hmul2(as_half2(a3[n]), s1)), as_u32(p0), as_u32(p1));
+                            as_u32(__hmul2(as_half2(a2[n]), s1)), as_u32(__hmul2(as_half2(a3[n]), s1)), pb0, pb1);
                 }
             }
 
             // ---- the stage is free: the copy of the unit kStages ahead ----
-            if (issued < n_mine) {
+            const int next = i + D;
+            if (next < n_mine) {
                 ptx::fence_proxy_async();
                 __syncwarp();
-                if ((issued & 31) == 0) look_up(issued);
-                if (!failed) issue(issued);
-                ++issued;
+                if ((next & 31) == 0) look_up(next);
+                if (!failed) issue(next);
             }
         }
 
-        // ---- the pair's piece ----
-        l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-        l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-        float* const piece = blk0 > 0 ? my_head : my_tail;
+        // ---- the pair's piece: of a pair that began in front of this run, or that begins in it ----
+        const bool head = blk0 > 0;
+        float* const piece = pieces + (2 * warp + (head ? 0 : 1)) * kPiece;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], d);
             const int h = 2 * j4 + e;
             if (h < R) {
 #pragma unroll
@@ -455,21 +524,18 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
                     piece[h * kDim + 16 * n + g8] = o[n][e];
                     piece[h * kDim + 16 * n + 8 + g8] = o[n][2 + e];
                 }
+                if (g8 == 0) {
+                    piece[R * kDim + h] = m_run[e];
+                    piece[R * kDim + R + h] = l_run[e];
+                }
             }
         }
-        if (j4 == 0 && g8 < R) {
-            piece[R * kDim + g8] = m_run;
-            piece[R * kDim + R + g8] = l_run;
-        }
         __syncwarp();
-        if (blk0 == 0 && n_here == blocks) {  // all of the pair
-            Merged<R> s;
-            s.clear();
-            s.template add_piece<false>(piece, lane);
-            finish<R>(p, s, b, kvh, heads, lane);
+        if (!head && lo + i - u0 == blocks) {  // all of the pair
+            merge_pieces<R>(p, piece, 1u, nullptr, b, kvh);
             __syncwarp();
         } else if (lane == 0) {
-            piece_pair[2 * warp + (blk0 > 0 ? 0 : 1)] = static_cast<long long>(b) * p.n_kv + kvh;
+            piece_pair[2 * warp + (head ? 0 : 1)] = static_cast<long long>(b) * p.n_kv + kvh;
         }
     }
     __syncthreads();
@@ -481,41 +547,37 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
         from = static_cast<long long>(first_s[pb]) * p.n_kv + static_cast<long long>(ph) * blocks;
         to = from + blocks;
     };
-    int chain = 0;
+    // (lane x of every warp looks at piece x; a chain starts where the piece in front of it is another pair's)
+    const long long pair_x = lane < 2 * W ? piece_pair[lane] : -1;
+    const uint32_t there = __ballot_sync(0xffffffffu, pair_x >= 0);
+    const uint32_t in_front = there & ((1u << lane) - 1);
+    const long long pair_before = __shfl_sync(0xffffffffu, pair_x, in_front ? 31 - __clz(in_front) : 0);
+    const uint32_t starts = __ballot_sync(0xffffffffu, pair_x >= 0 && (!in_front || pair_before != pair_x));
     long long open[2] = {-1, -1};  // pairs that go on in other CTAs: one that began ahead of this CTA's run, one that ends behind it
-    for (int x = 0; x < 2 * W;) {
-        const long long pair = piece_pair[x];
-        if (pair < 0) { ++x; continue; }
-        int y = x + 1, z = x;  // z: the last piece of the chain
-        while (y < 2 * W && (piece_pair[y] < 0 || piece_pair[y] == pair)) {
-            if (piece_pair[y] == pair) z = y;
-            ++y;
-        }
+    int chain = 0;
+#pragma unroll 1
+    for (uint32_t todo = starts; todo; todo &= todo - 1, ++chain) {
+        const int x = __ffs(todo) - 1;
+        const uint32_t later = todo & (todo - 1);
+        const uint32_t mine = there & (0xffffffffu << x) & (later ? (1u << (__ffs(later) - 1)) - 1 : 0xffffffffu);
+        const long long pair = __shfl_sync(0xffffffffu, pair_x, x);
         long long from, to;
         pair_units(pair, from, to);
-        const bool whole = from >= cta_lo && to <= cta_hi;
-        if (!whole) open[from < cta_lo ? 0 : 1] = pair;
-        if (chain % W == warp) {
-            Merged<R> s;
-            s.clear();
-            for (int k = x; k <= z; ++k)
-                if (piece_pair[k] == pair) s.template add_piece<false>(pieces + k * kPiece, lane);
-            if (whole)
-                finish<R>(p, s, static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv), heads, lane);
-            else {
-                s.store(p.scratch + (2ll * blockIdx.x + (from < cta_lo ? 0 : 1)) * kPiece, lane);
-                __threadfence();
-            }
-        }
-        ++chain;
-        x = y;
+        const bool whole = from >= cta_lo && to <= cta_hi, before = from < cta_lo;
+        if (!whole) open[before ? 0 : 1] = pair;
+        if (chain % W != warp) continue;
+        merge_pieces<R>(p, pieces, mine, whole ? nullptr : p.scratch + (2ll * blockIdx.x + (before ? 0 : 1)) * kPiece,
+                        static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
+        if (!whole) __threadfence();
     }
 
     // ---- pairs that lie in several CTAs: the last of them to come here adds their pieces ----
+#pragma unroll 1
     for (int side = 0; side < 2; ++side) {
-        if (open[side] < 0) continue;  // (uniform over the CTA)
+        const long long pair = open[side];
+        if (pair < 0) continue;  // (uniform over the CTA)
         long long from, to;
-        pair_units(open[side], from, to);
+        pair_units(pair, from, to);
         const int c0 = static_cast<int>(from / cta_units), c1 = static_cast<int>((to - 1) / cta_units);
         __syncthreads();
         if (tid == 0) {
@@ -527,19 +589,20 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
         }
         __syncthreads();
         if (!last_s) continue;
-        Merged<R> s;
-        s.clear();
         // pieces in the order of the pages: warp w a run of them, the runs then in order
         const int n = c1 - c0 + 1, run = (n + W - 1) / W, a = min(n, warp * run), z = min(n, a + run);
+        Merged<R> s;
+        s.clear();
 #pragma unroll 2
-        for (int k = a; k < z; ++k) s.template add_piece<true>(p.scratch + (2ll * (c0 + k) + (k == 0 ? 1 : 0)) * kPiece, lane);
+        for (int k = a; k < z; ++k) {
+            const float* piece = p.scratch + (2ll * (c0 + k) + (k == 0 ? 1 : 0)) * kPiece;
+#pragma unroll
+            for (int h = 0; h < R; ++h)
+                s.add(h, __ldcg(reinterpret_cast<const float4*>(piece + h * kDim) + lane), __ldcg(piece + R * kDim + h), __ldcg(piece + R * kDim + R + h));
+        }
         s.store(pieces + warp * kPiece, lane);
         __syncthreads();
-        if (warp == 0) {
-            s.clear();
-            for (int w = 0; w < W; ++w) s.template add_piece<false>(pieces + w * kPiece, lane);
-            finish<R>(p, s, static_cast<int>(open[side] / p.n_kv), static_cast<int>(open[side] % p.n_kv), heads, lane);
-        }
+        if (warp == 0) merge_pieces<R>(p, pieces, (1u << W) - 1, nullptr, static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
         __syncthreads();
     }
     if (failed) {  // copies that may still be on their way land before the CTA goes
@@ -584,7 +647,7 @@ int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const
     if (batch == 0) return W8A8_OK;
     const int ratio = n_q / n_kv;
     Kv4Params p = {q, static_cast<const unsigned char*>(cache), table, lens, out, Xq, Xs, g, batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers,
-                   sm_scale * 1.4426950408889634f, 1, scratch, tickets, status};
+                   sm_scale * 1.4426950408889634f * 0x1p24f, 1, scratch, tickets, status};
     int ctas = kv4_ctas(ratio, static_cast<long long>(batch) * n_kv * max_blocks, device_sms());
     if (ctas > kKv4Tickets) ctas = kKv4Tickets;
     cudaError_t e;
