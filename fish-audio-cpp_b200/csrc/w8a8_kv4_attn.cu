@@ -34,6 +34,10 @@ using q4::kTokens;
 
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
+#ifndef KV4_WHOLE
+#define KV4_WHOLE 256
+#endif
+constexpr int kWholePages = KV4_WHOLE;
 constexpr float kLag = 8.0f;  // p is at most 2^8: it keeps its precision in fp16
 
 struct Kv4Params {
@@ -47,7 +51,7 @@ struct Kv4Params {
     int g;
     int batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers;
     float scale_log2;  // sm_scale * log2(e) * 2^24: the scores' codes come as 2^-24 of themselves
-    int min_units;     // pages a warp takes at least
+    int whole_pages;   // pairs of at most so many pages lie in one CTA
     float* scratch;    // [CTAs][2] pieces
     int* tickets;      // [CTAs], zero between launches
     int* status;
@@ -224,9 +228,8 @@ __device__ __noinline__ void merge_pieces(const Kv4Params& p, const float* base,
 // G groups per head; R the most query heads per kv head (4 or 8); W warps.
 template <int R>
 struct Shape {
-    static constexpr int kWarps = R == 4 ? 8 : 12;
+    static constexpr int kWarps = R == 4 ? 16 : 12;
     static constexpr int kStages = 4;
-    static constexpr int kCtasPerSm = R == 4 ? 2 : 1;
 };
 template <int G, int R>
 constexpr int kv4_smem(int batch) {
@@ -234,7 +237,7 @@ constexpr int kv4_smem(int batch) {
 }
 
 template <int G, int R>
-__global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
+__global__ void __launch_bounds__(Shape<R>::kWarps * 32, 1) kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
     constexpr int W = Shape<R>::kWarps, D = Shape<R>::kStages, kPage = q4::page_bytes(G), kPiece = piece_floats(R);
     static_assert((D & (D - 1)) == 0 && D <= 32, "a stage is the low bits of a unit's number");
     extern __shared__ __align__(128) unsigned char kv4_smem_raw[];
@@ -291,14 +294,6 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
     __syncthreads();
     const long long units = static_cast<long long>(first_s[p.batch]) * p.n_kv;
 
-    // ---- this warp's run ----
-    const long long warps = static_cast<long long>(gridDim.x) * W;
-    long long per = (units + warps - 1) / warps;
-    if (per < p.min_units) per = p.min_units;
-    const long long cta_units = per * W, cta_lo = min(units, blockIdx.x * cta_units), cta_hi = min(units, cta_lo + cta_units);
-    const long long lo = min(cta_hi, cta_lo + warp * per);
-    const int n_mine = static_cast<int>(min(cta_hi, lo + per) - lo);
-
     // the sequence of a unit
     auto sequence_of = [&](long long u) {
         const int entry = static_cast<int>(u / p.n_kv);  // (a sequence's units are those of its entries, whatever their order in it)
@@ -310,6 +305,22 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
         }
         return a;  // (the last of those that start at or before u: empty ones in front of it start there too)
     };
+    // ---- this warp's run ----
+    const long long cta_units = max((units + gridDim.x - 1) / gridDim.x, 1ll);
+    // Where CTA c's run begins: at c cta_units, but not inside a pair of few pages, which goes to one side or the other as a whole.
+    auto border = [&](long long c) {
+        const long long u = c * cta_units;
+        if (u >= units) return units;
+        const int b = sequence_of(u), blocks = first_s[b + 1] - first_s[b];
+        const long long from = static_cast<long long>(first_s[b]) * p.n_kv;
+        const int in = static_cast<int>(u - from) % blocks;
+        return blocks > p.whole_pages ? u : 2 * in < blocks ? u - in : u - in + blocks;
+    };
+    const long long cta_lo = border(blockIdx.x), cta_hi = border(blockIdx.x + 1);
+    const int per = static_cast<int>((cta_hi - cta_lo + W - 1) / W);
+    const long long lo = min(cta_hi, cta_lo + warp * per);
+    const int n_mine = static_cast<int>(min(cta_hi, lo + per) - lo);
+
     const uint32_t ring = ptx::smem_u32(ring_all) + warp * (D * kPage);
     int page_of = 0;  // the page's number in the cache of unit (i & ~31) + lane of the run
     auto look_up = [&](int i0) {
@@ -568,7 +579,6 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
         if (chain % W != warp) continue;
         merge_pieces<R>(p, pieces, mine, whole ? nullptr : p.scratch + (2ll * blockIdx.x + (before ? 0 : 1)) * kPiece,
                         static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
-        if (!whole) __threadfence();
     }
 
     // ---- pairs that lie in several CTAs: the last of them to come here adds their pieces ----
@@ -580,12 +590,11 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, Shape<R>::kCtasPerSm) k
         pair_units(pair, from, to);
         const int c0 = static_cast<int>(from / cta_units), c1 = static_cast<int>((to - 1) / cta_units);
         __syncthreads();
-        if (tid == 0) {
-            __threadfence();
-            const int before = atomicAdd(p.tickets + c0, 1);
+        if (tid == 0) {  // (releases what the CTA's warps stored ahead of the barrier, acquires what the others' released)
+            int before;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + c0) : "memory");
             last_s = before == c1 - c0;
             if (last_s) p.tickets[c0] = 0;
-            __threadfence();
         }
         __syncthreads();
         if (!last_s) continue;
@@ -627,12 +636,6 @@ cudaError_t launch_kv4(const Kv4Params& p, int ctas, cudaStream_t stream) {
     return launch_with_smem(attribute, kv4_smem<G, R>(kMaxBatch), cfg, kv4_attention_kernel<G, R>, p);
 }
 
-int kv4_ctas(int heads_per_kv, long long most_units, int sms) {
-    const int W = heads_per_kv <= 4 ? Shape<4>::kWarps : Shape<8>::kWarps, per_sm = heads_per_kv <= 4 ? Shape<4>::kCtasPerSm : Shape<8>::kCtasPerSm;
-    const long long want = (most_units + W - 1) / W, room = static_cast<long long>(sms) * per_sm;
-    return static_cast<int>(want < 1 ? 1 : want < room ? want : room);
-}
-
 }  // namespace
 
 int kv4_max_batch() { return kMaxBatch; }
@@ -647,9 +650,9 @@ int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const
     if (batch == 0) return W8A8_OK;
     const int ratio = n_q / n_kv;
     Kv4Params p = {q, static_cast<const unsigned char*>(cache), table, lens, out, Xq, Xs, g, batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers,
-                   sm_scale * 1.4426950408889634f * 0x1p24f, 1, scratch, tickets, status};
-    int ctas = kv4_ctas(ratio, static_cast<long long>(batch) * n_kv * max_blocks, device_sms());
-    if (ctas > kKv4Tickets) ctas = kKv4Tickets;
+                   sm_scale * 1.4426950408889634f * 0x1p24f, kWholePages, scratch, tickets, status};
+    const long long most = static_cast<long long>(batch) * n_kv * max_blocks;  // units, were all sequences as long as their rows
+    const int sms = device_sms() < kKv4Tickets ? device_sms() : kKv4Tickets, ctas = most < sms ? static_cast<int>(most) : sms;
     cudaError_t e;
     if (ratio <= 4)
         e = group == 32 ? launch_kv4<4, 4>(p, ctas, stream) : group == 64 ? launch_kv4<2, 4>(p, ctas, stream) : launch_kv4<1, 4>(p, ctas, stream);
