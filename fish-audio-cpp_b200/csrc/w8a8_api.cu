@@ -655,7 +655,8 @@ int w8a8_linear4_q(w8a8_ctx* ctx, const void* W4, const void* w_scale, int group
     if (M > 0 && (!W4 || !w_scale || !Xq || !Xs || !Y)) return fail(W8A8_ERR_INVALID_ARG, "linear4_q: null pointer");
     if (int rc = check_device(ctx, "linear4_q")) return rc;
     return launch_linear4(W4, static_cast<const __half*>(w_scale), group_size, static_cast<const int8_t*>(Xq), static_cast<const float*>(Xs),
-                          static_cast<__half*>(Y), static_cast<const __half*>(residual), M, N, K, epilogue, static_cast<cudaStream_t>(stream));
+                          static_cast<__half*>(Y), static_cast<const __half*>(residual), M, N, K, epilogue, ctx->device_status,
+                          static_cast<cudaStream_t>(stream));
 }
 
 int w8a8_quantize_weight4(w8a8_ctx* ctx, const void* W, int N, int K, int group_size, void* W4, void* w_scale, void* stream) {

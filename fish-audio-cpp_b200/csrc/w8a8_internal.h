@@ -187,7 +187,7 @@ int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const
                          float* scratch, int* tickets, int* status, cudaStream_t stream);
 // w8a8_linear4.cu : few rows of activation codes times 4-bit weights.
 int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t* Xq, const float* Xs, __half* Y, const __half* residual, int M, int N,
-                   int K, int epilogue, cudaStream_t stream);
+                   int K, int epilogue, int* status, cudaStream_t stream);
 int launch_quantize_weight4(const __half* W, int N, int K, int group, void* codes, __half* scale, cudaStream_t stream);
 int launch_unpack_weight4(const void* codes, int N, int K, void* W, cudaStream_t stream);
 // w8a8_decode_stack.cu : a whole decode step as one persistent cooperative kernel.

@@ -10,8 +10,16 @@
 //
 // A word of eight codes becomes two operand registers of mma.m16n8k32.s8 by a shift and two masks: w << 4 and w, both & 0xf0f0f0f0, are
 // sixteen times the even and the odd codes as int8; the factor leaves with the weight scale (ws / 16, exact). The contraction index may
-// be permuted freely as long as both operands agree, so lane (row, j) takes 4 V consecutive bytes of its row, and the activations of the
-// same 8 V channels are split into even and odd bytes by two byte permutes per pair of words.
+// be permuted freely as long as both operands agree and a multiply stays inside one group, so a lane reads its row's codes as they lie (16, 8
+// or 4 bytes for groups of 128 and more, 64, 32), and the activations lie in shared memory in the same order, the eight channels of
+// a word split into even and odd bytes.
+//
+// A warp streams boxes of 16 rows x 256 channels (2 KB) by TMA through a ring of its own, kStages ahead and ahead of the dependency wait, so
+// no instructions are spent on addresses; rows and channels behind the matrix come as zeros. Row r of a box is row bitrev(r) of the tile: the
+// rows that lanes read together then lie in different banks of the 128-byte swizzle.
+//
+// Split. A CTA has whole tiles of 16 rows; its warps take equal runs of their boxes, so that only tiles that a border cuts are added
+// up over warps, in ascending channels, after one barrier at the end; all others leave from the registers.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 #include "w8a8_q4.cuh"
@@ -20,6 +28,8 @@ namespace w8a8 {
 namespace {
 
 constexpr int kL4Warps = 8;
+constexpr int kL4MaxSmem = 224 * 1024;
+constexpr int kBoxRows = 16, kBoxBytes = 128, kBox = kBoxRows * kBoxBytes, kBoxK = 2 * kBoxBytes;
 
 struct L4Params {
     const uint8_t* W;       // [N, K / 2]
@@ -30,7 +40,10 @@ struct L4Params {
     const __half* residual;
     int M, N, K, g, G;
     int epilogue;
-    int tiles;  // of 16 rows
+    int tiles;   // of 16 rows
+    int boxes;   // per tile
+    int stages;  // of a warp's ring
+    int* status;
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -38,20 +51,25 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int V>
-struct Words {
-    uint32_t w[V];
-};
-template <int V>
-__device__ __forceinline__ Words<V> load_weights(const uint8_t* p) {
-    Words<V> r;
-    if constexpr (V == 4)
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p));
-    else if constexpr (V == 2)
-        asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
-    else
-        asm volatile("ld.global.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
-    return r;
+__device__ __forceinline__ void mma_s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
 }
 
 // What the epilogues make of a finished fp32 sum (roundings of the reference's separate kernels, ffn_activations.cu:12-17, :35-45).
@@ -65,147 +83,296 @@ __device__ __forceinline__ __half l4_plain(float v, const __half* residual, size
     return residual ? __float2half_rn(__half2float(h) + __half2float(residual[at])) : h;
 }
 
-// T token tiles of 8; V words a lane and row per step (a step is 32 V channels, all in one group).
-template <int T, int V>
-__global__ void __launch_bounds__(kL4Warps * 32) linear4_kernel(const L4Params p) {
-    constexpr int U = 4;  // steps on their way
-    __shared__ float part_s[2][kL4Warps][16][8 * T + 1];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
-    const int steps = (p.K + 32 * V - 1) / (32 * V);
-    const int s0 = steps * warp / kL4Warps, s1 = steps * (warp + 1) / kL4Warps, mine = s1 - s0;
-    const int n_tiles = blockIdx.x < p.tiles ? (p.tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
-    const int total = mine * n_tiles;
-    const size_t pitch = static_cast<size_t>(p.K / 2);
+// T token tiles of 8; P promotes per box (256 / P channels each, all in one group); EXACT: groups of 256 / P channels, K in whole boxes and
+// the scales of a box in one aligned read.
+// Shared memory: rings [warps][stages][box]; pieces fp32 [warps][2][16][8 T + 1]; activation scales fp32 [G][8 T]; their codes
+// [box][quarter of 64 channels][M][lane of 4][16 bytes].
+template <int T>
+constexpr int l4_piece_floats() { return 16 * (8 * T + 1); }
+template <int T>
+size_t l4_smem(int M, int K, int G, int stages) {
+    return 1024 + static_cast<size_t>(kL4Warps) * stages * kBox + 2 * kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(G) * 8 * T * 4 +
+           static_cast<size_t>((K + kBoxK - 1) / kBoxK) * kBoxK * M;
+}
 
-    Words<V> wbuf[U][2];
-    int l_tile = blockIdx.x, l_step = s0;  // the next step to load
-    auto load = [&](Words<V> (&w)[2]) {
-        const int k = 32 * V * l_step + 8 * V * j4;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int row = l_tile * 16 + 8 * half + g8;
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[half].w[v] = 0u;
-            if (k < p.K && row < p.N) w[half] = load_weights<V>(p.W + row * pitch + k / 2);
-        }
-        if (++l_step == s1) {
-            l_step = s0;
-            l_tile += gridDim.x;
+template <int T, int P, bool EXACT>
+__global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ L4Params p) {
+    constexpr int kPiece = l4_piece_floats<T>(), kCols = 8 * T + 1;
+    extern __shared__ unsigned char l4_smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[kL4Warps][8];
+    unsigned char* const base = l4_smem_raw + ((1024u - (ptx::smem_u32(l4_smem_raw) & 1023u)) & 1023u);  // (the swizzle repeats every 1024 bytes)
+    float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kBox);
+    float* const xs_s = piece_s + 2 * kL4Warps * kPiece;
+    unsigned char* const codes_s = reinterpret_cast<unsigned char*>(xs_s + p.G * 8 * T);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
+    const int row8 = (g8 & 1) << 2 | (g8 & 2) | g8 >> 2;  // the row of the tile that this lane's fragment row is (and + 8)
+    // tiles [t0, t0 + nt) of this CTA, units [u0, u0 + n_mine) of this warp: the boxes of the CTA's tiles, one tile after the other
+    const int t0 = static_cast<int>(static_cast<long long>(p.tiles) * blockIdx.x / gridDim.x);
+    const int nt = static_cast<int>(static_cast<long long>(p.tiles) * (blockIdx.x + 1) / gridDim.x) - t0;
+    const int all = nt * p.boxes;
+    const int u0 = static_cast<int>(static_cast<long long>(all) * warp / kL4Warps);
+    const int n_mine = static_cast<int>(static_cast<long long>(all) * (warp + 1) / kL4Warps) - u0;
+    int tile = t0 + u0 / p.boxes, box = u0 % p.boxes;
+    bool head = box > 0;  // the tile began in another warp's run
+
+    const uint32_t ring = ptx::smem_u32(base) + warp * p.stages * kBox;
+    int l_tile = tile, l_box = box;
+    auto issue = [&](int stage) {  // (one lane)
+        uint64_t* bar = &full_bar[warp][stage];
+        ptx::mbar_arrive_expect_tx(bar, kBox);
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(ring + stage * kBox),
+            "l"(&map), "r"(ptx::smem_u32(bar)), "r"(l_box * kBoxBytes), "r"(l_tile * kBoxRows)
+            : "memory");
+        if (++l_box == p.boxes) {
+            l_box = 0;
+            ++l_tile;
         }
     };
+    if (lane == 0) {
+        for (int i = 0; i < p.stages; ++i) ptx::mbar_init(&full_bar[warp][i], 1);
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async();
+        for (int i = 0; i < min(p.stages, n_mine); ++i) issue(i);
+    }
+    // weight scales of the box that comes next, rows row8 and row8 + 8
+    __half2 ws_next[P > 1 ? P : 1];  // EXACT, P > 1: [row half][P / 2 pairs of groups]; else one {row, row + 8} pair per promote
+    auto group_of = [&](int bx, int pr) { return EXACT ? bx * P + pr : min(p.G - 1, (bx * kBoxK + pr * (kBoxK / P)) / p.g); };
+    auto load_scales = [&](int tl, int bx) {
+        const size_t r0 = static_cast<size_t>(min(tl * 16 + row8, p.N - 1)) * p.G, r1 = static_cast<size_t>(min(tl * 16 + row8 + 8, p.N - 1)) * p.G;
+        if constexpr (EXACT && P > 1) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(ws_next);
+            const __half *a = p.w_scale + r0 + bx * P, *b = p.w_scale + r1 + bx * P;
+            if constexpr (P == 2) {
+                w[0] = __ldg(reinterpret_cast<const uint32_t*>(a));
+                w[1] = __ldg(reinterpret_cast<const uint32_t*>(b));
+            } else if constexpr (P == 4) {
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(a)), y = __ldg(reinterpret_cast<const uint2*>(b));
+                w[0] = x.x; w[1] = x.y; w[2] = y.x; w[3] = y.y;
+            } else {
+                const uint4 x = __ldg(reinterpret_cast<const uint4*>(a)), y = __ldg(reinterpret_cast<const uint4*>(b));
+                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+            }
+        } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (u < total) load(wbuf[u]);
+            for (int pr = 0; pr < P; ++pr) {
+                const int gr = group_of(bx, pr);
+                ws_next[pr] = __halves2half2(p.w_scale[r0 + gr], p.w_scale[r1 + gr]);
+            }
+        }
+    };
+    if (n_mine > 0) load_scales(tile, box);
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
 
-    int tile = blockIdx.x, step = s0, parity = 0;
-    int sum[T][4];
+    // ---- the activations, in the order of the fragments ----
+    {
+        const int per_row = p.boxes * 16;  // lanes' 16-byte shares of a row
+        for (int m = warp; m < p.M; m += kL4Warps)
+            for (int x = lane; x < per_row; x += 32) {
+                const int quarter = x >> 2, j = x & 3;
+                int k[2];  // of the two words' eight channels
+                if (P <= 2) {
+                    k[0] = (quarter >> 1) * 128 + j * 32 + (quarter & 1) * 16;
+                    k[1] = k[0] + 8;
+                } else if (P == 4) {
+                    k[0] = quarter * 64 + j * 16;
+                    k[1] = k[0] + 8;
+                } else {
+                    k[0] = quarter * 64 + j * 8;
+                    k[1] = k[0] + 32;
+                }
+                uint32_t c[4];
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    uint2 two = {0u, 0u};
+                    if (k[v] < p.K) two = ptx::ld_result_v2(p.Xq + static_cast<size_t>(m) * p.K + k[v]);
+                    c[2 * v] = __byte_perm(two.x, two.y, 0x6420);
+                    c[2 * v + 1] = __byte_perm(two.x, two.y, 0x7531);
+                }
+                *reinterpret_cast<uint4*>(codes_s + (quarter * p.M + m) * 64 + j * 16) = {c[0], c[1], c[2], c[3]};
+            }
+        for (int x = tid; x < p.G * 8 * T; x += kL4Warps * 32) {
+            const int group = x / (8 * T), m = x % (8 * T);
+            xs_s[x] = m < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
+        }
+    }
+    __syncthreads();
+
+    // ---- the run ----
     float acc[T][4];
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            sum[t][e] = 0;
-            acc[t][e] = 0.0f;
-        }
-    auto finish_tile = [&] {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            part_s[parity][warp][g8][8 * t + 2 * j4] = acc[t][0];
-            part_s[parity][warp][g8][8 * t + 2 * j4 + 1] = acc[t][1];
-            part_s[parity][warp][g8 + 8][8 * t + 2 * j4] = acc[t][2];
-            part_s[parity][warp][g8 + 8][8 * t + 2 * j4 + 1] = acc[t][3];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
-        }
-        __syncthreads();
-        auto added = [&](int r, int m) {
-            float v = part_s[parity][0][r][m];
-#pragma unroll
-            for (int w = 1; w < kL4Warps; ++w) v += part_s[parity][w][r][m];
-            return v;
-        };
+        for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
+    auto emit = [&](int at_tile, int r, int m, float v, float up) {  // rows r and (SwiGLU only) r + 8 of a tile, token m
         if (p.epilogue == W8A8_EPI_SWIGLU) {
-            for (int x = tid; x < 8 * p.M; x += kL4Warps * 32) {
-                const int r = x & 7, m = x >> 3;
-                p.Y[static_cast<size_t>(m) * (p.N / 2) + tile * 8 + r] = l4_swiglu(added(r, m), added(r + 8, m));
-            }
-        } else {
-            for (int x = tid; x < 16 * p.M; x += kL4Warps * 32) {
-                const int r = x & 15, m = x >> 4;
-                const size_t at = static_cast<size_t>(m) * p.N + tile * 16 + r;
-                if (tile * 16 + r < p.N) p.Y[at] = l4_plain(added(r, m), p.residual, at);
-            }
+            p.Y[static_cast<size_t>(m) * (p.N / 2) + at_tile * 8 + r] = l4_swiglu(v, up);
+        } else if (at_tile * 16 + r < p.N) {
+            const size_t at = static_cast<size_t>(m) * p.N + at_tile * 16 + r;
+            p.Y[at] = l4_plain(v, p.residual, at);
         }
-        parity ^= 1;  // (the next tile's sums go to the other buffer; its barrier comes before this one is written again)
     };
-    if (mine == 0) {  // fewer steps than warps: nothing to add, but every barrier to meet
-        for (int t = 0; t < n_tiles; ++t, tile += gridDim.x) finish_tile();
-        return;
-    }
-    for (int i0 = 0; i0 < total; i0 += U) {
+    const uint32_t row_off = row8 * kBoxBytes;  // (the swizzle turns a row's 16-byte places by row8, the same for row8 + 8)
+    const uint32_t codes = ptx::smem_u32(codes_s) + j4 * 16;
+    const uint32_t xs_at = ptx::smem_u32(xs_s) + 2 * j4 * 4;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool failed = false;
+#pragma unroll 1
+    for (int i = 0; i < n_mine; ++i) {
+        __half2 ws[P > 1 ? P : 1];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u >= total) break;
-            const int k = 32 * V * step + 8 * V * j4;
-            uint32_t a[V][4];
+        for (int x = 0; x < (P > 1 ? P : 1); ++x) ws[x] = ws_next[x];
+        const bool tile_ends = box + 1 == p.boxes;
+        if (i + 1 < n_mine) load_scales(tile_ends ? tile + 1 : tile, tile_ends ? 0 : box + 1);
+        if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&full_bar[warp][stage], phase)) && !failed &&
+            !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&full_bar[warp][stage], phase))) {
+            atomicExch(p.status, 950);
+            failed = true;  // (the numbers are void from here on; the barriers still run their course)
+        }
+        const uint32_t at = ring + stage * kBox + row_off;
+        int sum[T][4];
+        uint4 wide[2];
 #pragma unroll
-            for (int v = 0; v < V; ++v)
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w[2][2];  // [row half][word]
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t w = wbuf[u][half].w[v];
-                    a[v][half] = (w << 4) & 0xf0f0f0f0u;
-                    a[v][2 + half] = w & 0xf0f0f0f0u;
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t r = at + half * 8 * kBoxBytes;
+                if constexpr (P <= 2) {
+                    if (!(q & 1)) wide[half] = lds128(r + (((2 * q + j4) ^ row8) << 4));
+                    w[half][0] = q & 1 ? wide[half].z : wide[half].x;
+                    w[half][1] = q & 1 ? wide[half].w : wide[half].y;
+                } else if constexpr (P == 4) {
+                    const uint2 v = lds64(r + (((2 * q + (j4 >> 1)) ^ row8) << 4) + (j4 & 1) * 8);
+                    w[half][0] = v.x;
+                    w[half][1] = v.y;
+                } else {
+                    w[half][0] = lds32(r + (((2 * q) ^ row8) << 4) + j4 * 4);
+                    w[half][1] = lds32(r + (((2 * q + 1) ^ row8) << 4) + j4 * 4);
                 }
-            if (i0 + u + U < total) load(wbuf[u]);
+            }
+            uint32_t a[2][4];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                a[v][0] = (w[0][v] << 4) & 0xf0f0f0f0u;
+                a[v][1] = (w[1][v] << 4) & 0xf0f0f0f0u;
+                a[v][2] = w[0][v] & 0xf0f0f0f0u;
+                a[v][3] = w[1][v] & 0xf0f0f0f0u;
+            }
+            uint4 x[T];
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const int m = 8 * t + g8;
-                uint32_t x[2 * V];
-#pragma unroll
-                for (int v = 0; v < 2 * V; ++v) x[v] = 0u;
-                if (m < p.M && k < p.K) {
-                    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.Xq + static_cast<size_t>(m) * p.K + k);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const uint2 two = ptx::ld_result_v2(src + 2 * v);
-                        x[2 * v] = two.x;
-                        x[2 * v + 1] = two.y;
-                    }
-                }
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    mma_s8(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], __byte_perm(x[2 * v], x[2 * v + 1], 0x6420),
-                           __byte_perm(x[2 * v], x[2 * v + 1], 0x7531));
+                x[t] = {0u, 0u, 0u, 0u};
+                if (8 * t + g8 < p.M) x[t] = lds128(codes + ((4 * box + q) * p.M + 8 * t + g8) * 64);
             }
-            const int group = 32 * V * step / p.g;
-            const bool tile_ends = step + 1 == s1;
-            if (tile_ends || 32 * V * (step + 1) / p.g != group) {
-                const int row = tile * 16 + g8;
-                const float ws0 = row < p.N ? __half2float(p.w_scale[static_cast<size_t>(row) * p.G + group]) * 0.0625f : 0.0f;
-                const float ws1 = row + 8 < p.N ? __half2float(p.w_scale[static_cast<size_t>(row + 8) * p.G + group]) * 0.0625f : 0.0f;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const bool first = P == 8 || (v == 0 && (P == 4 || (P == 2 && !(q & 1)) || (P == 1 && q == 0)));
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
-                    const int m = 8 * t + 2 * j4;
-                    const float x0 = m < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
-                    const float x1 = m + 1 < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m + 1) * p.G + group) : 0.0f;
-                    acc[t][0] = fmaf(static_cast<float>(sum[t][0]) * ws0, x0, acc[t][0]);
-                    acc[t][1] = fmaf(static_cast<float>(sum[t][1]) * ws0, x1, acc[t][1]);
-                    acc[t][2] = fmaf(static_cast<float>(sum[t][2]) * ws1, x0, acc[t][2]);
-                    acc[t][3] = fmaf(static_cast<float>(sum[t][3]) * ws1, x1, acc[t][3]);
+                    const uint32_t b0 = v ? x[t].z : x[t].x, b1 = v ? x[t].w : x[t].y;
+                    if (first)
+                        mma_s8_first(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], b0, b1);
+                    else
+                        mma_s8(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], b0, b1);
+                }
+                if (P == 8 || (v == 1 && (P == 4 || (P == 2 && (q & 1)) || q == 3))) {  // promote
+                    const int pr = P == 8 ? 2 * q + v : P == 4 ? q : P == 2 ? q >> 1 : 0;
+                    float ws0, ws1;
+                    if constexpr (EXACT && P > 1) {
+                        ws0 = pr & 1 ? __high2float(ws[pr / 2]) : __low2float(ws[pr / 2]);
+                        ws1 = pr & 1 ? __high2float(ws[P / 2 + pr / 2]) : __low2float(ws[P / 2 + pr / 2]);
+                    } else {
+                        ws0 = __low2float(ws[pr]);
+                        ws1 = __high2float(ws[pr]);
+                    }
+                    ws0 *= 0.0625f;
+                    ws1 *= 0.0625f;
+                    const uint32_t xg = xs_at + group_of(box, pr) * (8 * T * 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[t][e] = 0;
+                    for (int t = 0; t < T; ++t) {
+                        const uint2 xx = lds64(xg + t * 32);
+                        const float x0 = __uint_as_float(xx.x), x1 = __uint_as_float(xx.y);
+                        acc[t][0] = fmaf(static_cast<float>(sum[t][0]) * ws0, x0, acc[t][0]);
+                        acc[t][1] = fmaf(static_cast<float>(sum[t][1]) * ws0, x1, acc[t][1]);
+                        acc[t][2] = fmaf(static_cast<float>(sum[t][2]) * ws1, x0, acc[t][2]);
+                        acc[t][3] = fmaf(static_cast<float>(sum[t][3]) * ws1, x1, acc[t][3]);
+                    }
                 }
             }
-            if (tile_ends) {
-                finish_tile();
-                tile += gridDim.x;
-                step = s0;
-            } else {
-                ++step;
-            }
         }
+        // ---- the stage is free ----
+        if (i + p.stages < n_mine) {
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && !failed) issue(stage);
+        }
+        if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+        if (tile_ends || i + 1 == n_mine) {
+            if (tile_ends && !head) {  // all of the tile
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int m = 8 * t + 2 * j4 + e;
+                        if (m < p.M) {
+                            emit(tile, row8, m, acc[t][e], acc[t][2 + e]);
+                            if (p.epilogue != W8A8_EPI_SWIGLU) emit(tile, row8 + 8, m, acc[t][2 + e], 0.0f);
+                        }
+                    }
+            } else {
+                float* const piece = piece_s + (2 * warp + (head ? 0 : 1)) * kPiece;
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) piece[(row8 + 4 * (e & 2)) * kCols + 8 * t + 2 * j4 + (e & 1)] = acc[t][e];
+            }
+            head = false;
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
+        }
+        if (tile_ends) {
+            ++tile;
+            box = 0;
+        } else {
+            ++box;
+        }
+    }
+    __syncthreads();
+
+    // ---- tiles that a border between warps cuts: borders in order, a tile at its first one ----
+    const bool swiglu = p.epilogue == W8A8_EPI_SWIGLU;
+    const int rows = swiglu ? 8 : 16;
+    auto run_at = [&](int w) { return static_cast<int>(static_cast<long long>(all) * w / kL4Warps); };
+    int done = -1;
+#pragma unroll 1
+    for (int w = 1; w < kL4Warps; ++w) {
+        const int border = run_at(w), cut = border / p.boxes;
+        if (border % p.boxes == 0 || cut == done) continue;
+        done = cut;
+        const int from = cut * p.boxes, to = from + p.boxes;
+        for (int x = tid; x < rows * p.M; x += kL4Warps * 32) {
+            const int r = x % rows, m = x / rows;
+            float v = 0.0f, up = 0.0f;
+            for (int w2 = w - 1; w2 < kL4Warps && run_at(w2) < to; ++w2) {
+                if (run_at(w2 + 1) <= from || run_at(w2 + 1) == run_at(w2)) continue;
+                const float* piece = piece_s + (2 * w2 + (run_at(w2) > from ? 0 : 1)) * kPiece;
+                v += piece[r * kCols + m];
+                if (swiglu) up += piece[(r + 8) * kCols + m];
+            }
+            emit(t0 + cut, r, m, v, up);
+        }
+    }
+    if (failed) {  // copies that may still be on their way land before the CTA goes
+#pragma unroll 1
+        for (int w = 0; w < 1000; ++w) __nanosleep(1000);
     }
 }
 
@@ -267,46 +434,78 @@ __global__ void __launch_bounds__(256) unpack_weight4_kernel(const uint8_t* code
 }
 
 template <class... P, class... A>
-cudaError_t launch_l4(int ctas, cudaStream_t stream, void (*kern)(P...), const A&... args) {
+cudaError_t launch_l4(SmemAttribute* attribute, int ctas, size_t smem, cudaStream_t stream, void (*kern)(P...), const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled(kPdlLinear) ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, args...);
+    return attribute ? launch_with_smem(*attribute, kL4MaxSmem, cfg, kern, args...) : cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <int V>
-cudaError_t launch_rows4(const L4Params& p, cudaStream_t stream) {
-    const int room = 4 * device_sms(), ctas = p.tiles < room ? p.tiles : room;
-    return p.M <= 8 ? launch_l4(ctas, stream, linear4_kernel<1, V>, p) : p.M <= 16 ? launch_l4(ctas, stream, linear4_kernel<2, V>, p)
-                                                                                   : launch_l4(ctas, stream, linear4_kernel<4, V>, p);
+// Stages of a warp's ring: as many as leave room for two CTAs on an SM (four at most are worth their space), else for one.
+template <int T>
+int l4_stages(int M, int K, int G) {
+    for (size_t room : {static_cast<size_t>(112 * 1024), static_cast<size_t>(kL4MaxSmem)})
+        for (int stages = room > 112 * 1024 ? 8 : 4; stages >= (room > 112 * 1024 ? 2 : 3); --stages)
+            if (l4_smem<T>(M, K, G, stages) <= room) return stages;
+    return 0;
+}
+int l4_stages(int M, int K, int G) { return M > 16 ? l4_stages<4>(M, K, G) : M > 8 ? l4_stages<2>(M, K, G) : l4_stages<1>(M, K, G); }
+
+template <int T, int P, bool EXACT>
+cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream) {
+    static SmemAttribute attribute;
+    p.stages = l4_stages<T>(p.M, p.K, p.G);
+    const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages);
+    return launch_l4(&attribute, gemv_packed_ctas(p.tiles, device_sms(), smem <= 112 * 1024), smem, stream, linear4_kernel<T, P, EXACT>, map, p);
+}
+template <int T, bool EXACT>
+cudaError_t launch_rows4(const L4Params& p, const CUtensorMap& map, int P, cudaStream_t stream) {
+    return P == 1   ? launch_boxes<T, 1, EXACT>(p, map, stream)
+           : P == 2 ? launch_boxes<T, 2, EXACT>(p, map, stream)
+           : P == 4 ? launch_boxes<T, 4, EXACT>(p, map, stream)
+                    : launch_boxes<T, 8, EXACT>(p, map, stream);
 }
 
 }  // namespace
 
 int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t* Xq, const float* Xs, __half* Y, const __half* residual, int M, int N,
-                   int K, int epilogue, cudaStream_t stream) {
+                   int K, int epilogue, int* status, cudaStream_t stream) {
+    if (M == 0) return W8A8_OK;
     const int g = norm_group(K, group), G = num_groups(K, group);
     const bool swiglu = epilogue == W8A8_EPI_SWIGLU;
     const int columns = swiglu ? N / 2 : N;
-    const bool fast = K % 32 == 0 && g % 32 == 0 && ((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(Xq)) & 15u) == 0;
-    for (int m0 = 0; m0 < M; m0 += 32) {  // (32 rows a launch; the weights are streamed once for each)
-        const int m = fast ? (M - m0 < 32 ? M - m0 : 32) : M;
+    const int P = g % 256 == 0 ? 1 : g % 128 == 0 ? 2 : g % 64 == 0 ? 4 : 8;
+    const bool exact = g == kBoxK / P && K % kBoxK == 0 && (reinterpret_cast<uintptr_t>(w_scale) & (2 * P - 1)) == 0;
+    // rows of a launch: as many as fit shared memory; the weights are streamed once per launch
+    int rows = 32;
+    while (rows > 1 && l4_stages(rows, K, G) == 0) rows /= 2;
+    const bool fast = K % 32 == 0 && g % 32 == 0 && ((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(Xq)) & 15u) == 0 &&
+                      l4_stages(rows, K, G) > 0;
+    CUtensorMap map;
+    if (fast)
+        if (int rc = make_tensor_map_2d_u8(&map, W, K / 2, N, K / 2, kBoxBytes, kBoxRows, 1)) return rc;
+    for (int m0 = 0; m0 < M; m0 += rows) {
+        const int m = fast ? (M - m0 < rows ? M - m0 : rows) : M;
         L4Params p = {static_cast<const uint8_t*>(W), w_scale, Xq + static_cast<size_t>(m0) * K, Xs + static_cast<size_t>(m0) * G,
                       Y + static_cast<size_t>(m0) * columns, residual ? residual + static_cast<size_t>(m0) * N : nullptr, m, N, K, g, G, epilogue,
-                      (N + 15) / 16};
+                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, status};
         cudaError_t e;
         if (fast) {
-            e = g % 128 == 0 ? launch_rows4<4>(p, stream) : g % 64 == 0 ? launch_rows4<2>(p, stream) : launch_rows4<1>(p, stream);
+            if (exact)
+                e = m <= 8 ? launch_rows4<1, true>(p, map, P, stream) : m <= 16 ? launch_rows4<2, true>(p, map, P, stream) : launch_rows4<4, true>(p, map, P, stream);
+            else
+                e = m <= 8 ? launch_rows4<1, false>(p, map, P, stream) : m <= 16 ? launch_rows4<2, false>(p, map, P, stream) : launch_rows4<4, false>(p, map, P, stream);
         } else {
             const long long warps = static_cast<long long>(M) * columns, ctas = (warps + 7) / 8;
             if (ctas > 0x7fffffffll) return fail(W8A8_ERR_UNSUPPORTED, "linear4_q: M=%d N=%d is too large for this shape's kernel", M, N);
-            e = launch_l4(static_cast<int>(ctas), stream, linear4_generic_kernel, p);
+            e = launch_l4(nullptr, static_cast<int>(ctas), 0, stream, linear4_generic_kernel, p);
         }
         if (e != cudaSuccess) return fail(W8A8_ERR_CUDA, "linear4_q launch: %s", cudaGetErrorString(e));
         if (!fast) break;
