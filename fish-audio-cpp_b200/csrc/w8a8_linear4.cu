@@ -43,6 +43,7 @@ struct L4Params {
     int tiles;   // of 16 rows
     int boxes;   // per tile
     int stages;  // of a warp's ring
+    int pitch;   // of a row of codes in shared memory
     int* status;
 };
 
@@ -86,20 +87,22 @@ __device__ __forceinline__ __half l4_plain(float v, const __half* residual, size
 // T token tiles of 8; P promotes per box (256 / P channels each, all in one group); EXACT: groups of 256 / P channels, K in whole boxes and
 // the scales of a box in one aligned read.
 // Shared memory: rings [warps][stages][box]; pieces fp32 [warps][2][16][8 T + 1]; activation scales fp32 [G][8 T]; their codes
-// [box][quarter of 64 channels][M][lane of 4][16 bytes].
+// [M][pitch], a pitch at which the rows that lanes read together lie in different banks.
+// (reads run on to the end of the last box: what lies behind K meets weights of zero)
+inline int l4_pitch(int K, int P) { return (K + 127) / 128 * 128 + (P <= 2 ? 16 : P == 4 ? 64 : 32); }
 template <int T>
 constexpr int l4_piece_floats() { return 16 * (8 * T + 1); }
 template <int T>
 size_t l4_smem(int M, int K, int G, int stages) {
     return 1024 + static_cast<size_t>(kL4Warps) * stages * kBox + 2 * kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(G) * 8 * T * 4 +
-           static_cast<size_t>((K + kBoxK - 1) / kBoxK) * kBoxK * M;
+           static_cast<size_t>(l4_pitch(K, 4)) * M + kBoxK;
 }
 
 template <int T, int P, bool EXACT>
 __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ L4Params p) {
     constexpr int kPiece = l4_piece_floats<T>(), kCols = 8 * T + 1;
     extern __shared__ unsigned char l4_smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kL4Warps][8];
+    __shared__ __align__(8) uint64_t full_bar[kL4Warps][8], codes_bar;
     unsigned char* const base = l4_smem_raw + ((1024u - (ptx::smem_u32(l4_smem_raw) & 1023u)) & 1023u);  // (the swizzle repeats every 1024 bytes)
     float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kBox);
     float* const xs_s = piece_s + 2 * kL4Warps * kPiece;
@@ -131,6 +134,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     };
     if (lane == 0) {
         for (int i = 0; i < p.stages; ++i) ptx::mbar_init(&full_bar[warp][i], 1);
+        if (warp == 0) ptx::mbar_init(&codes_bar, 1);
         ptx::fence_barrier_init();
         ptx::fence_proxy_async();
         for (int i = 0; i < min(p.stages, n_mine); ++i) issue(i);
@@ -165,38 +169,30 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
 
-    // ---- the activations, in the order of the fragments ----
-    {
-        const int per_row = p.boxes * 16;  // lanes' 16-byte shares of a row
-        for (int m = warp; m < p.M; m += kL4Warps)
-            for (int x = lane; x < per_row; x += 32) {
-                const int quarter = x >> 2, j = x & 3;
-                int k[2];  // of the two words' eight channels
-                if (P <= 2) {
-                    k[0] = (quarter >> 1) * 128 + j * 32 + (quarter & 1) * 16;
-                    k[1] = k[0] + 8;
-                } else if (P == 4) {
-                    k[0] = quarter * 64 + j * 16;
-                    k[1] = k[0] + 8;
-                } else {
-                    k[0] = quarter * 64 + j * 8;
-                    k[1] = k[0] + 32;
-                }
-                uint32_t c[4];
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    uint2 two = {0u, 0u};
-                    if (k[v] < p.K) two = ptx::ld_result_v2(p.Xq + static_cast<size_t>(m) * p.K + k[v]);
-                    c[2 * v] = __byte_perm(two.x, two.y, 0x6420);
-                    c[2 * v + 1] = __byte_perm(two.x, two.y, 0x7531);
-                }
-                *reinterpret_cast<uint4*>(codes_s + (quarter * p.M + m) * 64 + j * 16) = {c[0], c[1], c[2], c[3]};
-            }
-        for (int x = tid; x < p.G * 8 * T; x += kL4Warps * 32) {
-            const int group = x / (8 * T), m = x % (8 * T);
-            xs_s[x] = m < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
-        }
+    // ---- the activations: rows as they are, each by one bulk copy; then the eight channels of a word even ones first, in place ----
+    if (tid == 0) {
+        ptx::mbar_arrive_expect_tx(&codes_bar, p.M * p.K);
+        for (int m = 0; m < p.M; ++m)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ptx::smem_u32(codes_s) + m * p.pitch),
+                         "l"(p.Xq + static_cast<size_t>(m) * p.K), "r"(p.K), "r"(ptx::smem_u32(&codes_bar))
+                         : "memory");
     }
+    for (int x = tid; x < p.G * 8 * T; x += kL4Warps * 32) {
+        const int group = x / (8 * T), m = x % (8 * T);
+        xs_s[x] = m < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
+    }
+    bool failed = false;
+    if (!ptx::mbar_wait_bounded(&codes_bar, 0)) {
+        atomicExch(p.status, 951);
+        failed = true;
+    }
+    failed = __syncthreads_or(failed);
+    for (int m = warp; m < p.M; m += kL4Warps)
+        for (int x = lane * 16; x < p.K; x += 32 * 16) {
+            uint4* at = reinterpret_cast<uint4*>(codes_s + m * p.pitch + x);
+            const uint4 v = *at;
+            *at = {__byte_perm(v.x, v.y, 0x6420), __byte_perm(v.x, v.y, 0x7531), __byte_perm(v.z, v.w, 0x6420), __byte_perm(v.z, v.w, 0x7531)};
+        }
     __syncthreads();
 
     // ---- the run ----
@@ -214,11 +210,10 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         }
     };
     const uint32_t row_off = row8 * kBoxBytes;  // (the swizzle turns a row's 16-byte places by row8, the same for row8 + 8)
-    const uint32_t codes = ptx::smem_u32(codes_s) + j4 * 16;
+    const uint32_t codes = ptx::smem_u32(codes_s) + g8 * p.pitch + j4 * (P <= 2 ? 32 : P == 4 ? 16 : 8);  // (rows behind the last: not read)
     const uint32_t xs_at = ptx::smem_u32(xs_s) + 2 * j4 * 4;
     int stage = 0;
     uint32_t phase = 0;
-    bool failed = false;
 #pragma unroll 1
     for (int i = 0; i < n_mine; ++i) {
         __half2 ws[P > 1 ? P : 1];
@@ -265,7 +260,17 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
 #pragma unroll
             for (int t = 0; t < T; ++t) {
                 x[t] = {0u, 0u, 0u, 0u};
-                if (8 * t + g8 < p.M) x[t] = lds128(codes + ((4 * box + q) * p.M + 8 * t + g8) * 64);
+                if (8 * t + g8 < p.M) {
+                    const uint32_t from = codes + 8 * t * p.pitch + box * kBoxK + q * 64;
+                    if constexpr (P <= 2) {
+                        x[t] = lds128(from - (q & 1) * 48);  // quarters 0, 1: the first and second 16 of the lane's 32 channels
+                    } else if constexpr (P == 4) {
+                        x[t] = lds128(from);
+                    } else {
+                        const uint2 a = lds64(from), b = lds64(from + 32);
+                        x[t] = {a.x, a.y, b.x, b.y};
+                    }
+                }
             }
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
@@ -347,28 +352,31 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     }
     __syncthreads();
 
-    // ---- tiles that a border between warps cuts: borders in order, a tile at its first one ----
+    // ---- tiles that a border between warps cuts: lane w looks at the border in front of warp w; a tile counts at its first border ----
     const bool swiglu = p.epilogue == W8A8_EPI_SWIGLU;
-    const int rows = swiglu ? 8 : 16;
-    auto run_at = [&](int w) { return static_cast<int>(static_cast<long long>(all) * w / kL4Warps); };
-    int done = -1;
+    auto run_at = [&](int w) { return static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(all)) * w / kL4Warps); };
+    const int border = run_at(min(lane, kL4Warps)), cut_at = border / p.boxes;
+    const bool cuts = lane > 0 && lane < kL4Warps && border != cut_at * p.boxes;
+    const bool cuts_before = __shfl_up_sync(0xffffffffu, cuts, 1);
+    const int cut_before = __shfl_up_sync(0xffffffffu, cut_at, 1);
+    const uint32_t cut_tiles = __ballot_sync(0xffffffffu, cuts && !(lane > 1 && cuts_before && cut_before == cut_at));
+    const int rows_log = swiglu ? 3 : 4, elements = p.M << rows_log;
 #pragma unroll 1
-    for (int w = 1; w < kL4Warps; ++w) {
-        const int border = run_at(w), cut = border / p.boxes;
-        if (border % p.boxes == 0 || cut == done) continue;
-        done = cut;
-        const int from = cut * p.boxes, to = from + p.boxes;
-        for (int x = tid; x < rows * p.M; x += kL4Warps * 32) {
-            const int r = x % rows, m = x / rows;
-            float v = 0.0f, up = 0.0f;
-            for (int w2 = w - 1; w2 < kL4Warps && run_at(w2) < to; ++w2) {
-                if (run_at(w2 + 1) <= from || run_at(w2 + 1) == run_at(w2)) continue;
-                const float* piece = piece_s + (2 * w2 + (run_at(w2) > from ? 0 : 1)) * kPiece;
-                v += piece[r * kCols + m];
-                if (swiglu) up += piece[(r + 8) * kCols + m];
-            }
-            emit(t0 + cut, r, m, v, up);
+    for (int x = tid, c = 0; x < elements * __popc(cut_tiles); x += kL4Warps * 32) {
+        while (x >= (c + 1) * elements) ++c;
+        uint32_t rest = cut_tiles;
+        for (int y = 0; y < c; ++y) rest &= rest - 1;
+        const int w = __ffs(rest) - 1, cut = run_at(w) / p.boxes, from = cut * p.boxes, to = from + p.boxes;
+        const int r = (x - c * elements) & ((1 << rows_log) - 1), m = (x - c * elements) >> rows_log;
+        float v = 0.0f, up = 0.0f;
+#pragma unroll 1
+        for (int w2 = w - 1; w2 < kL4Warps && run_at(w2) < to; ++w2) {
+            if (run_at(w2 + 1) <= from || run_at(w2 + 1) == run_at(w2)) continue;
+            const float* piece = piece_s + (2 * w2 + (run_at(w2) > from ? 0 : 1)) * kPiece;
+            v += piece[r * kCols + m];
+            if (swiglu) up += piece[(r + 8) * kCols + m];
         }
+        emit(t0 + cut, r, m, v, up);
     }
     if (failed) {  // copies that may still be on their way land before the CTA goes
 #pragma unroll 1
@@ -495,7 +503,7 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
         const int m = fast ? (M - m0 < rows ? M - m0 : rows) : M;
         L4Params p = {static_cast<const uint8_t*>(W), w_scale, Xq + static_cast<size_t>(m0) * K, Xs + static_cast<size_t>(m0) * G,
                       Y + static_cast<size_t>(m0) * columns, residual ? residual + static_cast<size_t>(m0) * N : nullptr, m, N, K, g, G, epilogue,
-                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, status};
+                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), status};
         cudaError_t e;
         if (fast) {
             if (exact)
