@@ -73,6 +73,10 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ uint4 evens_first(uint4 v) {
+    return {__byte_perm(v.x, v.y, 0x6420), __byte_perm(v.x, v.y, 0x7531), __byte_perm(v.z, v.w, 0x6420), __byte_perm(v.z, v.w, 0x7531)};
+}
+
 // What the epilogues make of a finished fp32 sum (roundings of the reference's separate kernels, ffn_activations.cu:12-17, :35-45).
 __device__ __forceinline__ __half l4_swiglu(float gate, float up) {
     const float x = __half2float(__float2half_rn(gate));
@@ -93,12 +97,12 @@ inline int l4_pitch(int K, int P) { return (K + 127) / 128 * 128 + (P <= 2 ? 16 
 template <int T>
 constexpr int l4_piece_floats() { return 16 * (8 * T + 1); }
 template <int T>
-size_t l4_smem(int M, int K, int G, int stages) {
+size_t l4_smem(int M, int K, int G, int stages, bool direct) {
     return 1024 + static_cast<size_t>(kL4Warps) * stages * kBox + 2 * kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(G) * 8 * T * 4 +
-           static_cast<size_t>(l4_pitch(K, 4)) * M + kBoxK;
+           (direct ? 0 : static_cast<size_t>(l4_pitch(K, 4)) * M + kBoxK);
 }
 
-template <int T, int P, bool EXACT>
+template <int T, int P, bool EXACT, bool DIRECT>
 __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ L4Params p) {
     constexpr int kPiece = l4_piece_floats<T>(), kCols = 8 * T + 1;
     extern __shared__ unsigned char l4_smem_raw[];
@@ -142,11 +146,15 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     // weight scales of the box that comes next, rows row8 and row8 + 8
     __half2 ws_next[P > 1 ? P : 1];  // EXACT, P > 1: [row half][P / 2 pairs of groups]; else one {row, row + 8} pair per promote
     auto group_of = [&](int bx, int pr) { return EXACT ? bx * P + pr : min(p.G - 1, (bx * kBoxK + pr * (kBoxK / P)) / p.g); };
-    auto load_scales = [&](int tl, int bx) {
-        const size_t r0 = static_cast<size_t>(min(tl * 16 + row8, p.N - 1)) * p.G, r1 = static_cast<size_t>(min(tl * 16 + row8 + 8, p.N - 1)) * p.G;
+    const __half *ws_row0 = nullptr, *ws_row1 = nullptr;  // of the tile that the next box belongs to
+    auto scale_rows = [&](int tl) {
+        ws_row0 = p.w_scale + static_cast<size_t>(min(tl * 16 + row8, p.N - 1)) * p.G;
+        ws_row1 = p.w_scale + static_cast<size_t>(min(tl * 16 + row8 + 8, p.N - 1)) * p.G;
+    };
+    auto load_scales = [&](int bx) {
         if constexpr (EXACT && P > 1) {
             uint32_t* w = reinterpret_cast<uint32_t*>(ws_next);
-            const __half *a = p.w_scale + r0 + bx * P, *b = p.w_scale + r1 + bx * P;
+            const __half *a = ws_row0 + bx * P, *b = ws_row1 + bx * P;
             if constexpr (P == 2) {
                 w[0] = __ldg(reinterpret_cast<const uint32_t*>(a));
                 w[1] = __ldg(reinterpret_cast<const uint32_t*>(b));
@@ -161,16 +169,45 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
 #pragma unroll
             for (int pr = 0; pr < P; ++pr) {
                 const int gr = group_of(bx, pr);
-                ws_next[pr] = __halves2half2(p.w_scale[r0 + gr], p.w_scale[r1 + gr]);
+                ws_next[pr] = __halves2half2(ws_row0[gr], ws_row1[gr]);
             }
         }
     };
-    if (n_mine > 0) load_scales(tile, box);
+    if (n_mine > 0) {
+        scale_rows(tile);
+        load_scales(box);
+    }
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
 
-    // ---- the activations: rows as they are, each by one bulk copy; then the eight channels of a word even ones first, in place ----
-    if (tid == 0) {
+    // ---- the activations ----
+    // DIRECT: a lane's codes of a box in registers, asked for a box ahead. Else rows as they are in shared memory, each by one bulk copy, then the eight
+    // channels of a word even ones first, in place.
+    uint4 x_next[DIRECT ? T : 1][4];
+    auto load_codes = [&](int bx) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int8_t* row = p.Xq + static_cast<size_t>(min(8 * t + g8, p.M - 1)) * p.K;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint4& x = x_next[DIRECT ? t : 0][q];
+                x = {0u, 0u, 0u, 0u};
+                const int k = bx * kBoxK + (P <= 2 ? (q >> 1) * 128 + j4 * 32 + (q & 1) * 16 : P == 4 ? q * 64 + j4 * 16 : q * 64 + j4 * 8);
+                if constexpr (P <= 4) {
+                    if (EXACT || k < p.K) x = ptx::ld_result_v4(row + k);
+                } else {
+                    uint2 a = {0u, 0u}, b = {0u, 0u};
+                    if (EXACT || k < p.K) a = ptx::ld_result_v2(row + k);
+                    if (EXACT || k + 32 < p.K) b = ptx::ld_result_v2(row + k + 32);
+                    x = {a.x, a.y, b.x, b.y};
+                }
+            }
+        }
+    };
+    bool failed = false;
+    if constexpr (DIRECT) {
+        if (n_mine > 0) load_codes(box);
+    } else if (tid == 0) {
         ptx::mbar_arrive_expect_tx(&codes_bar, p.M * p.K);
         for (int m = 0; m < p.M; ++m)
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ptx::smem_u32(codes_s) + m * p.pitch),
@@ -181,18 +218,18 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         const int group = x / (8 * T), m = x % (8 * T);
         xs_s[x] = m < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
     }
-    bool failed = false;
-    if (!ptx::mbar_wait_bounded(&codes_bar, 0)) {
-        atomicExch(p.status, 951);
-        failed = true;
-    }
-    failed = __syncthreads_or(failed);
-    for (int m = warp; m < p.M; m += kL4Warps)
-        for (int x = lane * 16; x < p.K; x += 32 * 16) {
-            uint4* at = reinterpret_cast<uint4*>(codes_s + m * p.pitch + x);
-            const uint4 v = *at;
-            *at = {__byte_perm(v.x, v.y, 0x6420), __byte_perm(v.x, v.y, 0x7531), __byte_perm(v.z, v.w, 0x6420), __byte_perm(v.z, v.w, 0x7531)};
+    if constexpr (!DIRECT) {
+        if (!ptx::mbar_wait_bounded(&codes_bar, 0)) {
+            atomicExch(p.status, 951);
+            failed = true;
         }
+        failed = __syncthreads_or(failed);
+        for (int m = warp; m < p.M; m += kL4Warps)
+            for (int x = lane * 16; x < p.K; x += 32 * 16) {
+                uint4* at = reinterpret_cast<uint4*>(codes_s + m * p.pitch + x);
+                *at = evens_first(*at);
+            }
+    }
     __syncthreads();
 
     // ---- the run ----
@@ -210,7 +247,10 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         }
     };
     const uint32_t row_off = row8 * kBoxBytes;  // (the swizzle turns a row's 16-byte places by row8, the same for row8 + 8)
-    const uint32_t codes = ptx::smem_u32(codes_s) + g8 * p.pitch + j4 * (P <= 2 ? 32 : P == 4 ? 16 : 8);  // (rows behind the last: not read)
+    uint32_t codes[T];  // (fragment rows behind the last row of X read that one: what becomes of them is not stored)
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+        codes[t] = ptx::smem_u32(codes_s) + min(8 * t + g8, p.M - 1) * p.pitch + j4 * (P <= 2 ? 32 : P == 4 ? 16 : 8);
     const uint32_t xs_at = ptx::smem_u32(xs_s) + 2 * j4 * 4;
     int stage = 0;
     uint32_t phase = 0;
@@ -220,7 +260,10 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
 #pragma unroll
         for (int x = 0; x < (P > 1 ? P : 1); ++x) ws[x] = ws_next[x];
         const bool tile_ends = box + 1 == p.boxes;
-        if (i + 1 < n_mine) load_scales(tile_ends ? tile + 1 : tile, tile_ends ? 0 : box + 1);
+        if (i + 1 < n_mine) {
+            if (tile_ends) scale_rows(tile + 1);
+            load_scales(tile_ends ? 0 : box + 1);
+        }
         if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&full_bar[warp][stage], phase)) && !failed &&
             !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&full_bar[warp][stage], phase))) {
             atomicExch(p.status, 950);
@@ -229,6 +272,14 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         const uint32_t at = ring + stage * kBox + row_off;
         int sum[T][4];
         uint4 wide[2];
+        uint4 x_now[DIRECT ? T : 1][4];
+        if constexpr (DIRECT) {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x_now[t][q] = x_next[t][q];
+            if (i + 1 < n_mine) load_codes(tile_ends ? 0 : box + 1);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             uint32_t w[2][2];  // [row half][word]
@@ -259,17 +310,16 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
             uint4 x[T];
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                x[t] = {0u, 0u, 0u, 0u};
-                if (8 * t + g8 < p.M) {
-                    const uint32_t from = codes + 8 * t * p.pitch + box * kBoxK + q * 64;
-                    if constexpr (P <= 2) {
-                        x[t] = lds128(from - (q & 1) * 48);  // quarters 0, 1: the first and second 16 of the lane's 32 channels
-                    } else if constexpr (P == 4) {
-                        x[t] = lds128(from);
-                    } else {
-                        const uint2 a = lds64(from), b = lds64(from + 32);
-                        x[t] = {a.x, a.y, b.x, b.y};
-                    }
+                const uint32_t from = codes[t] + box * kBoxK + q * 64;
+                if constexpr (DIRECT) {
+                    x[t] = evens_first(x_now[t][q]);
+                } else if constexpr (P <= 2) {
+                    x[t] = lds128(from - (q & 1) * 48);  // quarters 0, 1: the first and second 16 of the lane's 32 channels
+                } else if constexpr (P == 4) {
+                    x[t] = lds128(from);
+                } else {
+                    const uint2 a = lds64(from), b = lds64(from + 32);
+                    x[t] = {a.x, a.y, b.x, b.y};
                 }
             }
 #pragma unroll
@@ -456,22 +506,36 @@ cudaError_t launch_l4(SmemAttribute* attribute, int ctas, size_t smem, cudaStrea
     return attribute ? launch_with_smem(*attribute, kL4MaxSmem, cfg, kern, args...) : cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// Stages of a warp's ring: as many as leave room for two CTAs on an SM (four at most are worth their space), else for one.
+// Stages of a warp's ring: as many as leave room for two CTAs on an SM (more than four are not worth their space), else for one; 0: no room.
+constexpr size_t kHalfSm = 112 * 1024;
 template <int T>
-int l4_stages(int M, int K, int G) {
-    for (size_t room : {static_cast<size_t>(112 * 1024), static_cast<size_t>(kL4MaxSmem)})
-        for (int stages = room > 112 * 1024 ? 8 : 4; stages >= (room > 112 * 1024 ? 2 : 3); --stages)
-            if (l4_smem<T>(M, K, G, stages) <= room) return stages;
+int l4_stages(int M, int K, int G, bool direct) {
+    for (int stages = 4; stages >= 2; --stages)
+        if (l4_smem<T>(M, K, G, stages, direct) <= kHalfSm) return stages;
+    for (int stages = 8; stages >= 2; --stages)
+        if (l4_smem<T>(M, K, G, stages, direct) <= kL4MaxSmem) return stages;
     return 0;
 }
-int l4_stages(int M, int K, int G) { return M > 16 ? l4_stages<4>(M, K, G) : M > 8 ? l4_stages<2>(M, K, G) : l4_stages<1>(M, K, G); }
+int l4_stages(int M, int K, int G, bool direct) {
+    return M > 16 ? l4_stages<4>(M, K, G, direct) : M > 8 ? l4_stages<2>(M, K, G, direct) : l4_stages<1>(M, K, G, direct);
+}
 
+// Codes in shared memory, but where they leave no room for two CTAs on an SM (eight rows of 9728 channels on 160 tiles: 10.7 us, from global memory
+// 8.1; where there is room shared memory is as good or better: one row 6.9 and 7.6, sixteen rows of 2560 channels on 1216 tiles 11.8 and 14.0).
 template <int T, int P, bool EXACT>
 cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream) {
-    static SmemAttribute attribute;
-    p.stages = l4_stages<T>(p.M, p.K, p.G);
-    const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages);
-    return launch_l4(&attribute, gemv_packed_ctas(p.tiles, device_sms(), smem <= 112 * 1024), smem, stream, linear4_kernel<T, P, EXACT>, map, p);
+    static SmemAttribute attribute[2];
+    const int sms = device_sms();
+    if constexpr (T <= 2) {
+        if (l4_smem<T>(p.M, p.K, p.G, 2, false) > kHalfSm) {
+            p.stages = l4_stages<T>(p.M, p.K, p.G, true);
+            const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, true);
+            return launch_l4(&attribute[1], gemv_packed_ctas(p.tiles, sms, smem <= kHalfSm), smem, stream, linear4_kernel<T, P, EXACT, true>, map, p);
+        }
+    }
+    p.stages = l4_stages<T>(p.M, p.K, p.G, false);
+    const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, false);
+    return launch_l4(&attribute[0], gemv_packed_ctas(p.tiles, sms, smem <= kHalfSm), smem, stream, linear4_kernel<T, P, EXACT, false>, map, p);
 }
 template <int T, bool EXACT>
 cudaError_t launch_rows4(const L4Params& p, const CUtensorMap& map, int P, cudaStream_t stream) {
@@ -493,9 +557,9 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
     const bool exact = g == kBoxK / P && K % kBoxK == 0 && (reinterpret_cast<uintptr_t>(w_scale) & (2 * P - 1)) == 0;
     // rows of a launch: as many as fit shared memory; the weights are streamed once per launch
     int rows = 32;
-    while (rows > 1 && l4_stages(rows, K, G) == 0) rows /= 2;
+    while (rows > 1 && l4_stages(rows, K, G, rows <= 16) == 0) rows /= 2;
     const bool fast = K % 32 == 0 && g % 32 == 0 && ((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(Xq)) & 15u) == 0 &&
-                      l4_stages(rows, K, G) > 0;
+                      l4_stages(rows, K, G, rows <= 16) > 0;
     CUtensorMap map;
     if (fast)
         if (int rc = make_tensor_map_2d_u8(&map, W, K / 2, N, K / 2, kBoxBytes, kBoxRows, 1)) return rc;
