@@ -587,8 +587,8 @@ int w8a8_kv4_write(w8a8_ctx* ctx, const void* qkv, const void* q_norm_w, const v
     if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(W8A8_ERR_INVALID_ARG, "kv4_write: q_norm_w and k_norm_w go together");
     if ((freqs == nullptr) != (positions == nullptr)) return fail(W8A8_ERR_INVALID_ARG, "kv4_write: freqs and positions go together");
     if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w) |
-         reinterpret_cast<uintptr_t>(q_out)) & 7u)
-        return fail(W8A8_ERR_INVALID_ARG, "kv4_write: qkv, the norm weights and q_out must be 8-byte aligned");
+         reinterpret_cast<uintptr_t>(q_out)) & 15u)
+        return fail(W8A8_ERR_INVALID_ARG, "kv4_write: qkv, the norm weights and q_out must be 16-byte aligned");
     if (int rc = check_device(ctx, "kv4_write")) return rc;
     return launch_kv4_write(static_cast<const __half*>(qkv), static_cast<const __half*>(q_norm_w), static_cast<const __half*>(k_norm_w), eps, freqs,
                             positions, reinterpret_cast<const long long*>(slots), cache, n_blocks, layer, n_layers, tokens, n_q_heads, n_kv_heads,
@@ -599,8 +599,8 @@ int w8a8_kv4_read(w8a8_ctx* ctx, const void* cache, int n_blocks, const int64_t*
                   int head_dim, int group_size, void* k_out, void* v_out, void* stream) {
     if (int rc = check_kv4(ctx, "kv4_read", cache, n_blocks, layer, n_layers, tokens, 0, n_kv_heads, head_dim, group_size)) return rc;
     if (tokens > 0 && (!slots || (!k_out && !v_out))) return fail(W8A8_ERR_INVALID_ARG, "kv4_read: null pointer");
-    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 7u)
-        return fail(W8A8_ERR_INVALID_ARG, "kv4_read: k_out and v_out must be 8-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
+        return fail(W8A8_ERR_INVALID_ARG, "kv4_read: k_out and v_out must be 16-byte aligned");
     if (int rc = check_device(ctx, "kv4_read")) return rc;
     return launch_kv4_read(cache, n_blocks, reinterpret_cast<const long long*>(slots), layer, n_layers, tokens, n_kv_heads, group_size,
                            static_cast<__half*>(k_out), static_cast<__half*>(v_out), static_cast<cudaStream_t>(stream));

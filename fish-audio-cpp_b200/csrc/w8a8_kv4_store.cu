@@ -5,7 +5,9 @@
 // the fp16 cache would hold, in groups of 4 bits (w8a8_q4.cuh). Tokens are named by slots, so that a prompt's rows and a
 // decode step's go the same way, and rows with a negative slot (a captured step's empty rows) are left alone, their q too.
 //
-// Bound: bytes for prompts (2 (n_q + 2 n_kv) 128 read and 2 n_q 128 written per token), latency for a decode step.
+// Bound: for prompts instructions and bytes alike (2 (n_q + 2 n_kv) 128 read and 2 n_q 128 written per token), latency for a decode step.
+// Half a warp holds a head, eight neighbouring channels a lane: 16-byte reads and writes, a K word a lane, and of the norm's tree three levels
+// in the lane. A warp takes one token and one pair of heads after another, so that the angles are made once.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 #include "w8a8_q4.cuh"
@@ -27,167 +29,203 @@ struct StoreParams {
     unsigned char* cache;
     int tokens, n_q, n_kv, layer, n_layers;
     __half* q_out;           // [tokens, n_q, 128] or null
-    int heads_per_warp;
+    int pairs_per_warp;
 };
 
-// Lane l holds channels 4 l .. 4 l + 3 of a head.
+// Lane l of a half holds channels 8 l .. 8 l + 7 of a head, as four fp16 pairs.
 struct Row {
-    __half h[4];
+    __half2 h[4];
 };
-__device__ __forceinline__ Row load_row(const __half* src, int lane) {
-    const uint2 v = ptx::ld_result_v2(src + 4 * lane);
-    const __half2 a = *reinterpret_cast<const __half2*>(&v.x), b = *reinterpret_cast<const __half2*>(&v.y);
-    return {{__low2half(a), __high2half(a), __low2half(b), __high2half(b)}};
+__device__ __forceinline__ Row load_row(const __half* src, int l) {
+    const uint4 v = ptx::ld_result_v4(src + 8 * l);
+    Row r;
+    r.h[0] = *reinterpret_cast<const __half2*>(&v.x);
+    r.h[1] = *reinterpret_cast<const __half2*>(&v.y);
+    r.h[2] = *reinterpret_cast<const __half2*>(&v.z);
+    r.h[3] = *reinterpret_cast<const __half2*>(&v.w);
+    return r;
+}
+__device__ __forceinline__ void store_row(__half* dst, int l, const Row& r) {
+    uint4 v;
+    v.x = *reinterpret_cast<const uint32_t*>(&r.h[0]);
+    v.y = *reinterpret_cast<const uint32_t*>(&r.h[1]);
+    v.z = *reinterpret_cast<const uint32_t*>(&r.h[2]);
+    v.w = *reinterpret_cast<const uint32_t*>(&r.h[3]);
+    *reinterpret_cast<uint4*>(dst + 8 * l) = v;
 }
 
 // Per-head RMSNorm, the sum of squares in the order of the reference's tree (rms_norm.cu:23-49 with 128 threads): over the five bits of
-// an element's place in its run of 32, the highest first, then over the runs as (0 + 2) + (1 + 3). Place 4 (l & 7) + e of run
-// l >> 3 is lane l's element e, so the first three levels are lanes, two are the lane's own, and the runs are lanes again.
+// an element's place in its run of 32, the highest first, then over the runs as (0 + 2) + (1 + 3). Place 8 (l & 3) + e of run
+// l >> 2 is lane l's element e, so the first two levels are lanes, three are the lane's own, and the runs are lanes again.
 __device__ __forceinline__ void norm_row(Row& r, const Row& w, float eps) {
-    float s[4];
+    float s[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float v = __half2float(r.h[e]);
-        s[e] = v * v;
+    for (int x = 0; x < 4; ++x) {
+        const float2 f = __half22float2(r.h[x]);
+        s[2 * x] = f.x * f.x;
+        s[2 * x + 1] = f.y * f.y;
     }
 #pragma unroll
-    for (int d = 4; d > 0; d >>= 1)
+    for (int d = 2; d > 0; d >>= 1)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += __shfl_xor_sync(0xffffffffu, s[e], d);
-    float t = (s[0] + s[2]) + (s[1] + s[3]);
-    t += __shfl_xor_sync(0xffffffffu, t, 16);
+        for (int e = 0; e < 8; ++e) s[e] += __shfl_xor_sync(0xffffffffu, s[e], d);
+    float t = ((s[0] + s[4]) + (s[2] + s[6])) + ((s[1] + s[5]) + (s[3] + s[7]));
     t += __shfl_xor_sync(0xffffffffu, t, 8);
+    t += __shfl_xor_sync(0xffffffffu, t, 4);
     const float rms = rsqrtf(t / q4::kDim + eps);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float v = __half2float(r.h[e]) * rms;
-        r.h[e] = __float2half(v * __half2float(w.h[e]));
+    for (int x = 0; x < 4; ++x) {
+        const float2 f = __half22float2(r.h[x]), g = __half22float2(w.h[x]);
+        r.h[x] = __halves2half2(__float2half(__fmul_rn(f.x * rms, g.x)), __float2half(__fmul_rn(f.y * rms, g.y)));
     }
+}
+
+// V's word of a lane holds eight r of one n; a 16-bit piece of the page holds the four n of one r. The four lanes that differ in n alone
+// exchange their words (lanes are bits 1 and 2 of l): with `to_pieces` lane n gets the bytes of r = 2 n, 2 n + 1 (byte n' : n'), and back.
+__device__ __forceinline__ uint32_t exchange_bytes(uint32_t w, int n) {
+    const uint32_t x1 = __shfl_xor_sync(0xffffffffu, w, 2), x2 = __shfl_xor_sync(0xffffffffu, w, 4), x3 = __shfl_xor_sync(0xffffffffu, w, 6);
+    const uint32_t pick = n | (n + 4) << 4;  // byte n of either
+    const uint32_t own = __byte_perm(__byte_perm(w, x1, pick), __byte_perm(x2, x3, pick), 0x5410);  // of lanes n, n ^ 1, n ^ 2, n ^ 3
+    return __byte_perm(own, 0, n | (n ^ 1) << 4 | (n ^ 2) << 8 | (n ^ 3) << 12);
 }
 
 template <int GROUPS>
 __global__ void __launch_bounds__(kStoreWarps * 32) kv4_write_kernel(const StoreParams p) {
-    constexpr int kSpan = 32 / GROUPS;  // lanes of a group
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int heads = p.n_q + 2 * p.n_kv;
-    const int per_token = (heads + p.heads_per_warp - 1) / p.heads_per_warp;
+    constexpr int kSpan = 16 / GROUPS;  // lanes of a group
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & 15, side = lane >> 4;
+    const int heads = p.n_q + 2 * p.n_kv, pairs = (heads + 1) / 2;
+    const int per_token = (pairs + p.pairs_per_warp - 1) / p.pairs_per_warp;
     const long long item = static_cast<long long>(blockIdx.x) * kStoreWarps + warp;
-    const int token = static_cast<int>(item / per_token), h0 = static_cast<int>(item % per_token) * p.heads_per_warp;
+    const int token = static_cast<int>(item / per_token), first = static_cast<int>(item % per_token) * p.pairs_per_warp;
+    const int last = min(pairs, first + p.pairs_per_warp);
+    const bool normed = p.q_norm_w != nullptr, turned = p.freqs != nullptr;
     Row qw = {}, kw = {};
-    const bool normed = p.q_norm_w != nullptr;
     if (normed) {  // parameters: asked for before the wait
-        qw = load_row(p.q_norm_w, lane);
-        kw = load_row(p.k_norm_w, lane);
+        qw = load_row(p.q_norm_w, l);
+        kw = load_row(p.k_norm_w, l);
     }
     float f[2] = {0.0f, 0.0f};
-    if (p.freqs) { f[0] = p.freqs[2 * lane]; f[1] = p.freqs[2 * lane + 1]; }
+    if (turned) { f[0] = p.freqs[4 * l + 2 * side]; f[1] = p.freqs[4 * l + 2 * side + 1]; }
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
     if (token >= p.tokens) return;
     const long long slot = p.slots[token];
     if (slot < 0 || slot >= p.n_slots) return;
-    float c[2] = {1.0f, 1.0f}, s[2] = {0.0f, 0.0f};
-    if (p.freqs) {
+    const __half* const row = p.qkv + static_cast<size_t>(token) * heads * q4::kDim;
+    auto fetch = [&](int pair) { return load_row(row + min(2 * pair + side, heads - 1) * q4::kDim, l); };  // (a last head alone: twice)
+    Row next = fetch(first);
+    // cosines and sines of the lane's four pairs; either half makes two
+    float c[4], s[4];
+    if (turned) {
         const float pos = static_cast<float>(p.positions[token]);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
-            const float angle = f[i] * pos;
-            c[i] = cosf(angle);
-            s[i] = sinf(angle);
+            const float angle = (i ? f[1] : f[0]) * pos;
+            const float ca = cosf(angle), sa = sinf(angle);
+            const float co = __shfl_xor_sync(0xffffffffu, ca, 16), so = __shfl_xor_sync(0xffffffffu, sa, 16);
+            if (i) {
+                c[1] = side ? co : ca; s[1] = side ? so : sa;
+                c[3] = side ? ca : co; s[3] = side ? sa : so;
+            } else {
+                c[0] = side ? co : ca; s[0] = side ? so : sa;
+                c[2] = side ? ca : co; s[2] = side ? sa : so;
+            }
         }
     }
     const int in_page = static_cast<int>(slot) & (q4::kTokens - 1);
     unsigned char* const block = p.cache + ((slot >> 4) * p.n_layers + p.layer) * p.n_kv * static_cast<long long>(q4::page_bytes(GROUPS));
-    for (int head = h0; head < min(heads, h0 + p.heads_per_warp); ++head) {
-        const bool is_q = head < p.n_q, is_v = head >= p.n_q + p.n_kv;
-        if (is_q && !p.q_out) continue;
-        Row r = load_row(p.qkv + (static_cast<size_t>(token) * heads + head) * q4::kDim, lane);
-        if (!is_v) {
-            if (normed) norm_row(r, is_q ? qw : kw, p.eps);
-            if (p.freqs) {
+#pragma unroll 1
+    for (int pair = first; pair < last; ++pair) {
+        const int head = 2 * pair + side;
+        const bool is_q = head < p.n_q, is_v = head >= p.n_q + p.n_kv, real = head < heads;
+        Row r = next;
+        if (pair + 1 < last) next = fetch(pair + 1);
+        if (!__all_sync(0xffffffffu, is_v)) {
+            Row t = r;
+            if (normed) norm_row(t, is_q ? qw : kw, p.eps);
+            if (turned) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {  // interleaved pairs (rope.cu:36-45), rounded as qknorm_rope_kvwrite_kernel's are
-                    const float a = __half2float(r.h[2 * i]), b = __half2float(r.h[2 * i + 1]);
-                    r.h[2 * i] = __float2half(fmaf(a, c[i], -__fmul_rn(b, s[i])));
-                    r.h[2 * i + 1] = __float2half(fmaf(b, c[i], __fmul_rn(a, s[i])));
+                for (int x = 0; x < 4; ++x) {  // interleaved pairs (rope.cu:36-45), rounded as qknorm_rope_kvwrite_kernel's are
+                    const float2 v = __half22float2(t.h[x]);
+                    t.h[x] = __halves2half2(__float2half(fmaf(v.x, c[x], -__fmul_rn(v.y, s[x]))), __float2half(fmaf(v.y, c[x], __fmul_rn(v.x, s[x]))));
                 }
             }
+            if (!is_v) r = t;
         }
-        if (is_q) {
-            const __half2 a = __halves2half2(r.h[0], r.h[1]), b = __halves2half2(r.h[2], r.h[3]);
-            uint2 v = {*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b)};
-            *reinterpret_cast<uint2*>(p.q_out + (static_cast<size_t>(token) * p.n_q + head) * q4::kDim + 4 * lane) = v;
-            continue;
-        }
-        __half2 mx = __hmax2_nan(q4::extremes(r.h[0], r.h[1]), q4::extremes(r.h[2], r.h[3]));
+        if (is_q && p.q_out) store_row(p.q_out + (static_cast<size_t>(token) * p.n_q + head) * q4::kDim, l, r);
+        if (__all_sync(0xffffffffu, is_q)) continue;
+        // ---- k and v: in groups of 4 bits ----
+        __half2 hi = __hmax2_nan(__hmax2_nan(r.h[0], r.h[1]), __hmax2_nan(r.h[2], r.h[3]));
+        __half2 lo = __hmin2_nan(__hmin2_nan(r.h[0], r.h[1]), __hmin2_nan(r.h[2], r.h[3]));
+        __half2 mx = __halves2half2(__hmax_nan(__low2half(hi), __high2half(hi)), __hneg(__hmin_nan(__low2half(lo), __high2half(lo))));
 #pragma unroll
         for (int d = kSpan / 2; d > 0; d >>= 1) mx = __hmax2_nan(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const q4::Scale sc(mx);
+        uint32_t w = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            w |= static_cast<uint32_t>(sc.code(__low2half(r.h[x])) + 8) << (8 * x) | static_cast<uint32_t>(sc.code(__high2half(r.h[x])) + 8) << (8 * x + 4);
+        const int n = (l >> 1) & 3;
+        const uint32_t x = exchange_bytes(w, n);
+        if (is_q || !real) continue;
         unsigned char* const page = block + static_cast<long long>(head - p.n_q - (is_v ? p.n_kv : 0)) * q4::page_bytes(GROUPS);
-        uint32_t code[4];
+        if ((l & (kSpan - 1)) == 0) *reinterpret_cast<__half*>(page + q4::scale_off(GROUPS, is_v, in_page, l / kSpan)) = sc.s;
+        if (!is_v) {  // the lane's word: run l >> 2, quarter l & 3
+            *reinterpret_cast<uint32_t*>(page + in_page * 64 + (l & 3) * 16 + (l >> 2) * 4) = w;
+        } else {  // channel 8 l + e is channel 64 high + 16 n + 8 half + r with high = l >> 3, n = (l >> 1) & 3, half = l & 1, r = e
 #pragma unroll
-        for (int e = 0; e < 4; ++e) code[e] = static_cast<uint32_t>(sc.code(r.h[e]) + 8);
-        if ((lane & (kSpan - 1)) == 0)
-            *reinterpret_cast<__half*>(page + q4::scale_off(GROUPS, is_v, in_page, lane / kSpan)) = sc.s;
-        if (!is_v) {
-            // channels 4 l .. 4 l + 3: run l >> 3, quarter (l & 7) >> 1, nibbles 4 (l & 1) ..; the even lane stores both halves
-            uint32_t w = code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12;
-            w |= __shfl_down_sync(0xffffffffu, w, 1) << 16;
-            if (!(lane & 1)) *reinterpret_cast<uint32_t*>(page + in_page * 64 + ((lane & 7) >> 1) * 16 + (lane >> 3) * 4) = w;
-        } else {
-            // channel 4 l + e is channel 64 high + 16 n + 8 half + r with high = l >> 4, n = (l >> 2) & 3, half = (l >> 1) & 1,
-            // r = 4 (l & 1) + e: the four lanes that differ in n alone make four 16-bit pieces, one per e; each stores one
-            const int n = (lane >> 2) & 3;
-            uint32_t lo = (code[0] | code[1] << 16) << (4 * n), hi = (code[2] | code[3] << 16) << (4 * n);
-#pragma unroll
-            for (int d = 4; d <= 8; d <<= 1) {
-                lo |= __shfl_xor_sync(0xffffffffu, lo, d);
-                hi |= __shfl_xor_sync(0xffffffffu, hi, d);
+            for (int e = 0; e < 2; ++e) {
+                uint32_t t = (x >> (4 * e)) & 0x0f0f0f0fu;  // a nibble of each of four bytes, to sixteen bits
+                t = (t | t >> 4) & 0x00ff00ffu;
+                *reinterpret_cast<uint16_t*>(page + q4::kVOff + (in_page >> 1) * 128 + (2 * n + e) * 16 + (l & 1) * 8 + (l >> 3) * 4 + (in_page & 1) * 2) =
+                    static_cast<uint16_t>(t | t >> 8);
             }
-            const uint32_t both = n & 2 ? hi : lo;
-            const uint16_t piece = static_cast<uint16_t>(n & 1 ? both >> 16 : both);
-            const int r8 = 4 * (lane & 1) + n, half = (lane >> 1) & 1, high = lane >> 4;
-            *reinterpret_cast<uint16_t*>(page + q4::kVOff + (in_page >> 1) * 128 + r8 * 16 + half * 8 + high * 4 + (in_page & 1) * 2) = piece;
         }
     }
 }
 
-// The values of listed slots, fp16: what a prompt that continues a cached prefix computes with. A warp per (token, kv head).
+// The values of listed slots, fp16: what a prompt that continues a cached prefix computes with. Half a warp per (token, kv head).
 template <int GROUPS>
 __global__ void __launch_bounds__(kStoreWarps * 32) kv4_read_kernel(const unsigned char* cache, const long long* slots, long long n_slots,
                                                                      int tokens, int n_kv, int layer, int n_layers, __half* k_out,
                                                                      __half* v_out) {
-    constexpr int kSpan = 32 / GROUPS;
-    const int lane = threadIdx.x & 31;
-    const long long item = static_cast<long long>(blockIdx.x) * kStoreWarps + (threadIdx.x >> 5);
+    constexpr int kSpan = 16 / GROUPS;
+    const int lane = threadIdx.x & 31, l = lane & 15, n = (l >> 1) & 3;
+    const long long item = (static_cast<long long>(blockIdx.x) * kStoreWarps + (threadIdx.x >> 5)) * 2 + (lane >> 4);
     const int token = static_cast<int>(item / n_kv), head = static_cast<int>(item % n_kv);
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
-    if (token >= tokens) return;
-    const long long slot = slots[token];
-    if (slot < 0 || slot >= n_slots) return;
+    const long long slot = token < tokens ? slots[token] : -1;
+    const bool real = slot >= 0 && slot < n_slots;
     const int in_page = static_cast<int>(slot) & (q4::kTokens - 1);
-    const unsigned char* page = cache + (((slot >> 4) * n_layers + layer) * n_kv + head) * static_cast<long long>(q4::page_bytes(GROUPS));
-    const float ks = __half2float(*reinterpret_cast<const __half*>(page + q4::scale_off(GROUPS, 0, in_page, lane / kSpan)));
-    const float vs = __half2float(*reinterpret_cast<const __half*>(page + q4::scale_off(GROUPS, 1, in_page, lane / kSpan)));
-    const uint32_t kc = *reinterpret_cast<const uint16_t*>(page + in_page * 64 + ((lane & 7) >> 1) * 16 + (lane >> 3) * 4 + (lane & 1) * 2);
-    __half k[4], v[4];
+    const unsigned char* page = cache + ((((real ? slot : 0) >> 4) * n_layers + layer) * n_kv + head) * static_cast<long long>(q4::page_bytes(GROUPS));
+    uint32_t kw = 0, vw = 0;
+    float ks = 0.0f, vs = 0.0f;
+    if (real) {
+        kw = *reinterpret_cast<const uint32_t*>(page + in_page * 64 + (l & 3) * 16 + (l >> 2) * 4);
+        ks = __half2float(*reinterpret_cast<const __half*>(page + q4::scale_off(GROUPS, 0, in_page, l / kSpan)));
+        vs = __half2float(*reinterpret_cast<const __half*>(page + q4::scale_off(GROUPS, 1, in_page, l / kSpan)));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t piece = *reinterpret_cast<const uint16_t*>(page + q4::kVOff + (in_page >> 1) * 128 + (4 * (lane & 1) + e) * 16 +
-                                                                  ((lane >> 1) & 1) * 8 + (lane >> 4) * 4 + (in_page & 1) * 2);
-        k[e] = __float2half(static_cast<float>(static_cast<int>((kc >> (4 * e)) & 15) - 8) * ks);
-        v[e] = __float2half(static_cast<float>(static_cast<int>((piece >> (4 * ((lane >> 2) & 3))) & 15) - 8) * vs);
+        for (int e = 0; e < 2; ++e) {  // r = 2 n + e: sixteen bits to a nibble of each of four bytes
+            uint32_t t = *reinterpret_cast<const uint16_t*>(page + q4::kVOff + (in_page >> 1) * 128 + (2 * n + e) * 16 + (l & 1) * 8 + (l >> 3) * 4 +
+                                                            (in_page & 1) * 2);
+            t = (t | t << 8) & 0x00ff00ffu;
+            vw |= ((t | t << 4) & 0x0f0f0f0fu) << (4 * e);
+        }
     }
-    const size_t at = (static_cast<size_t>(token) * n_kv + head) * q4::kDim + 4 * lane;
-    if (k_out) {
-        const __half2 a = __halves2half2(k[0], k[1]), b = __halves2half2(k[2], k[3]);
-        *reinterpret_cast<uint2*>(k_out + at) = {*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b)};
-    }
-    if (v_out) {
-        const __half2 a = __halves2half2(v[0], v[1]), b = __halves2half2(v[2], v[3]);
-        *reinterpret_cast<uint2*>(v_out + at) = {*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b)};
-    }
+    vw = exchange_bytes(vw, n);
+    if (!real) return;
+    const size_t at = (static_cast<size_t>(token) * n_kv + head) * q4::kDim;
+    auto open = [&](uint32_t w, float s) {
+        Row r;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            r.h[x] = __floats2half2_rn(static_cast<float>(static_cast<int>((w >> (8 * x)) & 15) - 8) * s,
+                                       static_cast<float>(static_cast<int>((w >> (8 * x + 4)) & 15) - 8) * s);
+        return r;
+    };
+    if (k_out) store_row(k_out + at, l, open(kw, ks));
+    if (v_out) store_row(v_out + at, l, open(vw, vs));
 }
 
 template <class... P, class... A>
@@ -216,11 +254,11 @@ int launch_kv4_write(const __half* qkv, const __half* q_norm_w, const __half* k_
     if (tokens == 0) return W8A8_OK;
     StoreParams p = {qkv, q_norm_w, k_norm_w, eps, freqs, positions, slots, static_cast<long long>(n_blocks) * q4::kTokens,
                      static_cast<unsigned char*>(cache), tokens, n_q, n_kv, layer, n_layers, q_out, 1};
-    const int heads = n_q + 2 * n_kv;
-    // A warp a head while that does not fill the GPU.
-    const long long all = static_cast<long long>(tokens) * heads, room = 32ll * device_sms();
-    p.heads_per_warp = all > 4 * room ? 4 : all > 2 * room ? 2 : 1;
-    const long long warps = static_cast<long long>(tokens) * ((heads + p.heads_per_warp - 1) / p.heads_per_warp);
+    // A warp takes one pair of heads while that does not fill the GPU, else several, up to a token's.
+    const int pairs = (n_q + 2 * n_kv + 1) / 2;
+    const long long each = static_cast<long long>(tokens) * pairs / (48ll * device_sms());
+    p.pairs_per_warp = each < 1 ? 1 : each < pairs ? static_cast<int>(each) : pairs;
+    const long long warps = static_cast<long long>(tokens) * ((pairs + p.pairs_per_warp - 1) / p.pairs_per_warp);
     const cudaError_t e = group == 32   ? launch_rows(warps, stream, kv4_write_kernel<4>, p)
                           : group == 64 ? launch_rows(warps, stream, kv4_write_kernel<2>, p)
                                         : launch_rows(warps, stream, kv4_write_kernel<1>, p);
@@ -231,7 +269,7 @@ int launch_kv4_write(const __half* qkv, const __half* q_norm_w, const __half* k_
 int launch_kv4_read(const void* cache, int n_blocks, const long long* slots, int layer, int n_layers, int tokens, int n_kv, int group,
                     __half* k_out, __half* v_out, cudaStream_t stream) {
     if (tokens == 0) return W8A8_OK;
-    const long long warps = static_cast<long long>(tokens) * n_kv, n_slots = static_cast<long long>(n_blocks) * q4::kTokens;
+    const long long warps = (static_cast<long long>(tokens) * n_kv + 1) / 2, n_slots = static_cast<long long>(n_blocks) * q4::kTokens;
     const unsigned char* c = static_cast<const unsigned char*>(cache);
     const cudaError_t e =
         group == 32   ? launch_rows(warps, stream, kv4_read_kernel<4>, c, slots, n_slots, tokens, n_kv, layer, n_layers, k_out, v_out)
