@@ -54,31 +54,90 @@ __device__ __forceinline__ void store_row(__half* dst, int l, const Row& r) {
     *reinterpret_cast<uint4*>(dst + 8 * l) = v;
 }
 
+// Two fp32 numbers in one register pair: the packed arithmetic rounds each as the plain one does.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts(F2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator-(F2 a) { return {a.v ^ 0x8000000080000000ull}; }
+// The lane's channels as x (even) and y (odd) of the rotation's pairs 0, 1 and 2, 3.
+struct Wide {
+    F2 x[2], y[2];
+    Wide() = default;
+    __device__ __forceinline__ explicit Wide(const Row& r) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 a = __half22float2(r.h[2 * i]), b = __half22float2(r.h[2 * i + 1]);
+            x[i] = f2(a.x, b.x);
+            y[i] = f2(a.y, b.y);
+        }
+    }
+    __device__ __forceinline__ Row halves() const {
+        Row r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 a = parts(x[i]), b = parts(y[i]);
+            r.h[2 * i] = __floats2half2_rn(a.x, b.x);
+            r.h[2 * i + 1] = __floats2half2_rn(a.y, b.y);
+        }
+        return r;
+    }
+};
+
 // Per-head RMSNorm, the sum of squares in the order of the reference's tree (rms_norm.cu:23-49 with 128 threads): over the five bits of
 // an element's place in its run of 32, the highest first, then over the runs as (0 + 2) + (1 + 3). Place 8 (l & 3) + e of run
 // l >> 2 is lane l's element e, so the first two levels are lanes, three are the lane's own, and the runs are lanes again.
-__device__ __forceinline__ void norm_row(Row& r, const Row& w, float eps) {
-    float s[8];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const float2 f = __half22float2(r.h[x]);
-        s[2 * x] = f.x * f.x;
-        s[2 * x + 1] = f.y * f.y;
-    }
+__device__ __forceinline__ Row normed_row(const Row& r, const Wide& w, float eps) {
+    const Wide v(r);
+    F2 s[4] = {v.x[0] * v.x[0], v.x[1] * v.x[1], v.y[0] * v.y[0], v.y[1] * v.y[1]};
 #pragma unroll
     for (int d = 2; d > 0; d >>= 1)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += __shfl_xor_sync(0xffffffffu, s[e], d);
-    float t = ((s[0] + s[4]) + (s[2] + s[6])) + ((s[1] + s[5]) + (s[3] + s[7]));
+        for (int e = 0; e < 4; ++e) {
+            const float2 a = parts(s[e]);
+            s[e] = s[e] + f2(__shfl_xor_sync(0xffffffffu, a.x, d), __shfl_xor_sync(0xffffffffu, a.y, d));
+        }
+    const float2 even = parts(s[0] + s[1]), odd = parts(s[2] + s[3]);  // places e and e + 4
+    float t = (even.x + even.y) + (odd.x + odd.y);
     t += __shfl_xor_sync(0xffffffffu, t, 8);
     t += __shfl_xor_sync(0xffffffffu, t, 4);
     const float rms = rsqrtf(t / q4::kDim + eps);
+    const F2 rr = f2(rms, rms);
+    Wide o;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const float2 f = __half22float2(r.h[x]), g = __half22float2(w.h[x]);
-        r.h[x] = __halves2half2(__float2half(__fmul_rn(f.x * rms, g.x)), __float2half(__fmul_rn(f.y * rms, g.y)));
+    for (int i = 0; i < 2; ++i) {
+        o.x[i] = v.x[i] * rr * w.x[i];
+        o.y[i] = v.y[i] * rr * w.y[i];
     }
+    return o.halves();
 }
+
+// Cosine and sine of one angle. (One copy of the code: it runs cold, and once per token.)
+__device__ __noinline__ float2 cos_sin(float angle) { return make_float2(cosf(angle), sinf(angle)); }
 
 // V's word of a lane holds eight r of one n; a 16-bit piece of the page holds the four n of one r. The four lanes that differ in n alone
 // exchange their words (lanes are bits 1 and 2 of l): with `to_pieces` lane n gets the bytes of r = 2 n, 2 n + 1 (byte n' : n'), and back.
@@ -89,21 +148,22 @@ __device__ __forceinline__ uint32_t exchange_bytes(uint32_t w, int n) {
     return __byte_perm(own, 0, n | (n ^ 1) << 4 | (n ^ 2) << 8 | (n ^ 3) << 12);
 }
 
+// Pairs of heads of one kind: the query heads two by two, then k's, then v's (of an odd count the last pair's second half has nothing to do).
+__host__ __device__ inline int store_pairs(int n_q, int n_kv) { return (n_q + 1) / 2 + 2 * ((n_kv + 1) / 2); }
+
 template <int GROUPS>
-__global__ void __launch_bounds__(kStoreWarps * 32) kv4_write_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(kStoreWarps * 32, 8) kv4_write_kernel(const __grid_constant__ StoreParams p) {
     constexpr int kSpan = 16 / GROUPS;  // lanes of a group
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & 15, side = lane >> 4;
-    const int heads = p.n_q + 2 * p.n_kv, pairs = (heads + 1) / 2;
+    const int lane = threadIdx.x & 31, l = lane & 15, side = lane >> 4;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int q_pairs = (p.n_q + 1) / 2, kv_pairs = (p.n_kv + 1) / 2, pairs = q_pairs + 2 * kv_pairs;
     const int per_token = (pairs + p.pairs_per_warp - 1) / p.pairs_per_warp;
     const long long item = static_cast<long long>(blockIdx.x) * kStoreWarps + warp;
     const int token = static_cast<int>(item / per_token), first = static_cast<int>(item % per_token) * p.pairs_per_warp;
     const int last = min(pairs, first + p.pairs_per_warp);
     const bool normed = p.q_norm_w != nullptr, turned = p.freqs != nullptr;
-    Row qw = {}, kw = {};
-    if (normed) {  // parameters: asked for before the wait
-        qw = load_row(p.q_norm_w, l);
-        kw = load_row(p.k_norm_w, l);
-    }
+    Wide w;
+    if (normed && first < q_pairs + kv_pairs) w = Wide(load_row(first < q_pairs ? p.q_norm_w : p.k_norm_w, l));  // parameters: asked for before the wait
     float f[2] = {0.0f, 0.0f};
     if (turned) { f[0] = p.freqs[4 * l + 2 * side]; f[1] = p.freqs[4 * l + 2 * side + 1]; }
     ptx::pdl_wait();
@@ -111,71 +171,88 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kv4_write_kernel(const Store
     if (token >= p.tokens) return;
     const long long slot = p.slots[token];
     if (slot < 0 || slot >= p.n_slots) return;
-    const __half* const row = p.qkv + static_cast<size_t>(token) * heads * q4::kDim;
-    auto fetch = [&](int pair) { return load_row(row + min(2 * pair + side, heads - 1) * q4::kDim, l); };  // (a last head alone: twice)
-    Row next = fetch(first);
+    const __half* const row = p.qkv + static_cast<size_t>(token) * (p.n_q + 2 * p.n_kv) * q4::kDim;
+    auto fetch = [&](int pair) {  // (a half without a head: its neighbour's)
+        const int kind = pair < q_pairs ? 0 : pair < q_pairs + kv_pairs ? 1 : 2;
+        const int h = 2 * (pair - (kind > 0 ? q_pairs : 0) - (kind > 1 ? kv_pairs : 0)) + side;
+        return load_row(row + ((kind > 0 ? p.n_q : 0) + (kind > 1 ? p.n_kv : 0) + min(h, (kind > 0 ? p.n_kv : p.n_q) - 1)) * q4::kDim, l);
+    };
+    Row next = fetch(first);  // (more than one ahead gave nothing: 8192 tokens 48.3 us with one, 49.7 with two, 50.3 with three)
+    auto take = [&](int pair) {
+        const Row r = next;
+        if (pair + 1 < last) next = fetch(pair + 1);
+        return r;
+    };
     // cosines and sines of the lane's four pairs; either half makes two
-    float c[4], s[4];
-    if (turned) {
+    F2 c[2], s[2];
+    if (turned && first < q_pairs + kv_pairs) {
         const float pos = static_cast<float>(p.positions[token]);
+        const float2 a = cos_sin(f[0] * pos), b = cos_sin(f[1] * pos);
+        const float2 ao = {__shfl_xor_sync(0xffffffffu, a.x, 16), __shfl_xor_sync(0xffffffffu, a.y, 16)};
+        const float2 bo = {__shfl_xor_sync(0xffffffffu, b.x, 16), __shfl_xor_sync(0xffffffffu, b.y, 16)};
+        const F2 mine_c = f2(a.x, b.x), mine_s = f2(a.y, b.y), other_c = f2(ao.x, bo.x), other_s = f2(ao.y, bo.y);
+        c[0] = side ? other_c : mine_c;
+        c[1] = side ? mine_c : other_c;
+        s[0] = side ? other_s : mine_s;
+        s[1] = side ? mine_s : other_s;
+    }
+    auto turn = [&](const Row& r) {  // norm and rotation of a q or k row
+        const Row t = normed ? normed_row(r, w, p.eps) : r;
+        if (!turned) return t;
+        const Wide v(t);
+        Wide o;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // interleaved pairs (rope.cu:36-45), rounded as qknorm_rope_kvwrite_kernel's are
+            o.x[i] = fma2(v.x[i], c[i], -(v.y[i] * s[i]));
+            o.y[i] = fma2(v.y[i], c[i], v.x[i] * s[i]);
+        }
+        return o.halves();
+    };
+
+    // ---- query heads ----
+    int pair = first;
+    {
+        __half* out = p.q_out + (static_cast<size_t>(token) * p.n_q + 2 * first + side) * q4::kDim;
 #pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-            const float angle = (i ? f[1] : f[0]) * pos;
-            const float ca = cosf(angle), sa = sinf(angle);
-            const float co = __shfl_xor_sync(0xffffffffu, ca, 16), so = __shfl_xor_sync(0xffffffffu, sa, 16);
-            if (i) {
-                c[1] = side ? co : ca; s[1] = side ? so : sa;
-                c[3] = side ? ca : co; s[3] = side ? sa : so;
-            } else {
-                c[0] = side ? co : ca; s[0] = side ? so : sa;
-                c[2] = side ? ca : co; s[2] = side ? sa : so;
-            }
+        for (; pair < min(last, q_pairs); ++pair, out += 2 * q4::kDim) {
+            const Row r = take(pair);
+            if (!p.q_out) continue;
+            const Row t = turn(r);
+            if (2 * pair + side < p.n_q) store_row(out, l, t);
         }
     }
+    if (pair < q_pairs + kv_pairs && pair < last && first < q_pairs && normed) w = Wide(load_row(p.k_norm_w, l));
+
+    // ---- k, then v: in groups of 4 bits ----
     const int in_page = static_cast<int>(slot) & (q4::kTokens - 1);
     unsigned char* const block = p.cache + ((slot >> 4) * p.n_layers + p.layer) * p.n_kv * static_cast<long long>(q4::page_bytes(GROUPS));
 #pragma unroll 1
-    for (int pair = first; pair < last; ++pair) {
-        const int head = 2 * pair + side;
-        const bool is_q = head < p.n_q, is_v = head >= p.n_q + p.n_kv, real = head < heads;
-        Row r = next;
-        if (pair + 1 < last) next = fetch(pair + 1);
-        if (!__all_sync(0xffffffffu, is_v)) {
-            Row t = r;
-            if (normed) norm_row(t, is_q ? qw : kw, p.eps);
-            if (turned) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {  // interleaved pairs (rope.cu:36-45), rounded as qknorm_rope_kvwrite_kernel's are
-                    const float2 v = __half22float2(t.h[x]);
-                    t.h[x] = __halves2half2(__float2half(fmaf(v.x, c[x], -__fmul_rn(v.y, s[x]))), __float2half(fmaf(v.y, c[x], __fmul_rn(v.x, s[x]))));
-                }
-            }
-            if (!is_v) r = t;
-        }
-        if (is_q && p.q_out) store_row(p.q_out + (static_cast<size_t>(token) * p.n_q + head) * q4::kDim, l, r);
-        if (__all_sync(0xffffffffu, is_q)) continue;
-        // ---- k and v: in groups of 4 bits ----
+    for (; pair < last; ++pair) {
+        const bool is_v = pair >= q_pairs + kv_pairs;
+        const int head = 2 * (pair - q_pairs - (is_v ? kv_pairs : 0)) + side;
+        Row r = take(pair);
+        if (!is_v) r = turn(r);
         __half2 hi = __hmax2_nan(__hmax2_nan(r.h[0], r.h[1]), __hmax2_nan(r.h[2], r.h[3]));
         __half2 lo = __hmin2_nan(__hmin2_nan(r.h[0], r.h[1]), __hmin2_nan(r.h[2], r.h[3]));
         __half2 mx = __halves2half2(__hmax_nan(__low2half(hi), __high2half(hi)), __hneg(__hmin_nan(__low2half(lo), __high2half(lo))));
 #pragma unroll
         for (int d = kSpan / 2; d > 0; d >>= 1) mx = __hmax2_nan(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const q4::Scale sc(mx);
-        uint32_t w = 0;
+        uint32_t word = 0;
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            w |= static_cast<uint32_t>(sc.code(__low2half(r.h[x])) + 8) << (8 * x) | static_cast<uint32_t>(sc.code(__high2half(r.h[x])) + 8) << (8 * x + 4);
+            word |= static_cast<uint32_t>(sc.code(__low2half(r.h[x])) + 8) << (8 * x) | static_cast<uint32_t>(sc.code(__high2half(r.h[x])) + 8) << (8 * x + 4);
         const int n = (l >> 1) & 3;
-        const uint32_t x = exchange_bytes(w, n);
-        if (is_q || !real) continue;
-        unsigned char* const page = block + static_cast<long long>(head - p.n_q - (is_v ? p.n_kv : 0)) * q4::page_bytes(GROUPS);
+        const uint32_t pieces = is_v ? exchange_bytes(word, n) : 0u;
+        if (head >= p.n_kv) continue;
+        unsigned char* const page = block + static_cast<long long>(head) * q4::page_bytes(GROUPS);
         if ((l & (kSpan - 1)) == 0) *reinterpret_cast<__half*>(page + q4::scale_off(GROUPS, is_v, in_page, l / kSpan)) = sc.s;
         if (!is_v) {  // the lane's word: run l >> 2, quarter l & 3
-            *reinterpret_cast<uint32_t*>(page + in_page * 64 + (l & 3) * 16 + (l >> 2) * 4) = w;
+            *reinterpret_cast<uint32_t*>(page + in_page * 64 + (l & 3) * 16 + (l >> 2) * 4) = word;
         } else {  // channel 8 l + e is channel 64 high + 16 n + 8 half + r with high = l >> 3, n = (l >> 1) & 3, half = l & 1, r = e
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                uint32_t t = (x >> (4 * e)) & 0x0f0f0f0fu;  // a nibble of each of four bytes, to sixteen bits
+                uint32_t t = (pieces >> (4 * e)) & 0x0f0f0f0fu;  // a nibble of each of four bytes, to sixteen bits
                 t = (t | t >> 4) & 0x00ff00ffu;
                 *reinterpret_cast<uint16_t*>(page + q4::kVOff + (in_page >> 1) * 128 + (2 * n + e) * 16 + (l & 1) * 8 + (l >> 3) * 4 + (in_page & 1) * 2) =
                     static_cast<uint16_t>(t | t >> 8);
@@ -254,8 +331,9 @@ int launch_kv4_write(const __half* qkv, const __half* q_norm_w, const __half* k_
     if (tokens == 0) return W8A8_OK;
     StoreParams p = {qkv, q_norm_w, k_norm_w, eps, freqs, positions, slots, static_cast<long long>(n_blocks) * q4::kTokens,
                      static_cast<unsigned char*>(cache), tokens, n_q, n_kv, layer, n_layers, q_out, 1};
-    // A warp takes one pair of heads while that does not fill the GPU, else several, up to a token's.
-    const int pairs = (n_q + 2 * n_kv + 1) / 2;
+    // A warp takes one pair of heads while that does not fill the GPU (32 warps an SM run at once), else several, up to a token's: 48 warps an SM or
+    // more. (With 96 and 150: 613 tokens 8.6 us instead of 5.9, 2048 tokens 18.8 and 21.4 instead of 15.3, 8192 tokens 49.7 and 55.4 instead of 48.3.)
+    const int pairs = store_pairs(n_q, n_kv);
     const long long each = static_cast<long long>(tokens) * pairs / (48ll * device_sms());
     p.pairs_per_warp = each < 1 ? 1 : each < pairs ? static_cast<int>(each) : pairs;
     const long long warps = static_cast<long long>(tokens) * ((pairs + p.pairs_per_warp - 1) / p.pairs_per_warp);
