@@ -35,9 +35,13 @@ using q4::kTokens;
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
 #ifndef KV4_WHOLE
-#define KV4_WHOLE 256
+#define KV4_WHOLE 96
+#endif
+#ifndef KV4_COST
+#define KV4_COST 4
 #endif
 constexpr int kWholePages = KV4_WHOLE;
+constexpr int kPairCost = KV4_COST;
 constexpr float kLag = 8.0f;  // p is at most 2^8: it keeps its precision in fp16
 
 struct Kv4Params {
@@ -51,7 +55,6 @@ struct Kv4Params {
     int g;
     int batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers;
     float scale_log2;  // sm_scale * log2(e) * 2^24: the scores' codes come as 2^-24 of themselves
-    int whole_pages;   // pairs of at most so many pages lie in one CTA
     float* scratch;    // [CTAs][2] pieces
     int* tickets;      // [CTAs], zero between launches
     int* status;
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, 1) kv4_attention_kernel
     __shared__ __align__(8) uint64_t full_bar[W][D];
     __shared__ int scan_s[W + 1];
     __shared__ long long piece_pair[2 * W];  // the pair of a piece, or -1
-    __shared__ int last_s;
+    __shared__ int last_s[2];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (lane < D) {
@@ -306,20 +309,46 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, 1) kv4_attention_kernel
         return a;  // (the last of those that start at or before u: empty ones in front of it start there too)
     };
     // ---- this warp's run ----
-    const long long cta_units = max((units + gridDim.x - 1) / gridDim.x, 1ll);
-    // Where CTA c's run begins: at c cta_units, but not inside a pair of few pages, which goes to one side or the other as a whole.
-    auto border = [&](long long c) {
-        const long long u = c * cta_units;
-        if (u >= units) return units;
-        const int b = sequence_of(u), blocks = first_s[b + 1] - first_s[b];
-        const long long from = static_cast<long long>(first_s[b]) * p.n_kv;
-        const int in = static_cast<int>(u - from) % blocks;
-        return blocks > p.whole_pages ? u : 2 * in < blocks ? u - in : u - in + blocks;
+    // The range is cut by cost: a pair counts kPairCost pages more than it has (its q, its piece, its output; a run of many short pairs would
+    // else last longest). Cost v of the range is cost v - of pairs ahead - kPairCost pages into its pair, none where that is negative.
+    const long long costs = units + static_cast<long long>(kPairCost) * p.batch * p.n_kv;
+    const long long cta_cost = max((costs + gridDim.x - 1) / gridDim.x, 1ll);
+    auto cost_ahead = [&](int b) { return (static_cast<long long>(first_s[b]) + static_cast<long long>(kPairCost) * b) * p.n_kv; };
+    struct Place {
+        int b, h, in, of;  // cost `in` of `of` of the pair (b, h)
     };
-    const long long cta_lo = border(blockIdx.x), cta_hi = border(blockIdx.x + 1);
-    const int per = static_cast<int>((cta_hi - cta_lo + W - 1) / W);
-    const long long lo = min(cta_hi, cta_lo + warp * per);
-    const int n_mine = static_cast<int>(min(cta_hi, lo + per) - lo);
+    auto place_of = [&](long long v) {
+        int a = 0, z = p.batch - 1;
+#pragma unroll 1
+        while (a < z) {
+            const int mid = (a + z + 1) >> 1;
+            if (cost_ahead(mid) <= v) a = mid; else z = mid - 1;
+        }
+        const int of = first_s[a + 1] - first_s[a] + kPairCost, rest = static_cast<int>(v - cost_ahead(a)), h = rest / of;
+        return Place{a, h, rest - h * of, of};
+    };
+    auto pages_ahead = [&](long long v) {  // units ahead of cost v
+        if (v >= costs) return units;
+        const Place x = place_of(v);
+        return static_cast<long long>(first_s[x.b]) * p.n_kv + static_cast<long long>(x.h) * (x.of - kPairCost) + max(0, x.in - kPairCost);
+    };
+    // Where CTA c's run begins: at c cta_cost, but not inside a pair of few pages, which goes to one side or the other as a whole.
+    const long long whole_pages = min(static_cast<long long>(kWholePages), 4 * cta_cost);
+    auto border = [&](long long c) {
+        const long long v = c * cta_cost;
+        if (v >= costs) return costs;
+        const Place x = place_of(v);
+        return x.of - kPairCost > whole_pages ? v : 2 * x.in < x.of ? v - x.in : v - x.in + x.of;
+    };
+    long long at_border = border(blockIdx.x + (lane & 1));  // lanes 0, 1: the CTA's run, from and to; lanes 2, 3: the warp's
+    {
+        const long long from = __shfl_sync(0xffffffffu, at_border, 0), to = __shfl_sync(0xffffffffu, at_border, 1);
+        if (lane & 2) at_border = min(to, from + (warp + (lane & 1)) * ((to - from + W - 1) / W));
+        at_border = pages_ahead(at_border);
+    }
+    const long long cta_lo = __shfl_sync(0xffffffffu, at_border, 0), cta_hi = __shfl_sync(0xffffffffu, at_border, 1);
+    const long long lo = __shfl_sync(0xffffffffu, at_border, 2);
+    const int n_mine = static_cast<int>(__shfl_sync(0xffffffffu, at_border, 3) - lo);
 
     const uint32_t ring = ptx::smem_u32(ring_all) + warp * (D * kPage);
     int page_of = 0;  // the page's number in the cache of unit (i & ~31) + lane of the run
@@ -581,39 +610,47 @@ __global__ void __launch_bounds__(Shape<R>::kWarps * 32, 1) kv4_attention_kernel
                         static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
     }
 
-    // ---- pairs that lie in several CTAs: the last of them to come here adds their pieces ----
-#pragma unroll 1
-    for (int side = 0; side < 2; ++side) {
+    // ---- pairs that lie in several CTAs: the last of them to come here adds their pieces; half of the warps see to either open pair ----
+    if (open[0] < 0 && open[1] < 0) goto done;  // (uniform over the CTA)
+    __syncthreads();
+    {
+        constexpr int kHalf = W / 2;
+        const int side = warp >= kHalf, w = warp - side * kHalf;
         const long long pair = open[side];
-        if (pair < 0) continue;  // (uniform over the CTA)
-        long long from, to;
-        pair_units(pair, from, to);
-        const int c0 = static_cast<int>(from / cta_units), c1 = static_cast<int>((to - 1) / cta_units);
-        __syncthreads();
-        if (tid == 0) {  // (releases what the CTA's warps stored ahead of the barrier, acquires what the others' released)
-            int before;
-            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + c0) : "memory");
-            last_s = before == c1 - c0;
-            if (last_s) p.tickets[c0] = 0;
-        }
-        __syncthreads();
-        if (!last_s) continue;
-        // pieces in the order of the pages: warp w a run of them, the runs then in order
-        const int n = c1 - c0 + 1, run = (n + W - 1) / W, a = min(n, warp * run), z = min(n, a + run);
-        Merged<R> s;
-        s.clear();
-#pragma unroll 2
-        for (int k = a; k < z; ++k) {
-            const float* piece = p.scratch + (2ll * (c0 + k) + (k == 0 ? 1 : 0)) * kPiece;
+        if (pair >= 0) {
+            long long from, to;
+            pair_units(pair, from, to);
+            const long long first_cost = from + cost_ahead(static_cast<int>(pair / p.n_kv)) - static_cast<long long>(first_s[pair / p.n_kv]) * p.n_kv +
+                                         static_cast<long long>(kPairCost) * (pair % p.n_kv + 1);  // of the pair's first page
+            const int c0 = static_cast<int>(first_cost / cta_cost), c1 = static_cast<int>((first_cost + (to - from) - 1) / cta_cost), n = c1 - c0 + 1;
+            auto half_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + side), "n"(kHalf * 32) : "memory"); };
+            if (w == 0 && lane == 0) {  // (releases what the CTA's warps stored ahead of the barrier, acquires what the others' released)
+                int before;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.tickets + c0) : "memory");
+                last_s[side] = before == n - 1;
+                if (before == n - 1) p.tickets[c0] = 0;
+            }
+            half_barrier();
+            if (last_s[side]) {
+                // pieces in the order of the pages: warp w a run of them, the runs then in order
+                const int run = (n + kHalf - 1) / kHalf, x0 = min(n, w * run), x1 = min(n, x0 + run);
+                float* const mine = pieces + warp * kPiece;
+                Merged<R> s;
+                s.clear();
+                for (int k = x0; k < x1; ++k) {
+                    const float* piece = p.scratch + (2ll * (c0 + k) + (k == 0 ? 1 : 0)) * kPiece;
 #pragma unroll
-            for (int h = 0; h < R; ++h)
-                s.add(h, __ldcg(reinterpret_cast<const float4*>(piece + h * kDim) + lane), __ldcg(piece + R * kDim + h), __ldcg(piece + R * kDim + R + h));
+                    for (int h = 0; h < R; ++h)
+                        s.add(h, __ldcg(reinterpret_cast<const float4*>(piece + h * kDim) + lane), __ldcg(piece + R * kDim + h), __ldcg(piece + R * kDim + R + h));
+                }
+                if (x0 < x1) s.store(mine, lane);
+                half_barrier();
+                if (w == 0)
+                    merge_pieces<R>(p, mine, (1u << ((n + run - 1) / run)) - 1, nullptr, static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
+            }
         }
-        s.store(pieces + warp * kPiece, lane);
-        __syncthreads();
-        if (warp == 0) merge_pieces<R>(p, pieces, (1u << W) - 1, nullptr, static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
-        __syncthreads();
     }
+done:
     if (failed) {  // copies that may still be on their way land before the CTA goes
 #pragma unroll 1
         for (int w = 0; w < 1000; ++w) __nanosleep(1000);
@@ -650,7 +687,7 @@ int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const
     if (batch == 0) return W8A8_OK;
     const int ratio = n_q / n_kv;
     Kv4Params p = {q, static_cast<const unsigned char*>(cache), table, lens, out, Xq, Xs, g, batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers,
-                   sm_scale * 1.4426950408889634f * 0x1p24f, kWholePages, scratch, tickets, status};
+                   sm_scale * 1.4426950408889634f * 0x1p24f, scratch, tickets, status};
     const long long most = static_cast<long long>(batch) * n_kv * max_blocks;  // units, were all sequences as long as their rows
     const int sms = device_sms() < kKv4Tickets ? device_sms() : kKv4Tickets, ctas = most < sms ? static_cast<int>(most) : sms;
     cudaError_t e;
