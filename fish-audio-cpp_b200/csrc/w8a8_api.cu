@@ -22,7 +22,7 @@ struct w8a8_ctx {
     std::unordered_map<const void*, PackedEntry> packed;
     std::mutex packed_mu;
     short gemm_bt = 0, gemm_splits = 0;  // w8a8_debug_force_gemm_form
-    int* tail_counters = nullptr;     // arrival counters of the decode kernel's tails, then of the 4-bit attention; zero between launches
+    int* tail_counters = nullptr;     // arrival counters of the decode kernel's tails, tickets of the 4-bit attention and the step plan; zero between launches
     w8a8::TpState* tp = nullptr;  // tensor-parallel exchange, when w8a8_tp_create was called
 };
 
@@ -198,8 +198,8 @@ int w8a8_create(w8a8_ctx** out, int device, size_t workspace_bytes) {
     e = cudaMalloc(&c->workspace, c->workspace_bytes);
     if (e == cudaSuccess) e = cudaMalloc(&c->device_status, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(c->device_status, 0, sizeof(int));
-    if (e == cudaSuccess) e = cudaMalloc(&c->tail_counters, (kTailCounterInts + kKv4Tickets) * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(c->tail_counters, 0, (kTailCounterInts + kKv4Tickets) * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&c->tail_counters, (kTailCounterInts + kTicketInts) * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(c->tail_counters, 0, (kTailCounterInts + kTicketInts) * sizeof(int));
     cudaSetDevice(prev);
     if (e != cudaSuccess) {
         cudaFree(c->workspace);
@@ -240,7 +240,7 @@ int w8a8_check_device_status(w8a8_ctx* ctx, void* stream) {
     if (host != 0) {
         cudaMemsetAsync(ctx->device_status, 0, sizeof(int), s);
         // a kernel that gave up may have left arrival counters half-counted
-        cudaMemsetAsync(ctx->tail_counters, 0, (kTailCounterInts + kKv4Tickets) * sizeof(int), s);
+        cudaMemsetAsync(ctx->tail_counters, 0, (kTailCounterInts + kTicketInts) * sizeof(int), s);
         return fail(W8A8_ERR_TIMEOUT, "a kernel gave up a bounded wait (code %d)", host);
     }
     return W8A8_OK;
@@ -576,6 +576,7 @@ int w8a8_plan_blocks(w8a8_ctx* ctx, const int* cached_lens, const int* new_lens,
     if (int rc = check_device(ctx, "plan_blocks")) return rc;
     return launch_plan_blocks(cached_lens, new_lens, batch, block_table, max_blocks_per_seq, free_blocks, free_capacity, free_count, free_count_out,
                               reinterpret_cast<long long*>(slots), positions, seq_lens, first_token, max_tokens, info,
+                              ctx->tail_counters + kTailCounterInts + kKv4Tickets,
                               static_cast<cudaStream_t>(stream));
 }
 

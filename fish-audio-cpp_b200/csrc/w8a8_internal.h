@@ -170,7 +170,7 @@ int launch_qkv_attention_decode(const __half* qkv, const __half* q_norm_w, const
 int plan_max_batch();
 int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* table, int max_blocks, int* free_blocks, int capacity,
                        const int* free_count, int* free_count_out, long long* slots, int* positions, int* seq_lens, int* first_token,
-                       int max_tokens, int* info, cudaStream_t stream);
+                       int max_tokens, int* info, int* ticket, cudaStream_t stream);
 // w8a8_kv4_store.cu : rows of the qkv projection into the 4-bit cache, and back.
 size_t kv4_page_bytes(int group);  // 0: no such group size
 int launch_kv4_write(const __half* qkv, const __half* q_norm_w, const __half* k_norm_w, float eps, const float* freqs, const int* positions,
@@ -180,6 +180,7 @@ int launch_kv4_read(const void* cache, int n_blocks, const long long* slots, int
                     __half* k_out, __half* v_out, cudaStream_t stream);
 // w8a8_kv4_attn.cu : decode attention over the 4-bit cache.
 constexpr int kKv4Tickets = 512;  // one per CTA
+constexpr int kTicketInts = kKv4Tickets + 1;  // and the step plan's; behind the tails' counters
 int kv4_max_batch();
 size_t kv4_attention_scratch(int n_q, int n_kv);
 int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const int* table, const int* lens, __half* out, int batch, int n_q,

@@ -3,9 +3,10 @@
 //   out[b, h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(q_h . k_t sm_scale - max),  t < seq_lens[b];  zeros where seq_lens[b] is 0
 //   k_t, v_t = code * scale of the row's group; one pass with the running maximum and sum of the softmax, both fp32
 //
-// Bound: HBM. A token costs 128 + 8 G bytes per kv head (K and V; G = 128 / group) instead of the fp16 cache's 512, so the unpacking
-// comes close behind: per 16 tokens of a kv head a warp executes some 300 instructions for 2304 bytes at groups of 32, where
-// an SM is fed a page every ~100 clocks.
+// Bound: HBM and the unpacking, close to one another. A token costs 128 + 4 G bytes per kv head (K and V; G = 128 / group) instead of the fp16
+// cache's 512; a warp executes some 350 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 74 us, 61 % of
+// the measured copy rate; the copies alone, without arithmetic, take 54, the arithmetic alone, on pages that lie in L2, 71. Half of the
+// instructions go to the half-rate pipe that masks and shifts; two pages at a time, scales folded into p, and 8 or 16 warps instead of 12 changed nothing.
 //
 // Split. The unit is a page: 16 tokens of one (sequence, kv head). All units of the batch, in the order sequence, head, page, are one
 // range that is cut evenly over the warps of the grid (a CTA's warps take neighbouring runs), whatever the lengths are: nobody waits
@@ -34,14 +35,12 @@ using q4::kTokens;
 
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
-#ifndef KV4_WHOLE
-#define KV4_WHOLE 96
-#endif
-#ifndef KV4_COST
-#define KV4_COST 4
-#endif
-constexpr int kWholePages = KV4_WHOLE;
-constexpr int kPairCost = KV4_COST;
+// Pairs of at most so many pages (and at most four times a CTA's share) are not cut between CTAs: a join costs what a warp's six to eight pages
+// cost. us with 32, 96 and 256: 8 x 1024 tokens 13.5, 12.4, 12.4; 64 x 1024 31, 29, 29; 64 x 4000 73, 73, 79; 1 x 1024 10.4 where cut, 11.6 whole.
+constexpr int kWholePages = 96;
+// Pages that a pair counts for beyond its own. us with 0, 2, 4 and 8: 48 ragged sequences up to 8000 tokens 34, 23.5, 23.2, 23.4; 200 up to 2000
+// tokens 50, 31.7, 32.1, 35.1; 64 x 512 20.5, 21.1, 21.3, 22.0.
+constexpr int kPairCost = 3;
 constexpr float kLag = 8.0f;  // p is at most 2^8: it keeps its precision in fp16
 
 struct Kv4Params {
@@ -229,19 +228,17 @@ __device__ __noinline__ void merge_pieces(const Kv4Params& p, const float* base,
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 // G groups per head; R the most query heads per kv head (4 or 8); W warps.
-template <int R>
-struct Shape {
-    static constexpr int kWarps = R == 4 ? 16 : 12;
-    static constexpr int kStages = 4;
-};
+// Twelve warps of 168 registers: with sixteen of 128 the long cases take the same (64 x 4000 tokens 74 us) and the short ones more (8 x 1024 tokens
+// 12.5 us instead of 12.0, 1 x 8192 13.0 instead of 12.2); with eight the long ones more (91). Four stages are 9 KB a warp on their way.
+constexpr int kWarps = 12, kStages = 4;
 template <int G, int R>
 constexpr int kv4_smem(int batch) {
-    return Shape<R>::kWarps * (Shape<R>::kStages * q4::page_bytes(G) + 2 * piece_floats(R) * 4) + (batch + 1) * 4;
+    return kWarps * (kStages * q4::page_bytes(G) + 2 * piece_floats(R) * 4) + (batch + 1) * 4;
 }
 
 template <int G, int R>
-__global__ void __launch_bounds__(Shape<R>::kWarps * 32, 1) kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
-    constexpr int W = Shape<R>::kWarps, D = Shape<R>::kStages, kPage = q4::page_bytes(G), kPiece = piece_floats(R);
+__global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
+    constexpr int W = kWarps, D = kStages, kPage = q4::page_bytes(G), kPiece = piece_floats(R);
     static_assert((D & (D - 1)) == 0 && D <= 32, "a stage is the low bits of a unit's number");
     extern __shared__ __align__(128) unsigned char kv4_smem_raw[];
     unsigned char* const ring_all = kv4_smem_raw;                                  // [W][D][kPage]
@@ -662,7 +659,7 @@ cudaError_t launch_kv4(const Kv4Params& p, int ctas, cudaStream_t stream) {
     static SmemAttribute attribute;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, 1, 1);
-    cfg.blockDim = dim3(Shape<R>::kWarps * 32, 1, 1);
+    cfg.blockDim = dim3(kWarps * 32, 1, 1);
     cfg.dynamicSmemBytes = kv4_smem<G, R>(p.batch);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -7,12 +7,14 @@
 //   ended (new_b < 0): its have_b blocks go on the stack, give_b = have_b
 //   others: take_b = ceil((cached_b + new_b) / 16) - have_b blocks come from the stack's top (after all that was given back)
 //   token i of request b has the position cached_b + i and the slot 16 * table[b][position / 16] + position % 16
-// Three exclusive prefix sums (tokens, blocks taken, blocks given) make every one of these independent of the others.
+// Three exclusive prefix sums (tokens, blocks taken, blocks given) make every one of these independent of the others; a block that was given
+// back and taken again in the same call is read from the row that gives it, so that nothing that is read is written by the call, but
+// for the lengths and the stack's count where the caller has them updated in place.
 //
 // Bound: latency at decode sizes (one round trip for the lengths, one for block numbers), 12 bytes written per token for prompts. One
-// launch: a CTA, or a cluster of eight for many tokens, whose CTAs all make the same sums and share the tokens; the barriers of the
-// cluster separate "read the old lengths, push" from "pop, write". All or nothing: where the blocks, the table's width, the token
-// count or a length do not fit, no request gets anything, and `info` says why.
+// launch: a CTA per 4096 tokens, each of which makes the sums again (200000 tokens: 20.1 us when a cluster of eight shared them) and then
+// four tokens a thread. What may be updated in place is written by the CTA that comes last (a ticket, reset by that CTA). All or nothing:
+// where the blocks, the table's width, the token count or a length do not fit, no request gets anything, and `info` says why.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 
@@ -40,6 +42,7 @@ struct PlanParams {
     int max_tokens;
     int* info;
     int vector_stores;  // slots and positions are 16-byte aligned
+    int* ticket;        // zero between launches
 };
 
 struct Sums {
@@ -50,11 +53,6 @@ __device__ __forceinline__ Sums shfl_up(Sums v, int d) {
     return {__shfl_up_sync(0xffffffffu, v.tokens, d), __shfl_up_sync(0xffffffffu, v.take, d), __shfl_up_sync(0xffffffffu, v.give, d)};
 }
 
-__device__ __forceinline__ void plan_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanParams p) {
     extern __shared__ int plan_smem[];
     int* first_s = plan_smem;                      // [batch + 1] tokens ahead of request b
@@ -63,7 +61,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
     int* cached_s = give_s + p.batch;              // [batch]; minus one minus the length where the request ended
     __shared__ Sums warp_s[kPlanThreads / 32];
     __shared__ Sums run_s;
-    __shared__ int bad_s;
+    __shared__ int bad_s, last_s;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int part = blockIdx.x, parts = gridDim.x;
@@ -132,40 +130,39 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
     if (count < 0 || top > p.capacity) status = 5;
     const bool ok = status == 8;
 
-    // blocks of requests that ended go on the stack; a warp a request
-    if (ok && all.give > 0)
-        for (int b = part * (kPlanThreads / 32) + warp; b < p.batch; b += parts * (kPlanThreads / 32)) {
-            const int cached = -1 - cached_s[b];
-            if (cached < 0) continue;
-            const int have = (cached + kPlanBlock - 1) / kPlanBlock;
-            for (int j = lane; j < have; j += 32)
-                p.free_blocks[count + give_s[b] + j] = p.table[static_cast<size_t>(b) * p.max_blocks + j];
-        }
-    // all inputs that an output may replace are read, all pushes are there
-    __syncthreads();
-    plan_cluster_sync();
-
+    __syncthreads();  // (first_s[0])
     const int threads = parts * kPlanThreads, me = part * kPlanThreads + tid;
-    for (int b = part * (kPlanThreads / 32) + warp; b < p.batch; b += parts * (kPlanThreads / 32)) {
-        const int cached = cached_s[b];
-        const int fresh = first_s[b + 1] - first_s[b];
-        if (lane == 0) {
-            p.seq_lens[b] = !ok ? max(0, cached < 0 ? -1 - cached : cached) : cached < 0 ? 0 : cached + fresh;
-            p.first_token[b + 1] = ok ? first_s[b + 1] : 0;
+    // the request that item x of a prefix sum belongs to: the last whose items start at or before it
+    auto owner = [&](const int* ahead, int x) {
+        int lo = 0, hi = p.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (ahead[mid] <= x) lo = mid; else hi = mid - 1;
         }
-        if (ok && cached >= 0) {
-            const int have = (cached + kPlanBlock - 1) / kPlanBlock, end = (cached + fresh + kPlanBlock - 1) / kPlanBlock;
-            for (int j = have + lane; j < end; j += 32)
-                p.table[static_cast<size_t>(b) * p.max_blocks + j] = __ldcg(p.free_blocks + (top - 1 - (take_s[b] + j - have)));
+        return lo;
+    };
+    auto given = [&](int x) {  // the x-th block given back
+        const int b = owner(give_s, x);
+        return p.table[static_cast<size_t>(b) * p.max_blocks + x - give_s[b]];
+    };
+    auto taken = [&](int x) {  // the x-th block taken: from the stack's top, what was given back first
+        const long long at = top - 1 - x;
+        return at < count ? p.free_blocks[at] : given(static_cast<int>(at - count));
+    };
+    if (ok) {  // a thread a block
+        for (long long x = me; x < all.give; x += threads) p.free_blocks[count + x] = given(static_cast<int>(x));
+        for (long long x = me; x < all.take; x += threads) {
+            const int b = owner(take_s, static_cast<int>(x)), have = (cached_s[b] + kPlanBlock - 1) / kPlanBlock;
+            p.table[static_cast<size_t>(b) * p.max_blocks + have + static_cast<int>(x) - take_s[b]] = taken(static_cast<int>(x));
         }
     }
+    for (int b = me; b < p.batch; b += threads) p.first_token[b + 1] = ok ? first_s[b + 1] : 0;
     if (me == 0) {
         p.first_token[0] = 0;
         p.info[0] = ok ? 0 : status;
         p.info[1] = ok ? static_cast<int>(all.tokens) : 0;
         p.info[2] = ok ? static_cast<int>(all.take) : 0;
         p.info[3] = static_cast<int>(ok ? top - all.take : count);
-        *p.free_count_out = static_cast<int>(ok ? top - all.take : count);
     }
     // four tokens a thread: one search, then forward
     const int tokens = ok ? static_cast<int>(all.tokens) : 0;
@@ -173,12 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
         long long slot[4] = {-1, -1, -1, -1};
         int pos[4] = {0, 0, 0, 0};
         if (t0 < tokens) {
-            int lo = 0, hi = p.batch - 1;  // the last request whose first token is not behind t0
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (first_s[mid] <= t0) lo = mid; else hi = mid - 1;
-            }
-            int b = lo;
+            int b = owner(first_s, static_cast<int>(t0)), seen_b = -1, seen_blk = -1, phys = -1;  // (four tokens lie in one block or two of a request, most of the time)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int t = static_cast<int>(t0) + e;
@@ -187,8 +179,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
                     const int cached = cached_s[b], have = (cached + kPlanBlock - 1) / kPlanBlock;
                     pos[e] = cached + t - first_s[b];
                     const int blk = pos[e] / kPlanBlock;
-                    const int phys = blk >= have ? __ldcg(p.free_blocks + (top - 1 - (take_s[b] + blk - have)))
-                                                 : __ldcg(p.table + static_cast<size_t>(b) * p.max_blocks + blk);
+                    if (b != seen_b || blk != seen_blk) {
+                        phys = blk >= have ? taken(take_s[b] + blk - have) : p.table[static_cast<size_t>(b) * p.max_blocks + blk];
+                        seen_b = b;
+                        seen_blk = blk;
+                    }
                     slot[e] = phys < 0 ? -1 : static_cast<long long>(phys) * kPlanBlock + pos[e] % kPlanBlock;
                 }
             }
@@ -204,6 +199,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
             }
         }
     }
+    // what may be an input too: when every CTA has read it
+    if (parts > 1) {
+        __syncthreads();
+        if (tid == 0) {
+            int before;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.ticket) : "memory");
+            last_s = before == parts - 1;
+            if (last_s) *p.ticket = 0;
+        }
+        __syncthreads();
+        if (!last_s) return;
+    }
+    for (int b = tid; b < p.batch; b += kPlanThreads) {
+        const int cached = cached_s[b], was = cached < 0 ? -1 - cached : cached;
+        p.seq_lens[b] = !ok ? was : cached < 0 ? 0 : cached + first_s[b + 1] - first_s[b];
+    }
+    if (tid == 0) *p.free_count_out = static_cast<int>(ok ? top - all.take : count);
 }
 
 SmemAttribute plan_attribute;
@@ -215,25 +227,21 @@ int plan_max_batch() { return kPlanMaxBatch; }
 
 int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* table, int max_blocks, int* free_blocks, int capacity,
                        const int* free_count, int* free_count_out, long long* slots, int* positions, int* seq_lens, int* first_token,
-                       int max_tokens, int* info, cudaStream_t stream) {
+                       int max_tokens, int* info, int* ticket, cudaStream_t stream) {
     PlanParams p = {cached, fresh, batch, table, max_blocks, free_blocks, capacity, free_count, free_count_out, slots, positions,
                     seq_lens, first_token, max_tokens, info,
-                    ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) & 15u) == 0};
-    const int parts = max_tokens > 4 * kPlanThreads || batch > kPlanThreads ? 8 : 1;
+                    ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) & 15u) == 0, ticket};
+    const int want = (max_tokens + 4 * kPlanThreads - 1) / (4 * kPlanThreads), sms = device_sms(), parts = want < 1 ? 1 : want < sms ? want : sms;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(parts, 1, 1);
     cfg.blockDim = dim3(kPlanThreads, 1, 1);
     cfg.dynamicSmemBytes = (4 * batch + 1) * 4;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = parts;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled(kPdlRow) ? 2 : 1;
+    cfg.numAttrs = pdl_enabled(kPdlRow) ? 1 : 0;
     const cudaError_t e = launch_with_smem(plan_attribute, kPlanSmem, cfg, plan_blocks_kernel, p);
     if (e != cudaSuccess) return fail(W8A8_ERR_CUDA, "plan_blocks launch: %s", cudaGetErrorString(e));
     return W8A8_OK;
