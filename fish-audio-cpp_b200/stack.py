@@ -18,6 +18,10 @@ Tensor parallelism (the reference has none): wqkv and w1|w3 are column-parallel 
 SwiGLU channels per rank), wo and w2 row-parallel with K cut at quantisation-group boundaries, so every
 per-group int32 sum and every activation scale stays on one rank; the only exchange is one fp16 sum
 all-reduce of [batch, 2560] after wo and after w2.
+
+In 4 bits (one GPU): weight_bits=4 holds the four projections as 4-bit codes with group scales (linear4_q in place of linear_q), kv_bits=4
+the paged cache in 4 bits; kv4_write and kv4_attention_decode then take the place of the fused attention call, and one
+plan_blocks call per step makes positions, lengths and slots, taking the cache's blocks from a free stack as sequences grow.
 """
 from __future__ import annotations
 
@@ -146,10 +150,14 @@ def synthetic_kv(torch, cfg: SlowARConfig, batch: int, context: int, max_new: in
 class SlowARStack:
     def __init__(self, torch, ctx: capi.Context, cfg: SlowARConfig, batch: int, context: int, max_new: int = 256,
                  tp_rank: int = 0, tp_size: int = 1, seed: int = 0, all_reduce=None, pack: bool = True,
-                 attn_splits: int = 0, tp_mode: str = "fused", gather_handles=None, fuse_norm: bool = True):
+                 attn_splits: int = 0, tp_mode: str = "fused", gather_handles=None, fuse_norm: bool = True,
+                 weight_bits: int = 8, kv_bits: int = 16, kv_group: int = 32):
         self.torch, self.ctx, self.cfg = torch, ctx, cfg
         self.B, self.tp_rank, self.tp_size = batch, tp_rank, tp_size
         self.all_reduce = all_reduce
+        assert weight_bits in (4, 8) and kv_bits in (4, 16) and (tp_size == 1 or (weight_bits, kv_bits) == (8, 16)), "4 bits: one GPU"
+        self.weight_bits, self.kv_bits, self.kv_group = weight_bits, kv_bits, kv_group
+        pack = pack and weight_bits == 8  # (the 4-bit linear streams row-major codes as they are)
         self.attn_splits = int(os.environ.get("W8A8_STACK_ATTN_SPLITS", attn_splits))
         # "fused": the exchange happens inside the residual+norm+quant kernel over peer memory;
         # "nccl": a library all-reduce between the projection and that kernel (the baseline).
@@ -166,7 +174,7 @@ class SlowARStack:
         # w1|w3; five launches per layer. Measured slower than the eight-launch form inside a replayed graph (a tail
         # costs what the launch it replaces costs, and the next linear's prefetch overlaps less), so it is off by default.
         self.tails = (tp_size == 1 and pack and batch <= 8 and cfg.group in (64, 128, 256) and not self.fuse_norm and
-                      os.environ.get("W8A8_STACK_TAILS", "0") == "1")
+                      kv_bits == 16 and os.environ.get("W8A8_STACK_TAILS", "0") == "1")
         # qk-norm + RoPE + KV write inside the attention launch (W8A8_STACK_FUSE_ROPE=0: as two launches)
         self.fuse_rope = os.environ.get("W8A8_STACK_FUSE_ROPE", "1") == "1"
         c = cfg
@@ -191,12 +199,15 @@ class SlowARStack:
             so = f["so"][:, q_lo // g:q_hi // g].contiguous()
             w1, s1 = f["w1"][self.inter_lo:self.inter_hi].contiguous(), f["s1"][self.inter_lo:self.inter_hi].contiguous()
             w3, s3 = f["w3"][self.inter_lo:self.inter_hi].contiguous(), f["s3"][self.inter_lo:self.inter_hi].contiguous()
-            G = c.dim // g
-            w13 = torch.empty((2 * self.inter_l, c.dim), dtype=torch.int8, device=dev)
-            s13 = torch.empty((2 * self.inter_l, G), dtype=torch.float16, device=dev)
-            ctx.pack_gate_up(w1, s1, w3, s3, self.inter_l, c.dim, G, w13, s13)
             w2 = f["w2"][:, self.inter_lo:self.inter_hi].contiguous()
             s2 = f["s2"][:, self.inter_lo // g:self.inter_hi // g].contiguous()
+            if weight_bits == 4:
+                (wqkv, sqkv), (wo, so), (w1, s1), (w3, s3), (w2, s2) = (
+                    self._weight4(w, s) for w, s in ((wqkv, sqkv), (wo, so), (w1, s1), (w3, s3), (w2, s2)))
+            G = c.dim // g
+            w13 = torch.empty((2 * self.inter_l, w1.shape[1]), dtype=w1.dtype, device=dev)
+            s13 = torch.empty((2 * self.inter_l, G), dtype=torch.float16, device=dev)
+            ctx.pack_gate_up(w1, s1, w3, s3, self.inter_l, w1.shape[1], G, w13, s13)
             torch.cuda.synchronize()
             lw = dict(attn_norm=f["attn_norm"], ffn_norm=f["ffn_norm"], q_norm=f["q_norm"], k_norm=f["k_norm"],
                       wqkv=wqkv, sqkv=sqkv, wo=wo, so=so, w13=w13, s13=s13, w2=w2, s2=s2)
@@ -221,6 +232,8 @@ class SlowARStack:
         self.positions = torch.full((batch,), context, dtype=torch.int32, device=dev)   # the new token's position
         self.seq_lens = torch.full((batch,), context + 1, dtype=torch.int32, device=dev)
         self.context0 = context
+        if kv_bits == 4:
+            self._cache4(context)
 
         B = batch
         h16 = dict(dtype=torch.float16, device=dev)
@@ -241,11 +254,50 @@ class SlowARStack:
         self.launches_per_step = c.n_layer * ((7 if self.fuse_norm else 9) - (1 if self.fuse_rope else 0)) + 2
         if self.tails:
             self.launches_per_step = c.n_layer * (5 if self.fuse_rope else 6) + 1
+        if kv_bits == 4:
+            self.launches_per_step = c.n_layer * 9 + 3
         # bytes the step must move at least once (per rank): weights + scales + the KV it reads
         wbytes = sum(lw[n].numel() + lw[s].numel() * 2 for lw in self.layers
                      for n, s in (("wqkv", "sqkv"), ("wo", "so"), ("w13", "s13"), ("w2", "s2")))
         self.weight_bytes = wbytes
-        self.kv_bytes_per_step = lambda ctx_len: 2 * B * ctx_len * c.n_layer * self.nkv_l * D * 2
+        kv_row = 2 * D * 2 if kv_bits == 16 else capi.kv4_cache_bytes(1, 1, 1, D, kv_group) // c.block_tokens  # k and v of a token and kv head
+        self.kv_bytes_per_step = lambda ctx_len: B * ctx_len * c.n_layer * self.nkv_l * kv_row
+
+    def _weight4(self, w, s):
+        """A weight in 4 bits from its int8 codes and scales: what a loader does with the fp16 values of a checkpoint."""
+        torch, (n, k), g = self.torch, w.shape, self.cfg.group
+        values = (w.float().view(n, k // g, g) * s.float().view(n, k // g, 1)).view(n, k).half()
+        w4 = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+        s4 = torch.empty((n, k // g), dtype=torch.float16, device=w.device)
+        self.ctx.quantize_weight4(values, n, k, g, w4, s4)
+        return w4, s4
+
+    def _cache4(self, context):
+        """The synthetic prefill of the fp16 cache in 4 bits, and what plan_blocks works on: the table holds the context's blocks only,
+        those of the tokens to come wait on a free stack."""
+        torch, c, B, dev = self.torch, self.cfg, self.B, "cuda"
+        nblocks, n = self.k_cache.shape[0], self.nkv_l
+        self.cache4 = torch.empty(capi.kv4_cache_bytes(nblocks, c.n_layer, n, c.head_dim, self.kv_group), dtype=torch.uint8, device=dev)
+        self.n_blocks = nblocks
+        slots = torch.arange(nblocks * c.block_tokens, dtype=torch.int64, device=dev)
+        for l in range(c.n_layer):
+            rows = torch.cat([x[:, l].transpose(1, 2).reshape(-1, n, c.head_dim) for x in (self.k_cache, self.v_cache)], 1)
+            self.ctx.kv4_write(rows.contiguous(), slots, self.cache4, nblocks, l, c.n_layer, slots.numel(), 0, n, c.head_dim, self.kv_group)
+            torch.cuda.synchronize()
+        self.k_cache = self.v_cache = None
+        have = (context + c.block_tokens - 1) // c.block_tokens
+        self.free_blocks = torch.cat([self.block_table[:, have:].flatten().flip(0), self.block_table[:, :have].flatten()]).contiguous()
+        self.block_table[:, have:] = -1
+        self.free0 = B * (self.max_blocks - have)
+        self.free_count = torch.tensor([self.free0], dtype=torch.int32, device=dev)
+        self.new_lens = torch.ones((B,), dtype=torch.int32, device=dev)
+        self.seq_lens.fill_(context)  # tokens in the cache; a step's plan adds its own
+        self.slots = torch.empty((B,), dtype=torch.int64, device=dev)
+        self.first_token = torch.empty((B + 1,), dtype=torch.int32, device=dev)
+        self.plan_info = torch.empty((4,), dtype=torch.int32, device=dev)
+
+    def _linear(self, w, s, xq, xs, y, n, k, epilogue=capi.EPI_NONE):
+        (self.ctx.linear4_q if self.weight_bits == 4 else self.ctx.linear_q)(w, s, self.cfg.group, xq, xs, y, self.B, n, k, epilogue=epilogue)
 
     # ------------------------------------------------------------------------------------------
     def decode_step(self, x_in=None):
@@ -260,6 +312,9 @@ class SlowARStack:
         sm_scale = 1.0 / math.sqrt(D)
         if self.tails:
             return self._decode_step_tails(sm_scale)
+        if self.kv_bits == 4:
+            ctx.plan_blocks(self.seq_lens, self.new_lens, B, self.block_table, self.max_blocks, self.free_blocks, self.free_blocks.numel(),
+                            self.free_count, self.slots, self.positions, self.seq_lens, self.first_token, B, self.plan_info)
         pending = False  # a projection output waiting to be added to the residual stream
         x, x_alt = self.x, self.x_alt
         for l, lw in enumerate(self.layers):
@@ -275,8 +330,14 @@ class SlowARStack:
                 ctx.rmsnorm_quantize(self.x, lw["attn_norm"], c.eps, B, c.dim, g, self.xq, self.xs,
                                      residual=self.delta if pending else None)
             if not self.fuse_norm:
-                ctx.linear_q(lw["wqkv"], lw["sqkv"], g, self.xq, self.xs, self.qkv, B, self.qkv_n, c.dim)
-            if self.fuse_rope:
+                self._linear(lw["wqkv"], lw["sqkv"], self.xq, self.xs, self.qkv, self.qkv_n, c.dim)
+            if self.kv_bits == 4:
+                ctx.kv4_write(self.qkv, self.slots, self.cache4, self.n_blocks, l, c.n_layer, B, self.nq_l, self.nkv_l, D, self.kv_group,
+                              q_norm_w=lw["q_norm"], k_norm_w=lw["k_norm"], eps=c.eps, freqs=self.freqs, positions=self.positions, q_out=self.q)
+                ctx.kv4_attention_decode(self.q, self.cache4, self.n_blocks, self.block_table, self.seq_lens, None, B, self.nq_l, D,
+                                         self.max_blocks, sm_scale, l, c.n_layer, self.nkv_l, self.kv_group, quant_group_size=g,
+                                         Xq=self.aq, Xs=self.as_)
+            elif self.fuse_rope:
                 ctx.qkv_attention_decode(self.qkv, lw["q_norm"], lw["k_norm"], c.eps, self.freqs, self.positions,
                                          self.k_cache, self.v_cache, self.block_table, self.seq_lens, None, B, self.nq_l,
                                          D, self.max_blocks, sm_scale, l, c.n_layer, self.nkv_l, quant_group_size=g,
@@ -292,7 +353,7 @@ class SlowARStack:
             if self.tp_fused:  # the partial goes from the kernel's epilogue into every rank's exchange buffer
                 ctx.tp_linear_q(lw["wo"], lw["so"], g, self.aq, self.as_, B, c.dim, self.attn_k)
             else:
-                ctx.linear_q(lw["wo"], lw["so"], g, self.aq, self.as_, self.delta, B, c.dim, self.attn_k)
+                self._linear(lw["wo"], lw["so"], self.aq, self.as_, self.delta, c.dim, self.attn_k)
             if self.all_reduce is not None:
                 self.all_reduce(self.delta)
             if self.fuse_norm:
@@ -306,13 +367,12 @@ class SlowARStack:
                 else:
                     ctx.rmsnorm_quantize(self.x, lw["ffn_norm"], c.eps, B, c.dim, g, self.xq, self.xs,
                                          residual=self.delta)
-                ctx.linear_q(lw["w13"], lw["s13"], g, self.xq, self.xs, self.act, B, 2 * self.inter_l, c.dim,
-                             epilogue=capi.EPI_SWIGLU)
+                self._linear(lw["w13"], lw["s13"], self.xq, self.xs, self.act, 2 * self.inter_l, c.dim, epilogue=capi.EPI_SWIGLU)
             ctx.quantize(self.act, B, self.inter_l, g, self.actq, self.acts)
             if self.tp_fused:
                 ctx.tp_linear_q(lw["w2"], lw["s2"], g, self.actq, self.acts, B, c.dim, self.inter_l)
             else:
-                ctx.linear_q(lw["w2"], lw["s2"], g, self.actq, self.acts, self.delta, B, c.dim, self.inter_l)
+                self._linear(lw["w2"], lw["s2"], self.actq, self.acts, self.delta, c.dim, self.inter_l)
             if self.all_reduce is not None:
                 self.all_reduce(self.delta)
             pending = True
@@ -321,8 +381,9 @@ class SlowARStack:
         else:
             ctx.residual_add(x, self.delta, B * c.dim)
             ctx.rms_norm(x, self.final_norm, self.out, B, c.dim, c.eps)
-        self.positions.add_(1)
-        self.seq_lens.add_(1)
+        if self.kv_bits == 16:
+            self.positions.add_(1)
+            self.seq_lens.add_(1)
         return self.out
 
     def _attention(self, l, lw, sm_scale):
@@ -367,7 +428,7 @@ class SlowARStack:
         """The w8a8_decode_stack descriptor of this stack (single GPU, packed weights), built once."""
         if getattr(self, "_desc", None) is not None:
             return self._desc
-        assert self.tp_size == 1, "the one-launch step is the single-GPU form"
+        assert self.tp_size == 1 and (self.weight_bits, self.kv_bits) == (8, 16), "the one-launch step is the single-GPU form in 8 and 16 bits"
         torch, c = self.torch, self.cfg
         rows = []
         for lw in self.layers:
@@ -399,13 +460,12 @@ class SlowARStack:
     def linears_only(self):
         """Only the four W8A8 linears of every layer, on whatever the activation buffers hold: the
         benchmark times these alone to put the dominant kernel on the roofline."""
-        c, ctx, B, g = self.cfg, self.ctx, self.B, self.cfg.group
+        c = self.cfg
         for lw in self.layers:
-            ctx.linear_q(lw["wqkv"], lw["sqkv"], g, self.xq, self.xs, self.qkv, B, self.qkv_n, c.dim)
-            ctx.linear_q(lw["wo"], lw["so"], g, self.aq, self.as_, self.delta, B, c.dim, self.attn_k)
-            ctx.linear_q(lw["w13"], lw["s13"], g, self.xq, self.xs, self.act, B, 2 * self.inter_l, c.dim,
-                         epilogue=capi.EPI_SWIGLU)
-            ctx.linear_q(lw["w2"], lw["s2"], g, self.actq, self.acts, self.delta, B, c.dim, self.inter_l)
+            self._linear(lw["wqkv"], lw["sqkv"], self.xq, self.xs, self.qkv, self.qkv_n, c.dim)
+            self._linear(lw["wo"], lw["so"], self.aq, self.as_, self.delta, c.dim, self.attn_k)
+            self._linear(lw["w13"], lw["s13"], self.xq, self.xs, self.act, 2 * self.inter_l, c.dim, epilogue=capi.EPI_SWIGLU)
+            self._linear(lw["w2"], lw["s2"], self.actq, self.acts, self.delta, c.dim, self.inter_l)
 
     def close(self):
         """Removes this stack's weights from the context's packed-weight registry (before the tensors are freed)."""
@@ -414,5 +474,9 @@ class SlowARStack:
         self._registered = []
 
     def reset_positions(self):
+        if self.kv_bits == 4:  # (the blocks taken since go back on the stack, where the next steps find them in the same order)
+            self.seq_lens.fill_(self.context0)
+            self.free_count.fill_(self.free0)
+            return
         self.positions.fill_(self.context0)
         self.seq_lens.fill_(self.context0 + 1)
