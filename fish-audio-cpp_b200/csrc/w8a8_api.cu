@@ -618,7 +618,8 @@ int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, i
     if (int rc = check_kv4(ctx, "kv4_attention_decode", cache, n_blocks, layer, n_layers, batch, n_heads, n_kv_heads, head_dim, group_size)) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8)
         return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: %d query heads over %d kv heads (1 to 8 each are built)", n_heads, n_kv_heads);
-    if (max_blocks_per_seq <= 0 || max_blocks_per_seq > (1 << 26) / n_kv_heads || (batch > 0 && max_blocks_per_seq > (1 << 30) / batch))
+    if (max_blocks_per_seq <= 0 || max_blocks_per_seq > (1 << 26) / n_kv_heads ||
+        static_cast<long long>(batch) * n_kv_heads * (static_cast<long long>(max_blocks_per_seq) + 8) > 0x7fffffffll)
         return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: a table of %d x %d blocks", batch, max_blocks_per_seq);
     if (batch > kv4_max_batch()) return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: batch %d (at most %d)", batch, kv4_max_batch());
     if (batch > 0 && (!q || !block_table || !seq_lens || (!out && !Xq))) return fail(W8A8_ERR_INVALID_ARG, "kv4_attention_decode: null pointer");

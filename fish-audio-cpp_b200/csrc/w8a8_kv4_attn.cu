@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     int* const first_s = reinterpret_cast<int*>(pieces + W * 2 * kPiece);          // [batch + 1]: table entries in use ahead of a sequence
     __shared__ __align__(8) uint64_t full_bar[W][D];
     __shared__ int scan_s[W + 1];
-    __shared__ long long piece_pair[2 * W];  // the pair of a piece, or -1
+    __shared__ int piece_pair[2 * W];  // the pair of a piece, or -1
     __shared__ int last_s[2];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -292,70 +292,62 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         for (int b = b0; b < b1; ++b) first_s[b + 1] = at += entries_of(b);
     }
     __syncthreads();
-    const long long units = static_cast<long long>(first_s[p.batch]) * p.n_kv;
+    const int units = first_s[p.batch] * p.n_kv;
 
-    // the sequence of a unit
-    auto sequence_of = [&](long long u) {
-        const int entry = static_cast<int>(u / p.n_kv);  // (a sequence's units are those of its entries, whatever their order in it)
+    // ---- this warp's run (all numbers below 2^31: the host sees to it) ----
+    // The range is cut by cost: a pair counts kPairCost pages more than it has (its q, its piece, its output; a run of many short pairs would
+    // else last longest). Cost v of the range is cost v - of pairs ahead - kPairCost pages into its pair, none where that is negative.
+    const int costs = units + kPairCost * p.batch * p.n_kv;
+    const int cta_cost = max(static_cast<int>((costs + gridDim.x - 1) / gridDim.x), 1);
+    auto cost_ahead = [&](int b) { return (first_s[b] + kPairCost * b) * p.n_kv; };
+    auto last_at = [&](auto ahead, int v) {  // the last sequence b with ahead(b) <= v
         int a = 0, z = p.batch - 1;
 #pragma unroll 1
         while (a < z) {
             const int mid = (a + z + 1) >> 1;
-            if (first_s[mid] <= entry) a = mid; else z = mid - 1;
+            if (ahead(mid) <= v) a = mid; else z = mid - 1;
         }
-        return a;  // (the last of those that start at or before u: empty ones in front of it start there too)
+        return a;
     };
-    // ---- this warp's run ----
-    // The range is cut by cost: a pair counts kPairCost pages more than it has (its q, its piece, its output; a run of many short pairs would
-    // else last longest). Cost v of the range is cost v - of pairs ahead - kPairCost pages into its pair, none where that is negative.
-    const long long costs = units + static_cast<long long>(kPairCost) * p.batch * p.n_kv;
-    const long long cta_cost = max((costs + gridDim.x - 1) / gridDim.x, 1ll);
-    auto cost_ahead = [&](int b) { return (static_cast<long long>(first_s[b]) + static_cast<long long>(kPairCost) * b) * p.n_kv; };
     struct Place {
         int b, h, in, of;  // cost `in` of `of` of the pair (b, h)
     };
-    auto place_of = [&](long long v) {
-        int a = 0, z = p.batch - 1;
-#pragma unroll 1
-        while (a < z) {
-            const int mid = (a + z + 1) >> 1;
-            if (cost_ahead(mid) <= v) a = mid; else z = mid - 1;
-        }
-        const int of = first_s[a + 1] - first_s[a] + kPairCost, rest = static_cast<int>(v - cost_ahead(a)), h = rest / of;
-        return Place{a, h, rest - h * of, of};
+    auto place_of = [&](int v) {
+        const int b = last_at(cost_ahead, v), of = first_s[b + 1] - first_s[b] + kPairCost, rest = v - cost_ahead(b), h = rest / of;
+        return Place{b, h, rest - h * of, of};
     };
-    auto pages_ahead = [&](long long v) {  // units ahead of cost v
-        if (v >= costs) return units;
-        const Place x = place_of(v);
-        return static_cast<long long>(first_s[x.b]) * p.n_kv + static_cast<long long>(x.h) * (x.of - kPairCost) + max(0, x.in - kPairCost);
-    };
-    // Where CTA c's run begins: at c cta_cost, but not inside a pair of few pages, which goes to one side or the other as a whole.
-    const long long whole_pages = min(static_cast<long long>(kWholePages), 4 * cta_cost);
-    auto border = [&](long long c) {
-        const long long v = c * cta_cost;
-        if (v >= costs) return costs;
-        const Place x = place_of(v);
-        return x.of - kPairCost > whole_pages ? v : 2 * x.in < x.of ? v - x.in : v - x.in + x.of;
-    };
-    long long at_border = border(blockIdx.x + (lane & 1));  // lanes 0, 1: the CTA's run, from and to; lanes 2, 3: the warp's
+    // Lanes 0, 1: where the CTA's run begins and ends; lanes 2, 3: the warp's. A CTA's borders are at multiples of cta_cost, but not inside a
+    // pair of few pages, which goes to one side or the other as a whole.
+    int at_border;
     {
-        const long long from = __shfl_sync(0xffffffffu, at_border, 0), to = __shfl_sync(0xffffffffu, at_border, 1);
-        if (lane & 2) at_border = min(to, from + (warp + (lane & 1)) * ((to - from + W - 1) / W));
-        at_border = pages_ahead(at_border);
+        const int whole_pages = min(kWholePages, 4 * cta_cost);
+        const long long nominal = static_cast<long long>(blockIdx.x + (lane & 1)) * cta_cost;
+        int v = static_cast<int>(min(nominal, static_cast<long long>(costs)));
+#pragma unroll 1
+        for (int step = 0; step < 2; ++step) {  // (two rounds through one copy of the code: the CTA's borders, then all four in pages)
+            Place x = {0, 0, 0, kPairCost};
+            if (v < costs) x = place_of(v);
+            if (step == 0) {
+                if (v < costs && x.of - kPairCost <= whole_pages) v += 2 * x.in < x.of ? -x.in : x.of - x.in;
+                const int from = __shfl_sync(0xffffffffu, v, 0), to = __shfl_sync(0xffffffffu, v, 1);
+                if (lane & 2) v = min(to, from + (warp + (lane & 1)) * ((to - from + W - 1) / W));
+            } else {
+                v = v < costs ? first_s[x.b] * p.n_kv + x.h * (x.of - kPairCost) + max(0, x.in - kPairCost) : units;
+            }
+        }
+        at_border = v;
     }
-    const long long cta_lo = __shfl_sync(0xffffffffu, at_border, 0), cta_hi = __shfl_sync(0xffffffffu, at_border, 1);
-    const long long lo = __shfl_sync(0xffffffffu, at_border, 2);
-    const int n_mine = static_cast<int>(__shfl_sync(0xffffffffu, at_border, 3) - lo);
+    const int cta_lo = __shfl_sync(0xffffffffu, at_border, 0), cta_hi = __shfl_sync(0xffffffffu, at_border, 1);
+    const int lo = __shfl_sync(0xffffffffu, at_border, 2), n_mine = __shfl_sync(0xffffffffu, at_border, 3) - lo;
+    auto units_ahead = [&](int b) { return first_s[b] * p.n_kv; };
 
     const uint32_t ring = ptx::smem_u32(ring_all) + warp * (D * kPage);
     int page_of = 0;  // the page's number in the cache of unit (i & ~31) + lane of the run
     auto look_up = [&](int i0) {
         const int i = i0 + lane;
         if (i < n_mine) {
-            const long long u = lo + i;
-            const int b = sequence_of(u);
-            const int blocks = first_s[b + 1] - first_s[b];
-            const int rest = static_cast<int>(u - static_cast<long long>(first_s[b]) * p.n_kv), h = rest / blocks, blk = rest - h * blocks;
+            const int u = lo + i, b = last_at(units_ahead, u);  // (the last of those that start at or before u: empty ones in front of it start there too)
+            const int blocks = first_s[b + 1] - first_s[b], rest = u - units_ahead(b), h = rest / blocks, blk = rest - h * blocks;
             int phys = p.table[static_cast<size_t>(b) * p.max_blocks + blk];
             if (phys < 0 || phys >= p.n_blocks) phys = 0;  // (the caller's mistake; reads stay inside the cache)
             page_of = (phys * p.n_layers + p.layer) * p.n_kv + h;
@@ -380,13 +372,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
 
     const int g8 = lane >> 2, j4 = lane & 3;
     bool failed = false;
-    int b = n_mine > 0 ? sequence_of(lo) : 0;
+    int b = n_mine > 0 ? last_at(units_ahead, lo) : 0;
     for (int i = 0; i < n_mine;) {
         // ---- the next pair of the run ----
-        const long long u0 = lo + i;
-        while (static_cast<long long>(first_s[b + 1]) * p.n_kv <= u0) ++b;
-        const int blocks = first_s[b + 1] - first_s[b];
-        const int rest = static_cast<int>(u0 - static_cast<long long>(first_s[b]) * p.n_kv), kvh = rest / blocks, blk0 = rest - kvh * blocks;
+        const int u0 = lo + i;
+        while (units_ahead(b + 1) <= u0) ++b;
+        const int blocks = first_s[b + 1] - first_s[b], rest = u0 - units_ahead(b), kvh = rest / blocks, blk0 = rest - kvh * blocks;
         const int i_end = min(n_mine, i + blocks - blk0);
         int tokens = min(max(p.lens[b], 0), cap) - blk0 * kTokens;  // from the page's first on
 
@@ -572,39 +563,38 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             merge_pieces<R>(p, piece, 1u, nullptr, b, kvh);
             __syncwarp();
         } else if (lane == 0) {
-            piece_pair[2 * warp + (head ? 0 : 1)] = static_cast<long long>(b) * p.n_kv + kvh;
+            piece_pair[2 * warp + (head ? 0 : 1)] = b * p.n_kv + kvh;
         }
     }
     __syncthreads();
 
     // ---- pieces that meet in the CTA: chains of neighbours of one pair; a warp a chain ----
-    auto pair_units = [&](long long pair, long long& from, long long& to) {
-        const int pb = static_cast<int>(pair / p.n_kv), ph = static_cast<int>(pair % p.n_kv);
-        const int blocks = first_s[pb + 1] - first_s[pb];
-        from = static_cast<long long>(first_s[pb]) * p.n_kv + static_cast<long long>(ph) * blocks;
+    auto pair_units = [&](int pair, int& from, int& to) {
+        const int pb = pair / p.n_kv, blocks = first_s[pb + 1] - first_s[pb];
+        from = units_ahead(pb) + (pair - pb * p.n_kv) * blocks;
         to = from + blocks;
     };
     // (lane x of every warp looks at piece x; a chain starts where the piece in front of it is another pair's)
-    const long long pair_x = lane < 2 * W ? piece_pair[lane] : -1;
+    const int pair_x = lane < 2 * W ? piece_pair[lane] : -1;
     const uint32_t there = __ballot_sync(0xffffffffu, pair_x >= 0);
     const uint32_t in_front = there & ((1u << lane) - 1);
-    const long long pair_before = __shfl_sync(0xffffffffu, pair_x, in_front ? 31 - __clz(in_front) : 0);
+    const int pair_before = __shfl_sync(0xffffffffu, pair_x, in_front ? 31 - __clz(in_front) : 0);
     const uint32_t starts = __ballot_sync(0xffffffffu, pair_x >= 0 && (!in_front || pair_before != pair_x));
-    long long open[2] = {-1, -1};  // pairs that go on in other CTAs: one that began ahead of this CTA's run, one that ends behind it
+    int open[2] = {-1, -1};  // pairs that go on in other CTAs: one that began ahead of this CTA's run, one that ends behind it
     int chain = 0;
 #pragma unroll 1
     for (uint32_t todo = starts; todo; todo &= todo - 1, ++chain) {
         const int x = __ffs(todo) - 1;
         const uint32_t later = todo & (todo - 1);
         const uint32_t mine = there & (0xffffffffu << x) & (later ? (1u << (__ffs(later) - 1)) - 1 : 0xffffffffu);
-        const long long pair = __shfl_sync(0xffffffffu, pair_x, x);
-        long long from, to;
+        const int pair = __shfl_sync(0xffffffffu, pair_x, x);
+        int from, to;
         pair_units(pair, from, to);
         const bool whole = from >= cta_lo && to <= cta_hi, before = from < cta_lo;
         if (!whole) open[before ? 0 : 1] = pair;
         if (chain % W != warp) continue;
         merge_pieces<R>(p, pieces, mine, whole ? nullptr : p.scratch + (2ll * blockIdx.x + (before ? 0 : 1)) * kPiece,
-                        static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
+                        pair / p.n_kv, pair % p.n_kv);
     }
 
     // ---- pairs that lie in several CTAs: the last of them to come here adds their pieces; half of the warps see to either open pair ----
@@ -613,13 +603,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     {
         constexpr int kHalf = W / 2;
         const int side = warp >= kHalf, w = warp - side * kHalf;
-        const long long pair = open[side];
+        const int pair = open[side];
         if (pair >= 0) {
-            long long from, to;
+            int from, to;
             pair_units(pair, from, to);
-            const long long first_cost = from + cost_ahead(static_cast<int>(pair / p.n_kv)) - static_cast<long long>(first_s[pair / p.n_kv]) * p.n_kv +
-                                         static_cast<long long>(kPairCost) * (pair % p.n_kv + 1);  // of the pair's first page
-            const int c0 = static_cast<int>(first_cost / cta_cost), c1 = static_cast<int>((first_cost + (to - from) - 1) / cta_cost), n = c1 - c0 + 1;
+            const int first_cost = from + kPairCost * (pair + 1);  // of the pair's first page
+            const int c0 = first_cost / cta_cost, c1 = (first_cost + (to - from) - 1) / cta_cost, n = c1 - c0 + 1;
             auto half_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + side), "n"(kHalf * 32) : "memory"); };
             if (w == 0 && lane == 0) {  // (releases what the CTA's warps stored ahead of the barrier, acquires what the others' released)
                 int before;
@@ -643,7 +632,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                 if (x0 < x1) s.store(mine, lane);
                 half_barrier();
                 if (w == 0)
-                    merge_pieces<R>(p, mine, (1u << ((n + run - 1) / run)) - 1, nullptr, static_cast<int>(pair / p.n_kv), static_cast<int>(pair % p.n_kv));
+                    merge_pieces<R>(p, mine, (1u << ((n + run - 1) / run)) - 1, nullptr, pair / p.n_kv, pair % p.n_kv);
             }
         }
     }
