@@ -44,6 +44,8 @@ struct L4Params {
     int boxes;   // per tile
     int stages;  // of a warp's ring
     int pitch;   // of a row of codes in shared memory
+    int cta_tiles, longer;  // tiles of a CTA; the first `longer` CTAs have one more
+    unsigned box_magic;     // 2^32 / boxes, rounded up (0: one box): x / boxes is the high word of x box_magic while x boxes < 2^32
     int* status;
 };
 
@@ -114,12 +116,13 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
     const int row8 = (g8 & 1) << 2 | (g8 & 2) | g8 >> 2;  // the row of the tile that this lane's fragment row is (and + 8)
     // tiles [t0, t0 + nt) of this CTA, units [u0, u0 + n_mine) of this warp: the boxes of the CTA's tiles, one tile after the other
-    const int t0 = static_cast<int>(static_cast<long long>(p.tiles) * blockIdx.x / gridDim.x);
-    const int nt = static_cast<int>(static_cast<long long>(p.tiles) * (blockIdx.x + 1) / gridDim.x) - t0;
+    const int cta = blockIdx.x, t0 = cta * p.cta_tiles + min(cta, p.longer), nt = p.cta_tiles + (cta < p.longer ? 1 : 0);
     const int all = nt * p.boxes;
-    const int u0 = static_cast<int>(static_cast<long long>(all) * warp / kL4Warps);
-    const int n_mine = static_cast<int>(static_cast<long long>(all) * (warp + 1) / kL4Warps) - u0;
-    int tile = t0 + u0 / p.boxes, box = u0 % p.boxes;
+    auto run_at = [&](int w) { return all * w / kL4Warps; };  // (below 2^31: the host sees to it; all is not negative)
+    auto tile_of = [&](int unit) { return p.box_magic ? static_cast<int>(__umulhi(static_cast<unsigned>(unit), p.box_magic)) : unit; };
+    const int u0 = run_at(warp), n_mine = run_at(warp + 1) - u0;
+    const int first_tile = tile_of(u0);
+    int tile = t0 + first_tile, box = u0 - first_tile * p.boxes;
     bool head = box > 0;  // the tile began in another warp's run
 
     const uint32_t ring = ptx::smem_u32(base) + warp * p.stages * kBox;
@@ -136,13 +139,13 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
             ++l_tile;
         }
     };
-    if (lane == 0) {
-        for (int i = 0; i < p.stages; ++i) ptx::mbar_init(&full_bar[warp][i], 1);
-        if (warp == 0) ptx::mbar_init(&codes_bar, 1);
-        ptx::fence_barrier_init();
-        ptx::fence_proxy_async();
+    if (lane < p.stages) ptx::mbar_init(&full_bar[warp][lane], 1);
+    if (tid == 0) ptx::mbar_init(&codes_bar, 1);
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0)
         for (int i = 0; i < min(p.stages, n_mine); ++i) issue(i);
-    }
     // weight scales of the box that comes next, rows row8 and row8 + 8
     __half2 ws_next[P > 1 ? P : 1];  // EXACT, P > 1: [row half][P / 2 pairs of groups]; else one {row, row + 8} pair per promote
     auto group_of = [&](int bx, int pr) { return EXACT ? bx * P + pr : min(p.G - 1, (bx * kBoxK + pr * (kBoxK / P)) / p.g); };
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         load_scales(box);
     }
     ptx::pdl_wait();
-    ptx::pdl_launch_dependents();
+    ptx::pdl_launch_dependents();  // (at the start it costs 1 % of a step: what is launched then takes room)
 
     // ---- the activations ----
     // DIRECT: a lane's codes of a box in registers, asked for a box ahead. Else rows as they are in shared memory, each by one bulk copy, then the eight
@@ -404,8 +407,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
 
     // ---- tiles that a border between warps cuts: lane w looks at the border in front of warp w; a tile counts at its first border ----
     const bool swiglu = p.epilogue == W8A8_EPI_SWIGLU;
-    auto run_at = [&](int w) { return static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(all)) * w / kL4Warps); };
-    const int border = run_at(min(lane, kL4Warps)), cut_at = border / p.boxes;
+    const int border = run_at(min(lane, kL4Warps)), cut_at = tile_of(border);
     const bool cuts = lane > 0 && lane < kL4Warps && border != cut_at * p.boxes;
     const bool cuts_before = __shfl_up_sync(0xffffffffu, cuts, 1);
     const int cut_before = __shfl_up_sync(0xffffffffu, cut_at, 1);
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         while (x >= (c + 1) * elements) ++c;
         uint32_t rest = cut_tiles;
         for (int y = 0; y < c; ++y) rest &= rest - 1;
-        const int w = __ffs(rest) - 1, cut = run_at(w) / p.boxes, from = cut * p.boxes, to = from + p.boxes;
+        const int w = __ffs(rest) - 1, cut = tile_of(run_at(w)), from = cut * p.boxes, to = from + p.boxes;
         const int r = (x - c * elements) & ((1 << rows_log) - 1), m = (x - c * elements) >> rows_log;
         float v = 0.0f, up = 0.0f;
 #pragma unroll 1
@@ -525,17 +527,18 @@ int l4_stages(int M, int K, int G, bool direct) {
 template <int T, int P, bool EXACT>
 cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream) {
     static SmemAttribute attribute[2];
-    const int sms = device_sms();
-    if constexpr (T <= 2) {
-        if (l4_smem<T>(p.M, p.K, p.G, 2, false) > kHalfSm) {
-            p.stages = l4_stages<T>(p.M, p.K, p.G, true);
-            const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, true);
-            return launch_l4(&attribute[1], gemv_packed_ctas(p.tiles, sms, smem <= kHalfSm), smem, stream, linear4_kernel<T, P, EXACT, true>, map, p);
-        }
-    }
-    p.stages = l4_stages<T>(p.M, p.K, p.G, false);
-    const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, false);
-    return launch_l4(&attribute[0], gemv_packed_ctas(p.tiles, sms, smem <= kHalfSm), smem, stream, linear4_kernel<T, P, EXACT, false>, map, p);
+    const bool direct = T <= 2 && l4_smem<T>(p.M, p.K, p.G, 2, false) > kHalfSm;
+    p.stages = l4_stages<T>(p.M, p.K, p.G, direct);
+    const int ctas = gemv_packed_ctas(p.tiles, device_sms(), l4_smem<T>(p.M, p.K, p.G, p.stages, direct) <= kHalfSm);
+    p.cta_tiles = p.tiles / ctas;
+    p.longer = p.tiles - p.cta_tiles * ctas;
+    p.box_magic = p.boxes == 1 ? 0u : static_cast<unsigned>(((1ull << 32) + p.boxes - 1) / p.boxes);
+    const int longest = ((p.cta_tiles + (p.longer ? 1 : 0)) * p.boxes + kL4Warps - 1) / kL4Warps;
+    if (longest < p.stages) p.stages = longest;  // (what an SM has left is room for the launch behind this one to start in)
+    const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, direct);
+    if constexpr (T <= 2)
+        if (direct) return launch_l4(&attribute[1], ctas, smem, stream, linear4_kernel<T, P, EXACT, true>, map, p);
+    return launch_l4(&attribute[0], ctas, smem, stream, linear4_kernel<T, P, EXACT, false>, map, p);
 }
 template <int T, bool EXACT>
 cudaError_t launch_rows4(const L4Params& p, const CUtensorMap& map, int P, cudaStream_t stream) {
@@ -559,7 +562,9 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
     int rows = 32;
     while (rows > 1 && l4_stages(rows, K, G, rows <= 16) == 0) rows /= 2;
     const bool fast = K % 32 == 0 && g % 32 == 0 && ((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(Xq)) & 15u) == 0 &&
-                      l4_stages(rows, K, G, rows <= 16) > 0;
+                      l4_stages(rows, K, G, rows <= 16) > 0 &&
+                      // the kernel's 32-bit arithmetic
+                      (static_cast<unsigned long long>((N + 15) / 16) / device_sms() + 2) * ((K + kBoxK - 1) / kBoxK) * ((K + kBoxK - 1) / kBoxK) < (1ull << 28);
     CUtensorMap map;
     if (fast)
         if (int rc = make_tensor_map_2d_u8(&map, W, K / 2, N, K / 2, kBoxBytes, kBoxRows, 1)) return rc;
@@ -567,7 +572,7 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
         const int m = fast ? (M - m0 < rows ? M - m0 : rows) : M;
         L4Params p = {static_cast<const uint8_t*>(W), w_scale, Xq + static_cast<size_t>(m0) * K, Xs + static_cast<size_t>(m0) * G,
                       Y + static_cast<size_t>(m0) * columns, residual ? residual + static_cast<size_t>(m0) * N : nullptr, m, N, K, g, G, epilogue,
-                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), status};
+                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), 0, 0, 0, status};
         cudaError_t e;
         if (fast) {
             if (exact)
