@@ -339,8 +339,9 @@ W8A8_API size_t w8a8_kv4_cache_bytes(int n_blocks, int n_layers, int n_kv_heads,
 /* w8a8_qknorm_rope_kvwrite for this cache, tokens named by slots (w8a8_plan_blocks): a prompt's rows as well as a decode step's. qkv
  * fp16 [tokens, (n_q + 2 n_kv) * head_dim]; q_norm_w and k_norm_w both or neither; freqs and positions both or neither (no
  * rotation). q_out fp16 [tokens, n_q, head_dim] or NULL; the fp16 q, k and v are bit-identical to that call's, k and v are then held
- * in 4 bits. A token whose slot is negative or outside the cache (n_blocks * 16 slots) is left out, its row of q_out too. Two tokens of one call must
- * not have the same slot. */
+ * in 4 bits. A token whose slot is negative or outside the cache (n_blocks * 16 slots) is left out, its row of q_out too. Two tokens of
+ * one call must not have the same slot, and q_out must not overlap qkv. qkv, the norm weights and q_out are 16-byte aligned. Fewer than
+ * 2^31 pages (blocks * n_layers * n_kv). */
 W8A8_API int w8a8_kv4_write(w8a8_ctx* ctx, const void* qkv, const void* q_norm_w, const void* k_norm_w, float eps,
                    const float* freqs, const int* positions, const int64_t* slots, void* cache, int n_blocks, int layer,
                    int n_layers, int tokens, int n_q_heads, int n_kv_heads, int head_dim, int group_size, void* q_out,
@@ -365,9 +366,12 @@ W8A8_API int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void*
 /* w8a8_linear_q over 4-bit weights: W4 uint8 [N, K / 2], row-major, two codes a byte as two's complement, the even k in the low four
  * bits; w_scale fp16 [N, G] (4-bit groups along K); Xq, Xs as there. Per group an exact int32 sum, promoted with both scales in
  * fp32. epilogue W8A8_EPI_*, residual fp16 [M, N] with W8A8_EPI_RESIDUAL only (may alias Y); for W8A8_EPI_SWIGLU the rows are interleaved
- * by w8a8_pack_gate_up, called with K / 2 in place of K. K and the group size are even. Built for a few rows: the weights are streamed
- * once per 32 rows; longer prompts run w8a8_linear_q over what w8a8_unpack_weight4 makes, with the same scales. The fast kernel takes
- * K and group sizes that are multiples of 32 with W4 and Xq 16-byte aligned, everything else a generic one. */
+ * by w8a8_pack_gate_up, called with K / 2 in place of K. K and the group size are even. The fast kernel takes K and group sizes that are
+ * multiples of 32 with W4 and Xq 16-byte aligned (a group of more than 256 channels, or of an odd multiple of 32, 64 or 128, is promoted in
+ * parts), everything else a generic one. Built for a few rows: the weights are streamed once for as many rows as shared memory has room
+ * for, 32 where K is not very large; longer prompts run w8a8_linear_q over what w8a8_unpack_weight4 makes, with the same scales. W4
+ * and w_scale are parameters: they may be read before the launches ahead on the stream have finished, so a loader waits for
+ * w8a8_quantize_weight4 and w8a8_pack_gate_up (a synchronised stream, an event) before the first call. */
 W8A8_API int w8a8_linear4_q(w8a8_ctx* ctx, const void* W4, const void* w_scale, int group_size, const void* Xq, const void* Xs,
                    void* Y, int M, int N, int K, int epilogue, const void* residual, void* stream);
 /* Loader side: fp16 weights [N, K] to W4 and w_scale; and W4 to int8 codes [N, K], which with the same scales are a weight of

@@ -656,3 +656,132 @@ def test_requests_come_and_go(ctx, captured):
         assert (np.abs(got - want).max(-1) <= np.maximum(tol, 2.0**-24)).all()
         wy, mag = q4.linear(codes, scale, g, xq.cpu().numpy(), xs.cpu().numpy())
         assert (np.abs(y.cpu().numpy() - wy) <= (K // g + 20) * 2.0**-24 * mag + 2.0**-11 * (np.abs(wy) + 1e-3) + 2.0**-24).all()
+
+
+# ---- calls that meet -----------------------------------------------------------------------------------------------
+
+
+def test_two_contexts_on_two_streams(pkg):
+    """A context of its own per stream: a run of calls on either, both on their way at once, gives what it gives alone."""
+    rng = np.random.default_rng(30)
+    n_q, n_kv, group, g = 8, 2, 32, 64
+    contexts, streams = [pkg.Context(0, 0) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    jobs = []
+    for lens in ([9000, 1, 700], [300] * 40):
+        q, pages, table, n = attention_case(rng, lens, n_q, n_kv, group, 1, max(lens) // 16 + 1)
+        B, K, N = len(lens), n_q * D, 320
+        codes, scale, _, _ = linear_case(rng, 1, N, K, g)
+        jobs.append(dict(q=dev(q), pages=dev(pages), blocks=len(pages), table=dev(table), lens=dev(n), B=B, K=K, N=N, W=dev(q4.pack_codes(codes)),
+                         ws=dev(scale), xq=torch.empty((B, K), dtype=torch.int8, device="cuda"), xs=torch.empty((B, K // g), device="cuda"),
+                         y=torch.empty((B, N), dtype=torch.float16, device="cuda"), zero=i32(B, fill=0), slots=torch.empty(9000, dtype=torch.int64, device="cuda"),
+                         positions=i32(9000), plan_lens=i32(B), first=i32(B + 1), info=i32(4), count=i32(1, fill=0), free=i32(1)))
+
+    def run(ctx, j, stream):
+        ctx.kv4_attention_decode(j["q"], j["pages"], j["blocks"], j["table"], j["lens"], None, j["B"], n_q, D, j["table"].shape[1], 0.1, 0, 1, n_kv, group,
+                                 quant_group_size=g, Xq=j["xq"], Xs=j["xs"], stream=stream)
+        ctx.linear4_q(j["W"], j["ws"], g, j["xq"], j["xs"], j["y"], j["B"], j["N"], j["K"], stream=stream)
+        ctx.plan_blocks(j["lens"], j["zero"], j["B"], j["table"], j["table"].shape[1], j["free"], 1, j["count"], j["slots"], j["positions"], j["plan_lens"],
+                        j["first"], 9000, j["info"], stream=stream)
+
+    alone = []
+    for ctx, j in zip(contexts, jobs):
+        run(ctx, j, None)
+        torch.cuda.synchronize()
+        alone.append(j["y"].clone())
+        j["y"].fill_(7)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for ctx, j, s in zip(contexts, jobs, streams):
+            run(ctx, j, s.cuda_stream)
+    torch.cuda.synchronize()
+    for ctx, j, want in zip(contexts, jobs, alone):
+        ctx.check_device_status()
+        assert torch.equal(j["y"], want) and torch.equal(j["plan_lens"], j["lens"]) and j["info"].tolist() == [0, 0, 0, 0]
+        ctx.close()
+
+
+def test_replays_and_eager_calls_in_turn(ctx):
+    """Two graphs and eager calls of other sizes take turns on one stream: they share the context's scratch and tickets."""
+    rng = np.random.default_rng(31)
+    cases = [attention_case(rng, lens, 8, 2, 64, 1, max(lens) // 16 + 1) for lens in ([20000], [3000, 5, 8000], [40] * 30)]
+    side, calls = torch.cuda.Stream(), []
+    for q, pages, table, lens in cases:
+        d = [dev(x) for x in (q, pages, table, lens)] + [torch.empty(q.shape, dtype=torch.float16, device="cuda")]
+
+        def call(d=d, stream=None):
+            ctx.kv4_attention_decode(d[0], d[1], d[1].shape[0], d[2], d[3], d[4], d[0].shape[0], 8, D, d[2].shape[1], 0.1, 0, 1, 2, 64, stream=stream)
+
+        calls.append((call, d[4]))
+    want = []
+    with torch.cuda.stream(side):
+        for call, out in calls:
+            call()
+            want.append(out.clone())
+        side.synchronize()
+        graphs = []
+        for call, _ in calls[:2]:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                call()
+        for _ in range(5):
+            for which in (0, 2, 1, 0, 1):
+                calls[which][1].fill_(7)
+                graphs[which].replay() if which < 2 else calls[2][0]()
+            for (_, out), w in zip(calls, want):
+                assert torch.equal(out, w)
+    ctx.check_device_status()
+
+
+def test_kv4_write_of_a_long_prompt_is_that_of_its_parts(ctx):
+    """However many pairs of heads a warp takes: 20000 rows at once and in calls of 7 and up give the same cache and the same q."""
+    rng = np.random.default_rng(32)
+    T, n_q, n_kv, group = 20000, 5, 3, 64
+    blocks = (T + 15) // 16
+    qkv = torch.from_numpy(rng.standard_normal((T, n_q + 2 * n_kv, D)).astype(np.float16)).cuda()
+    w = [dev(rng.uniform(0.5, 1.5, D).astype(np.float16)) for _ in range(2)]
+    freqs = dev((10000.0 ** (-np.arange(64) / 64)).astype(np.float32))
+    positions, slots = torch.arange(T, dtype=torch.int32, device="cuda"), torch.from_numpy(rng.permutation(blocks * 16)[:T]).cuda()
+    got = []
+    for cuts in ([0, T], [0, 7, 20, 1000, 1001, 9000, T]):
+        cache = torch.zeros(blocks * n_kv * q4.page_bytes(group), dtype=torch.uint8, device="cuda")
+        q = torch.zeros((T, n_q, D), dtype=torch.float16, device="cuda")
+        for a, b in zip(cuts, cuts[1:]):
+            ctx.kv4_write(qkv[a:b], slots[a:b], cache, blocks, 0, 1, b - a, n_q, n_kv, D, group, q_norm_w=w[0], k_norm_w=w[1], eps=1e-6, freqs=freqs,
+                          positions=positions[a:b], q_out=q[a:b])
+        torch.cuda.synchronize()
+        got.append((cache, q))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_plan_blocks_long_prompts(ctx):
+    """More tokens than one CTA writes, into requests that take blocks which others give back in the same call."""
+    cached, new = [160, 0, 48000, 7], [-1, 70001, -3, 9990]
+    blocks = (70001 + 15) // 16 + 1
+    table = np.full((4, blocks), -1, np.int64)
+    perm = np.random.default_rng(33).permutation(6000)
+    table[0, :10], table[2, :3000], table[3, 0] = perm[:10], perm[10:3010], perm[3010]
+    free = np.concatenate([perm[3011:6000], np.full(3011, -5)])
+    case = (cached, new, table.tolist(), free.tolist(), 2989)
+    want = q4.plan(*case, max_tokens=80000, capacity=6000)
+    assert want["info"][0] == 0
+    for in_place in (False, True):
+        assert run_plan(ctx, *case, 80000, in_place=in_place) == want
+
+
+def test_linear4_many_rows_add_to_their_own_output(ctx):
+    """More rows than a launch takes, the residual being the output itself; weight scales off the boundary that the wide reads want."""
+    rng = np.random.default_rng(34)
+    for M, N, K, g in ((70, 48, 512, 32), (45, 33, 1024, 64), (5, 64, 1024, 64)):
+        codes, scale, Xq, Xs = linear_case(rng, M, N, K, g)
+        y, mag = q4.linear(codes, scale, g, Xq, Xs)
+        room = torch.empty(scale.size + 1, dtype=torch.float16, device="cuda")
+        room[1:].copy_(dev(scale).flatten())
+        start = rng.standard_normal((M, N)).astype(np.float16)
+        out = dev(start)
+        ctx.linear4_q(dev(q4.pack_codes(codes)), room[1:], g, dev(Xq), dev(Xs), out, M, N, K, epilogue=1, residual=out)
+        torch.cuda.synchronize()
+        err = (K // g + 19) * 2.0**-24 * mag  # as in check_linear
+        tol = err + 2.0**-11 * (np.abs(y) + err)
+        want = y + start
+        tol = tol + 2.0**-11 * (np.abs(want) + tol)
+        assert (np.abs(out.cpu().numpy() - want) <= tol + 2.0**-24).all()
