@@ -54,36 +54,8 @@ __device__ __forceinline__ void store_row(__half* dst, int l, const Row& r) {
     *reinterpret_cast<uint4*>(dst + 8 * l) = v;
 }
 
-// Two fp32 numbers in one register pair: the packed arithmetic rounds each as the plain one does.
-struct F2 {
-    unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 parts(F2 x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
-    return r;
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ F2 operator-(F2 a) { return {a.v ^ 0x8000000080000000ull}; }
+using q4::F2;
+using q4::f2;
 // The lane's channels as x (even) and y (odd) of the rotation's pairs 0, 1 and 2, 3.
 struct Wide {
     F2 x[2], y[2];

@@ -27,6 +27,9 @@
 namespace w8a8 {
 namespace {
 
+using q4::F2;
+using q4::f2;
+
 constexpr int kL4Warps = 8;
 constexpr int kL4MaxSmem = 224 * 1024;
 constexpr int kBoxRows = 16, kBoxBytes = 128, kBox = kBoxRows * kBoxBytes, kBoxK = 2 * kBoxBytes;
@@ -90,6 +93,13 @@ __device__ __forceinline__ __half l4_plain(float v, const __half* residual, size
     return residual ? __float2half_rn(__half2float(h) + __half2float(residual[at])) : h;
 }
 
+// The wait for a box that is not there yet. (One copy of this code.)
+__device__ __noinline__ bool l4_wait_long(uint64_t* bar, uint32_t phase, int* status) {
+    if (__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar, phase))) return false;
+    atomicExch(status, 950);
+    return true;  // (the numbers are void from here on; the barriers still run their course)
+}
+
 // T token tiles of 8; P promotes per box (256 / P channels each, all in one group); EXACT: groups of 256 / P channels, K in whole boxes and
 // the scales of a box in one aligned read.
 // Shared memory: rings [warps][stages][box]; pieces fp32 [warps][2][16][8 T + 1]; activation scales fp32 [G][8 T]; their codes
@@ -113,7 +123,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kBox);
     float* const xs_s = piece_s + 2 * kL4Warps * kPiece;
     unsigned char* const codes_s = reinterpret_cast<unsigned char*>(xs_s + p.G * 8 * T);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
     const int row8 = (g8 & 1) << 2 | (g8 & 2) | g8 >> 2;  // the row of the tile that this lane's fragment row is (and + 8)
     // tiles [t0, t0 + nt) of this CTA, units [u0, u0 + n_mine) of this warp: the boxes of the CTA's tiles, one tile after the other
     const int cta = blockIdx.x, t0 = cta * p.cta_tiles + min(cta, p.longer), nt = p.cta_tiles + (cta < p.longer ? 1 : 0);
@@ -219,7 +229,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     }
     for (int x = tid; x < p.G * 8 * T; x += kL4Warps * 32) {
         const int group = x / (8 * T), m = x % (8 * T);
-        xs_s[x] = m < p.M ? ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
+        xs_s[x] = m < p.M ? 0.0625f * ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
     }
     if constexpr (!DIRECT) {
         if (!ptx::mbar_wait_bounded(&codes_bar, 0)) {
@@ -236,11 +246,9 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     __syncthreads();
 
     // ---- the run ----
-    float acc[T][4];
+    F2 sums[T][2];  // of rows row8, row8 + 8: tokens 8 t + 2 j4, + 1
 #pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
+    for (int t = 0; t < T; ++t) sums[t][0] = sums[t][1] = f2(0.0f, 0.0f);
     auto emit = [&](int at_tile, int r, int m, float v, float up) {  // rows r and (SwiGLU only) r + 8 of a tile, token m
         if (p.epilogue == W8A8_EPI_SWIGLU) {
             p.Y[static_cast<size_t>(m) * (p.N / 2) + at_tile * 8 + r] = l4_swiglu(v, up);
@@ -257,151 +265,161 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     const uint32_t xs_at = ptx::smem_u32(xs_s) + 2 * j4 * 4;
     int stage = 0;
     uint32_t phase = 0;
+    int left = n_mine;  // boxes of the run that are not done
 #pragma unroll 1
-    for (int i = 0; i < n_mine; ++i) {
-        __half2 ws[P > 1 ? P : 1];
+    while (left > 0) {
+        const int end = min(p.boxes, box + left);  // the run's boxes of this tile
+        const bool tile_ends = end == p.boxes;
+#pragma unroll 1
+        for (; box < end; ++box, --left) {
+            __half2 ws[P > 1 ? P : 1];
 #pragma unroll
-        for (int x = 0; x < (P > 1 ? P : 1); ++x) ws[x] = ws_next[x];
-        const bool tile_ends = box + 1 == p.boxes;
-        if (i + 1 < n_mine) {
-            if (tile_ends) scale_rows(tile + 1);
-            load_scales(tile_ends ? 0 : box + 1);
-        }
-        if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&full_bar[warp][stage], phase)) && !failed &&
-            !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&full_bar[warp][stage], phase))) {
-            atomicExch(p.status, 950);
-            failed = true;  // (the numbers are void from here on; the barriers still run their course)
-        }
-        const uint32_t at = ring + stage * kBox + row_off;
-        int sum[T][4];
-        uint4 wide[2];
-        uint4 x_now[DIRECT ? T : 1][4];
-        if constexpr (DIRECT) {
+            for (int x = 0; x < (P > 1 ? P : 1); ++x) ws[x] = ws_next[x];
+            if (box + 1 == end && left > 1) scale_rows(tile + 1);
+            const int next_box = box + 1 < end ? box + 1 : left > 1 ? 0 : box;
+            load_scales(next_box);
+            if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&full_bar[warp][stage], phase)) && !failed) failed = l4_wait_long(&full_bar[warp][stage], phase, p.status);
+            const uint32_t at = ring + stage * kBox + row_off;
+            int sum[T][4];
+            uint4 wide[2];
+            uint4 x_now[DIRECT ? T : 1][4];
+            if constexpr (DIRECT) {
 #pragma unroll
-            for (int t = 0; t < T; ++t)
+                for (int t = 0; t < T; ++t)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) x_now[t][q] = x_next[t][q];
-            if (i + 1 < n_mine) load_codes(tile_ends ? 0 : box + 1);
-        }
+                    for (int q = 0; q < 4; ++q) x_now[t][q] = x_next[t][q];
+                load_codes(next_box);
+            }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint32_t w[2][2];  // [row half][word]
+            for (int q = 0; q < 4; ++q) {
+                uint32_t w[2][2];  // [row half][word]
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t r = at + half * 8 * kBoxBytes;
-                if constexpr (P <= 2) {
-                    if (!(q & 1)) wide[half] = lds128(r + (((2 * q + j4) ^ row8) << 4));
-                    w[half][0] = q & 1 ? wide[half].z : wide[half].x;
-                    w[half][1] = q & 1 ? wide[half].w : wide[half].y;
-                } else if constexpr (P == 4) {
-                    const uint2 v = lds64(r + (((2 * q + (j4 >> 1)) ^ row8) << 4) + (j4 & 1) * 8);
-                    w[half][0] = v.x;
-                    w[half][1] = v.y;
-                } else {
-                    w[half][0] = lds32(r + (((2 * q) ^ row8) << 4) + j4 * 4);
-                    w[half][1] = lds32(r + (((2 * q + 1) ^ row8) << 4) + j4 * 4);
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t r = at + half * 8 * kBoxBytes;
+                    if constexpr (P <= 2) {
+                        if (!(q & 1)) wide[half] = lds128(r + (((2 * q + j4) ^ row8) << 4));
+                        w[half][0] = q & 1 ? wide[half].z : wide[half].x;
+                        w[half][1] = q & 1 ? wide[half].w : wide[half].y;
+                    } else if constexpr (P == 4) {
+                        const uint2 v = lds64(r + (((2 * q + (j4 >> 1)) ^ row8) << 4) + (j4 & 1) * 8);
+                        w[half][0] = v.x;
+                        w[half][1] = v.y;
+                    } else {
+                        w[half][0] = lds32(r + (((2 * q) ^ row8) << 4) + j4 * 4);
+                        w[half][1] = lds32(r + (((2 * q + 1) ^ row8) << 4) + j4 * 4);
+                    }
                 }
-            }
-            uint32_t a[2][4];
+                uint32_t a[2][4];
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                a[v][0] = (w[0][v] << 4) & 0xf0f0f0f0u;
-                a[v][1] = (w[1][v] << 4) & 0xf0f0f0f0u;
-                a[v][2] = w[0][v] & 0xf0f0f0f0u;
-                a[v][3] = w[1][v] & 0xf0f0f0f0u;
-            }
-            uint4 x[T];
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const uint32_t from = codes[t] + box * kBoxK + q * 64;
-                if constexpr (DIRECT) {
-                    x[t] = evens_first(x_now[t][q]);
-                } else if constexpr (P <= 2) {
-                    x[t] = lds128(from - (q & 1) * 48);  // quarters 0, 1: the first and second 16 of the lane's 32 channels
-                } else if constexpr (P == 4) {
-                    x[t] = lds128(from);
-                } else {
-                    const uint2 a = lds64(from), b = lds64(from + 32);
-                    x[t] = {a.x, a.y, b.x, b.y};
+                for (int v = 0; v < 2; ++v) {
+                    a[v][0] = (w[0][v] << 4) & 0xf0f0f0f0u;
+                    a[v][1] = (w[1][v] << 4) & 0xf0f0f0f0u;
+                    a[v][2] = w[0][v] & 0xf0f0f0f0u;
+                    a[v][3] = w[1][v] & 0xf0f0f0f0u;
                 }
-            }
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const bool first = P == 8 || (v == 0 && (P == 4 || (P == 2 && !(q & 1)) || (P == 1 && q == 0)));
+                uint4 x[T];
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
-                    const uint32_t b0 = v ? x[t].z : x[t].x, b1 = v ? x[t].w : x[t].y;
-                    if (first)
-                        mma_s8_first(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], b0, b1);
-                    else
-                        mma_s8(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], b0, b1);
-                }
-                if (P == 8 || (v == 1 && (P == 4 || (P == 2 && (q & 1)) || q == 3))) {  // promote
-                    const int pr = P == 8 ? 2 * q + v : P == 4 ? q : P == 2 ? q >> 1 : 0;
-                    float ws0, ws1;
-                    if constexpr (EXACT && P > 1) {
-                        ws0 = pr & 1 ? __high2float(ws[pr / 2]) : __low2float(ws[pr / 2]);
-                        ws1 = pr & 1 ? __high2float(ws[P / 2 + pr / 2]) : __low2float(ws[P / 2 + pr / 2]);
+                    const uint32_t from = codes[t] + box * kBoxK + q * 64;
+                    if constexpr (DIRECT) {
+                        x[t] = evens_first(x_now[t][q]);
+                    } else if constexpr (P <= 2) {
+                        x[t] = lds128(from - (q & 1) * 48);  // quarters 0, 1: the first and second 16 of the lane's 32 channels
+                    } else if constexpr (P == 4) {
+                        x[t] = lds128(from);
                     } else {
-                        ws0 = __low2float(ws[pr]);
-                        ws1 = __high2float(ws[pr]);
+                        const uint2 a = lds64(from), b = lds64(from + 32);
+                        x[t] = {a.x, a.y, b.x, b.y};
                     }
-                    ws0 *= 0.0625f;
-                    ws1 *= 0.0625f;
-                    const uint32_t xg = xs_at + group_of(box, pr) * (8 * T * 4);
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const bool first = P == 8 || (v == 0 && (P == 4 || (P == 2 && !(q & 1)) || (P == 1 && q == 0)));
 #pragma unroll
                     for (int t = 0; t < T; ++t) {
-                        const uint2 xx = lds64(xg + t * 32);
-                        const float x0 = __uint_as_float(xx.x), x1 = __uint_as_float(xx.y);
-                        acc[t][0] = fmaf(static_cast<float>(sum[t][0]) * ws0, x0, acc[t][0]);
-                        acc[t][1] = fmaf(static_cast<float>(sum[t][1]) * ws0, x1, acc[t][1]);
-                        acc[t][2] = fmaf(static_cast<float>(sum[t][2]) * ws1, x0, acc[t][2]);
-                        acc[t][3] = fmaf(static_cast<float>(sum[t][3]) * ws1, x1, acc[t][3]);
+                        const uint32_t b0 = v ? x[t].z : x[t].x, b1 = v ? x[t].w : x[t].y;
+                        if (first)
+                            mma_s8_first(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], b0, b1);
+                        else
+                            mma_s8(sum[t], a[v][0], a[v][1], a[v][2], a[v][3], b0, b1);
+                    }
+                    if (P == 8 || (v == 1 && (P == 4 || (P == 2 && (q & 1)) || q == 3))) {  // promote
+                        const int pr = P == 8 ? 2 * q + v : P == 4 ? q : P == 2 ? q >> 1 : 0;
+                        float ws0, ws1;
+                        if constexpr (EXACT && P > 1) {
+                            ws0 = pr & 1 ? __high2float(ws[pr / 2]) : __low2float(ws[pr / 2]);
+                            ws1 = pr & 1 ? __high2float(ws[P / 2 + pr / 2]) : __low2float(ws[P / 2 + pr / 2]);
+                        } else {
+                            ws0 = __low2float(ws[pr]);
+                            ws1 = __high2float(ws[pr]);
+                        }
+                        const uint32_t xg = xs_at + group_of(box, pr) * (8 * T * 4);
+#pragma unroll
+                        for (int t = 0; t < T; ++t) {
+                            const uint2 xx = lds64(xg + t * 32);
+                            const F2 x01 = f2(__uint_as_float(xx.x), __uint_as_float(xx.y));
+                            sums[t][0] = fma2(f2(static_cast<float>(sum[t][0]), static_cast<float>(sum[t][1])) * f2(ws0, ws0), x01, sums[t][0]);
+                            sums[t][1] = fma2(f2(static_cast<float>(sum[t][2]), static_cast<float>(sum[t][3])) * f2(ws1, ws1), x01, sums[t][1]);
+                        }
                     }
                 }
             }
-        }
-        // ---- the stage is free ----
-        if (i + p.stages < n_mine) {
-            ptx::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0 && !failed) issue(stage);
-        }
-        if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1;
-        }
-        if (tile_ends || i + 1 == n_mine) {
-            if (tile_ends && !head) {  // all of the tile
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int m = 8 * t + 2 * j4 + e;
-                        if (m < p.M) {
-                            emit(tile, row8, m, acc[t][e], acc[t][2 + e]);
-                            if (p.epilogue != W8A8_EPI_SWIGLU) emit(tile, row8 + 8, m, acc[t][2 + e], 0.0f);
-                        }
-                    }
-            } else {
-                float* const piece = piece_s + (2 * warp + (head ? 0 : 1)) * kPiece;
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) piece[(row8 + 4 * (e & 2)) * kCols + 8 * t + 2 * j4 + (e & 1)] = acc[t][e];
+            // ---- the stage is free ----
+            if (left > p.stages) {
+                ptx::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0 && !failed) issue(stage);
             }
-            head = false;
+            if (++stage == p.stages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        float acc[T][4];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const float2 a = parts(sums[t][0]), c = parts(sums[t][1]);
+            acc[t][0] = a.x; acc[t][1] = a.y; acc[t][2] = c.x; acc[t][3] = c.y;
+            sums[t][0] = sums[t][1] = f2(0.0f, 0.0f);
+        }
+        if (tile_ends && !head) {  // all of the tile
+            const int columns = p.epilogue == W8A8_EPI_SWIGLU ? p.N / 2 : p.N, n = p.epilogue == W8A8_EPI_SWIGLU ? tile * 8 + row8 : tile * 16 + row8;
+            const size_t first = static_cast<size_t>(2 * j4) * columns + n;
+            __half* y = p.Y + first;
+            auto each = [&](auto put) {  // put(y, t, e) for the lane's tokens
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (8 * t + 2 * j4 + e < p.M) put(static_cast<size_t>(8 * t + e) * columns, t, e);
+            };
+            if (p.epilogue == W8A8_EPI_SWIGLU) {
+                each([&](size_t at, int t, int e) { y[at] = l4_swiglu(acc[t][e], acc[t][2 + e]); });
+            } else {
+                const bool row0 = n < p.N, row1 = n + 8 < p.N;
+                if (p.residual) {
+                    const __half* const r = p.residual + first;
+                    each([&](size_t at, int t, int e) {
+                        if (row0) y[at] = l4_plain(acc[t][e], r, at);
+                        if (row1) y[at + 8] = l4_plain(acc[t][2 + e], r, at + 8);
+                    });
+                } else {
+                    each([&](size_t at, int t, int e) {
+                        if (row0) y[at] = __float2half_rn(acc[t][e]);
+                        if (row1) y[at + 8] = __float2half_rn(acc[t][2 + e]);
+                    });
+                }
+            }
+        } else {
+            float* const piece = piece_s + (2 * warp + (head ? 0 : 1)) * kPiece;
 #pragma unroll
             for (int t = 0; t < T; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) piece[(row8 + 4 * (e & 2)) * kCols + 8 * t + 2 * j4 + (e & 1)] = acc[t][e];
         }
-        if (tile_ends) {
-            ++tile;
-            box = 0;
-        } else {
-            ++box;
-        }
+        head = false;
+        ++tile;
+        box = 0;
     }
     __syncthreads();
 
@@ -412,23 +430,31 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     const bool cuts_before = __shfl_up_sync(0xffffffffu, cuts, 1);
     const int cut_before = __shfl_up_sync(0xffffffffu, cut_at, 1);
     const uint32_t cut_tiles = __ballot_sync(0xffffffffu, cuts && !(lane > 1 && cuts_before && cut_before == cut_at));
-    const int rows_log = swiglu ? 3 : 4, elements = p.M << rows_log;
+    const int n_cuts = __popc(cut_tiles);
+    if (n_cuts > 0) {  // the warps take the cut tiles in turn; a lane has one row of the tile (SwiGLU: and the one 8 below) and every so many tokens
+        int c = warp, share = 0, shares = 0;
+        for (; c >= n_cuts; c -= n_cuts) ++share;
+        for (int x = c; x < kL4Warps; x += n_cuts) ++shares;
+        uint32_t later = cut_tiles;
+        for (int x = 0; x < c; ++x) later &= later - 1;
+        const int w = __ffs(later) - 1, to = (__shfl_sync(0xffffffffu, cut_at, w) + 1) * p.boxes;
+        // its pieces: of warp w - 1, whose run it ends, and of those behind that border that begin inside it
+        const int next_border = __shfl_down_sync(0xffffffffu, border, 1);
+        const uint32_t has = __ballot_sync(0xffffffffu, lane >= w && lane < kL4Warps && border < to && next_border > border);
+        const int cut = __shfl_sync(0xffffffffu, cut_at, w);
+        const int rows_log = swiglu ? 3 : 4, r = lane & ((1 << rows_log) - 1);
 #pragma unroll 1
-    for (int x = tid, c = 0; x < elements * __popc(cut_tiles); x += kL4Warps * 32) {
-        while (x >= (c + 1) * elements) ++c;
-        uint32_t rest = cut_tiles;
-        for (int y = 0; y < c; ++y) rest &= rest - 1;
-        const int w = __ffs(rest) - 1, cut = tile_of(run_at(w)), from = cut * p.boxes, to = from + p.boxes;
-        const int r = (x - c * elements) & ((1 << rows_log) - 1), m = (x - c * elements) >> rows_log;
-        float v = 0.0f, up = 0.0f;
+        for (int m = (share << (5 - rows_log)) + (lane >> rows_log); m < p.M; m += shares << (5 - rows_log)) {
+            const float* piece = piece_s + (2 * w - 1) * kPiece + r * kCols + m;
+            float v = piece[0], up = swiglu ? piece[8 * kCols] : 0.0f;
 #pragma unroll 1
-        for (int w2 = w - 1; w2 < kL4Warps && run_at(w2) < to; ++w2) {
-            if (run_at(w2 + 1) <= from || run_at(w2 + 1) == run_at(w2)) continue;
-            const float* piece = piece_s + (2 * w2 + (run_at(w2) > from ? 0 : 1)) * kPiece;
-            v += piece[r * kCols + m];
-            if (swiglu) up += piece[(r + 8) * kCols + m];
+            for (uint32_t rest = has; rest; rest &= rest - 1) {
+                piece = piece_s + 2 * (__ffs(rest) - 1) * kPiece + r * kCols + m;
+                v += piece[0];
+                if (swiglu) up += piece[8 * kCols];
+            }
+            emit(t0 + cut, r, m, v, up);
         }
-        emit(t0 + cut, r, m, v, up);
     }
     if (failed) {  // copies that may still be on their way land before the CTA goes
 #pragma unroll 1

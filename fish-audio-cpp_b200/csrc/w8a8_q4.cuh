@@ -40,6 +40,38 @@ struct Scale {
     }
 };
 
+// ---- packed arithmetic ----
+// Two fp32 numbers in one register pair: the packed arithmetic rounds each as the plain one does.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts(F2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator-(F2 a) { return {a.v ^ 0x8000000080000000ull}; }
+
 // ---- a page of the cache: 16 tokens of one (layer, kv head), 128 channels ----
 //   [0, 1024)       K codes: token t at 64 t; in it 16 bytes for each quarter j of eight channels of every 32-channel run: the word
 //                   16 j + 4 run holds channels 32 run + 8 j + n as nibbles n = 0 .. 7 (low first)
