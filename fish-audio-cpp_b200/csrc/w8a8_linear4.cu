@@ -49,6 +49,8 @@ struct L4Params {
     int pitch;   // of a row of codes in shared memory
     int cta_tiles, longer;  // tiles of a CTA; the first `longer` CTAs have one more
     unsigned box_magic;     // 2^32 / boxes, rounded up (0: one box): x / boxes is the high word of x box_magic while x boxes < 2^32
+    unsigned chunk_magic;   // the same for K / 16
+    int pad;                // pitch - K
     int* status;
 };
 
@@ -118,7 +120,7 @@ template <int T, int P, bool EXACT, bool DIRECT>
 __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ L4Params p) {
     constexpr int kPiece = l4_piece_floats<T>(), kCols = 8 * T + 1;
     extern __shared__ unsigned char l4_smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kL4Warps][8], codes_bar;
+    __shared__ __align__(8) uint64_t full_bar[kL4Warps][8];
     unsigned char* const base = l4_smem_raw + ((1024u - (ptx::smem_u32(l4_smem_raw) & 1023u)) & 1023u);  // (the swizzle repeats every 1024 bytes)
     float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kBox);
     float* const xs_s = piece_s + 2 * kL4Warps * kPiece;
@@ -150,7 +152,6 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         }
     };
     if (lane < p.stages) ptx::mbar_init(&full_bar[warp][lane], 1);
-    if (tid == 0) ptx::mbar_init(&codes_bar, 1);
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
     __syncwarp();
@@ -194,8 +195,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     ptx::pdl_launch_dependents();  // (at the start it costs 1 % of a step: what is launched then takes room)
 
     // ---- the activations ----
-    // DIRECT: a lane's codes of a box in registers, asked for a box ahead. Else rows as they are in shared memory, each by one bulk copy, then the eight
-    // channels of a word even ones first, in place.
+    // DIRECT: a lane's codes of a box in registers, asked for a box ahead. Else rows in shared memory, the eight channels of a word even ones first.
     uint4 x_next[DIRECT ? T : 1][4];
     auto load_codes = [&](int bx) {
 #pragma unroll
@@ -218,30 +218,32 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         }
     };
     bool failed = false;
+    constexpr int kAhead = 4;
+    uint4 c_next[kAhead];
+    const int chunks = p.M * (p.K / 16);  // of 16 codes; X is [M, K] without gaps
+    auto ask = [&](int x0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (x0 + i * kL4Warps * 32 < chunks) c_next[i] = ptx::ld_result_v4(p.Xq + 16ll * (x0 + i * kL4Warps * 32));
+    };
     if constexpr (DIRECT) {
         if (n_mine > 0) load_codes(box);
-    } else if (tid == 0) {
-        ptx::mbar_arrive_expect_tx(&codes_bar, p.M * p.K);
-        for (int m = 0; m < p.M; ++m)
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ptx::smem_u32(codes_s) + m * p.pitch),
-                         "l"(p.Xq + static_cast<size_t>(m) * p.K), "r"(p.K), "r"(ptx::smem_u32(&codes_bar))
-                         : "memory");
+    } else {
+        ask(tid);
     }
     for (int x = tid; x < p.G * 8 * T; x += kL4Warps * 32) {
         const int group = x / (8 * T), m = x % (8 * T);
         xs_s[x] = m < p.M ? 0.0625f * ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
     }
     if constexpr (!DIRECT) {
-        if (!ptx::mbar_wait_bounded(&codes_bar, 0)) {
-            atomicExch(p.status, 951);
-            failed = true;
-        }
-        failed = __syncthreads_or(failed);
-        for (int m = warp; m < p.M; m += kL4Warps)
-            for (int x = lane * 16; x < p.K; x += 32 * 16) {
-                uint4* at = reinterpret_cast<uint4*>(codes_s + m * p.pitch + x);
-                *at = evens_first(*at);
+#pragma unroll 1
+        for (int x0 = tid; x0 < chunks; ask(x0 += kAhead * kL4Warps * 32)) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int x = x0 + i * kL4Warps * 32;
+                if (x < chunks) *reinterpret_cast<uint4*>(codes_s + 16 * x + __umulhi(x, p.chunk_magic) * p.pad) = evens_first(c_next[i]);
             }
+        }
     }
     __syncthreads();
 
@@ -558,6 +560,8 @@ cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream
     const int ctas = gemv_packed_ctas(p.tiles, device_sms(), l4_smem<T>(p.M, p.K, p.G, p.stages, direct) <= kHalfSm);
     p.cta_tiles = p.tiles / ctas;
     p.longer = p.tiles - p.cta_tiles * ctas;
+    p.chunk_magic = static_cast<unsigned>(((1ull << 32) + p.K / 16 - 1) / (p.K / 16));
+    p.pad = p.pitch - p.K;
     p.box_magic = p.boxes == 1 ? 0u : static_cast<unsigned>(((1ull << 32) + p.boxes - 1) / p.boxes);
     const int longest = ((p.cta_tiles + (p.longer ? 1 : 0)) * p.boxes + kL4Warps - 1) / kL4Warps;
     if (longest < p.stages) p.stages = longest;  // (what an SM has left is room for the launch behind this one to start in)
@@ -598,7 +602,7 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
         const int m = fast ? (M - m0 < rows ? M - m0 : rows) : M;
         L4Params p = {static_cast<const uint8_t*>(W), w_scale, Xq + static_cast<size_t>(m0) * K, Xs + static_cast<size_t>(m0) * G,
                       Y + static_cast<size_t>(m0) * columns, residual ? residual + static_cast<size_t>(m0) * N : nullptr, m, N, K, g, G, epilogue,
-                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), 0, 0, 0, status};
+                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), 0, 0, 0, 0, 0, status};
         cudaError_t e;
         if (fast) {
             if (exact)
