@@ -33,6 +33,8 @@ int device_sms();
 // A launch that fails all the same asks again (`anew`): a device reset takes the attribute back. One object per kernel, static.
 class SmemAttribute {
   public:
+    // widest: the SM's L1 as small as it goes whatever the launch asks for, so that launches of different sizes may share an SM.
+    constexpr explicit SmemAttribute(bool widest = false) : widest_(widest) {}
     cudaError_t operator()(const void* kernel, int bytes, bool anew = false) {
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
@@ -40,11 +42,13 @@ class SmemAttribute {
         const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
         if (!anew && (done_.load(std::memory_order_acquire) & bit)) return cudaSuccess;
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && widest_) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e == cudaSuccess) done_.fetch_or(bit, std::memory_order_release);
         return e;
     }
 
   private:
+    const bool widest_;
     std::atomic<unsigned long long> done_{0};
 };
 // Launches `kern`; `attr` as above.

@@ -103,27 +103,34 @@ __device__ __noinline__ bool l4_wait_long(uint64_t* bar, uint32_t phase, int* st
 }
 
 // T token tiles of 8; P promotes per box (256 / P channels each, all in one group); EXACT: groups of 256 / P channels, K in whole boxes and
-// the scales of a box in one aligned read.
-// Shared memory: rings [warps][stages][box]; pieces fp32 [warps][2][16][8 T + 1]; activation scales fp32 [G][8 T]; their codes
-// [M][pitch], a pitch at which the rows that lanes read together lie in different banks.
+// the scales of a box in one aligned read; DIRECT: the codes that meet a box come through the ring behind it (two boxes of 128 channels), by the
+// warp that uses them.
+// Shared memory: rings [warps][stages][box, codes]; pieces fp32 [warps][16][8 T + 1]; activation scales over 16, fp32 [G][8 T]; not DIRECT: codes
+// [M][pitch], a pitch at which the rows that lanes read together lie in different banks. A run's last piece goes where its ring was.
 // (reads run on to the end of the last box: what lies behind K meets weights of zero)
 inline int l4_pitch(int K, int P) { return (K + 127) / 128 * 128 + (P <= 2 ? 16 : P == 4 ? 64 : 32); }
 template <int T>
 constexpr int l4_piece_floats() { return 16 * (8 * T + 1); }
 template <int T>
+__host__ __device__ constexpr int l4_stage_bytes(bool direct) { return kBox + (direct ? T * kBoxK * 8 : 0); }
+template <int T>
+constexpr int kDirectStages = T == 1 ? 3 : 2;
+template <int T>
 size_t l4_smem(int M, int K, int G, int stages, bool direct) {
-    return 1024 + static_cast<size_t>(kL4Warps) * stages * kBox + 2 * kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(G) * 8 * T * 4 +
+    return 1024 + static_cast<size_t>(kL4Warps) * stages * l4_stage_bytes<T>(direct) + kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(G) * 8 * T * 4 +
            (direct ? 0 : static_cast<size_t>(l4_pitch(K, 4)) * M + kBoxK);
 }
 
 template <int T, int P, bool EXACT, bool DIRECT>
-__global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ L4Params p) {
-    constexpr int kPiece = l4_piece_floats<T>(), kCols = 8 * T + 1;
+__global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap x_map,
+                                                                         const __grid_constant__ L4Params p) {
+    constexpr int kPiece = l4_piece_floats<T>(), kCols = 8 * T + 1, kStage = l4_stage_bytes<T>(DIRECT);
     extern __shared__ unsigned char l4_smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kL4Warps][8];
     unsigned char* const base = l4_smem_raw + ((1024u - (ptx::smem_u32(l4_smem_raw) & 1023u)) & 1023u);  // (the swizzle repeats every 1024 bytes)
-    float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kBox);
-    float* const xs_s = piece_s + 2 * kL4Warps * kPiece;
+    float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kStage);
+    float* const xs_s = piece_s + kL4Warps * kPiece;
+    auto end_piece = [&](int w) { return reinterpret_cast<float*>(base + w * p.stages * kStage); };  // of a finished run, in its ring
     unsigned char* const codes_s = reinterpret_cast<unsigned char*>(xs_s + p.G * 8 * T);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
     const int row8 = (g8 & 1) << 2 | (g8 & 2) | g8 >> 2;  // the row of the tile that this lane's fragment row is (and + 8)
@@ -137,19 +144,23 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     int tile = t0 + first_tile, box = u0 - first_tile * p.boxes;
     bool head = box > 0;  // the tile began in another warp's run
 
-    const uint32_t ring = ptx::smem_u32(base) + warp * p.stages * kBox;
+    const uint32_t ring = ptx::smem_u32(base) + warp * p.stages * kStage;
     int l_tile = tile, l_box = box;
     auto issue = [&](int stage) {  // (one lane)
         uint64_t* bar = &full_bar[warp][stage];
-        ptx::mbar_arrive_expect_tx(bar, kBox);
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(ring + stage * kBox),
-            "l"(&map), "r"(ptx::smem_u32(bar)), "r"(l_box * kBoxBytes), "r"(l_tile * kBoxRows)
-            : "memory");
+        ptx::mbar_arrive_expect_tx(bar, kStage);
+        ptx::tma_load_2d_at(ring + stage * kStage, &map, bar, l_box * kBoxBytes, l_tile * kBoxRows);
         if (++l_box == p.boxes) {
             l_box = 0;
             ++l_tile;
         }
+    };
+    int c_box = box;
+    auto issue_codes = [&](int stage) {  // (DIRECT; one lane) the codes that meet the box: two boxes of 8 T rows x 128 channels
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            ptx::tma_load_2d_at(ring + stage * kStage + kBox + h * 8 * T * 128, &x_map, &full_bar[warp][stage], c_box * kBoxK + h * 128, 0);
+        if (++c_box == p.boxes) c_box = 0;
     };
     if (lane < p.stages) ptx::mbar_init(&full_bar[warp][lane], 1);
     ptx::fence_barrier_init();
@@ -195,28 +206,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     ptx::pdl_launch_dependents();  // (at the start it costs 1 % of a step: what is launched then takes room)
 
     // ---- the activations ----
-    // DIRECT: a lane's codes of a box in registers, asked for a box ahead. Else rows in shared memory, the eight channels of a word even ones first.
-    uint4 x_next[DIRECT ? T : 1][4];
-    auto load_codes = [&](int bx) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const int8_t* row = p.Xq + static_cast<size_t>(min(8 * t + g8, p.M - 1)) * p.K;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint4& x = x_next[DIRECT ? t : 0][q];
-                x = {0u, 0u, 0u, 0u};
-                const int k = bx * kBoxK + (P <= 2 ? (q >> 1) * 128 + j4 * 32 + (q & 1) * 16 : P == 4 ? q * 64 + j4 * 16 : q * 64 + j4 * 8);
-                if constexpr (P <= 4) {
-                    if (EXACT || k < p.K) x = ptx::ld_result_v4(row + k);
-                } else {
-                    uint2 a = {0u, 0u}, b = {0u, 0u};
-                    if (EXACT || k < p.K) a = ptx::ld_result_v2(row + k);
-                    if (EXACT || k + 32 < p.K) b = ptx::ld_result_v2(row + k + 32);
-                    x = {a.x, a.y, b.x, b.y};
-                }
-            }
-        }
-    };
+    // DIRECT: each box's codes come with it. Else all rows to shared memory, the eight channels of a word even ones first.
     bool failed = false;
     constexpr int kAhead = 4;
     uint4 c_next[kAhead];
@@ -227,7 +217,9 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
             if (x0 + i * kL4Warps * 32 < chunks) c_next[i] = ptx::ld_result_v4(p.Xq + 16ll * (x0 + i * kL4Warps * 32));
     };
     if constexpr (DIRECT) {
-        if (n_mine > 0) load_codes(box);
+        ptx::fence_proxy_async();  // (what the launch ahead wrote is read by bulk copies)
+        if (lane == 0)
+            for (int i = 0; i < min(p.stages, n_mine); ++i) issue_codes(i);
     } else {
         ask(tid);
     }
@@ -281,17 +273,9 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
             const int next_box = box + 1 < end ? box + 1 : left > 1 ? 0 : box;
             load_scales(next_box);
             if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&full_bar[warp][stage], phase)) && !failed) failed = l4_wait_long(&full_bar[warp][stage], phase, p.status);
-            const uint32_t at = ring + stage * kBox + row_off;
+            const uint32_t at = ring + stage * kStage + row_off;
             int sum[T][4];
             uint4 wide[2];
-            uint4 x_now[DIRECT ? T : 1][4];
-            if constexpr (DIRECT) {
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) x_now[t][q] = x_next[t][q];
-                load_codes(next_box);
-            }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t w[2][2];  // [row half][word]
@@ -323,8 +307,15 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
                     const uint32_t from = codes[t] + box * kBoxK + q * 64;
-                    if constexpr (DIRECT) {
-                        x[t] = evens_first(x_now[t][q]);
+                    if constexpr (DIRECT) {  // chunks of 16 lie in the 128-byte swizzle
+                        const uint32_t row = ring + stage * kStage + kBox + (8 * t + g8) * 128 + (q >> 1) * 8 * T * 128;
+                        if constexpr (P <= 4) {
+                            x[t] = evens_first(lds128(row + (((P <= 2 ? 2 * j4 + (q & 1) : (q & 1) * 4 + j4) ^ g8) << 4)));
+                        } else {
+                            const uint2 a = lds64(row + ((((q & 1) * 4 + (j4 >> 1)) ^ g8) << 4) + (j4 & 1) * 8);
+                            const uint2 b = lds64(row + ((((q & 1) * 4 + 2 + (j4 >> 1)) ^ g8) << 4) + (j4 & 1) * 8);
+                            x[t] = evens_first({a.x, a.y, b.x, b.y});
+                        }
                     } else if constexpr (P <= 2) {
                         x[t] = lds128(from - (q & 1) * 48);  // quarters 0, 1: the first and second 16 of the lane's 32 channels
                     } else if constexpr (P == 4) {
@@ -370,7 +361,10 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
             if (left > p.stages) {
                 ptx::fence_proxy_async();
                 __syncwarp();
-                if (lane == 0 && !failed) issue(stage);
+                if (lane == 0 && !failed) {
+                    issue(stage);
+                    if constexpr (DIRECT) issue_codes(stage);
+                }
             }
             if (++stage == p.stages) {
                 stage = 0;
@@ -413,7 +407,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
                 }
             }
         } else {
-            float* const piece = piece_s + (2 * warp + (head ? 0 : 1)) * kPiece;
+            float* const piece = head ? piece_s + warp * kPiece : end_piece(warp);
 #pragma unroll
             for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -447,11 +441,11 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         const int rows_log = swiglu ? 3 : 4, r = lane & ((1 << rows_log) - 1);
 #pragma unroll 1
         for (int m = (share << (5 - rows_log)) + (lane >> rows_log); m < p.M; m += shares << (5 - rows_log)) {
-            const float* piece = piece_s + (2 * w - 1) * kPiece + r * kCols + m;
+            const float* piece = end_piece(w - 1) + r * kCols + m;
             float v = piece[0], up = swiglu ? piece[8 * kCols] : 0.0f;
 #pragma unroll 1
             for (uint32_t rest = has; rest; rest &= rest - 1) {
-                piece = piece_s + 2 * (__ffs(rest) - 1) * kPiece + r * kCols + m;
+                piece = piece_s + (__ffs(rest) - 1) * kPiece + r * kCols + m;
                 v += piece[0];
                 if (swiglu) up += piece[8 * kCols];
             }
@@ -536,10 +530,12 @@ cudaError_t launch_l4(SmemAttribute* attribute, int ctas, size_t smem, cudaStrea
     return attribute ? launch_with_smem(*attribute, kL4MaxSmem, cfg, kern, args...) : cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// Stages of a warp's ring: as many as leave room for two CTAs on an SM (more than four are not worth their space), else for one; 0: no room.
-constexpr size_t kHalfSm = 112 * 1024;
+// Stages of a warp's ring: as many as leave room for two CTAs on an SM (more than four are not worth their space), else for one; 0: no room. (At
+// least two: in the end the ring holds a piece of up to 2112 bytes.)
+constexpr size_t kHalfSm = 112 * 1024, kThirdSm = 76 * 1024;
 template <int T>
 int l4_stages(int M, int K, int G, bool direct) {
+    if (direct) return l4_smem<T>(M, K, G, kDirectStages<T>, true) <= kL4MaxSmem ? kDirectStages<T> : 0;
     for (int stages = 4; stages >= 2; --stages)
         if (l4_smem<T>(M, K, G, stages, direct) <= kHalfSm) return stages;
     for (int stages = 8; stages >= 2; --stages)
@@ -550,12 +546,13 @@ int l4_stages(int M, int K, int G, bool direct) {
     return M > 16 ? l4_stages<4>(M, K, G, direct) : M > 8 ? l4_stages<2>(M, K, G, direct) : l4_stages<1>(M, K, G, direct);
 }
 
-// Codes in shared memory, but where they leave no room for two CTAs on an SM (eight rows of 9728 channels on 160 tiles: 10.7 us, from global memory
-// 8.1; where there is room shared memory is as good or better: one row 6.9 and 7.6, sixteen rows of 2560 channels on 1216 tiles 11.8 and 14.0).
+// DIRECT where every CTA has one tile, so that a code is read once either way, and there are rows enough: eight rows of 4096 channels on 160 tiles
+// in a run of launches 3.9 us, through shared memory 4.2; sixteen 4.7 and 5.7; one row 5.0 and 3.5; eight rows of 2560 on 1216 tiles 8.3 and 7.7.
+// And where a CTA's codes leave no room for two CTAs on an SM (eight rows of 9728 channels: 10.7 us with one of them).
 template <int T, int P, bool EXACT>
 cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream) {
-    static SmemAttribute attribute[2];
-    const bool direct = T <= 2 && l4_smem<T>(p.M, p.K, p.G, 2, false) > kHalfSm;
+    static SmemAttribute attribute[2] = {SmemAttribute(true), SmemAttribute(true)};
+    const bool direct = T <= 2 && ((p.M > 4 && p.tiles <= 2 * device_sms()) || l4_smem<T>(p.M, p.K, p.G, 2, false) > kHalfSm);
     p.stages = l4_stages<T>(p.M, p.K, p.G, direct);
     const int ctas = gemv_packed_ctas(p.tiles, device_sms(), l4_smem<T>(p.M, p.K, p.G, p.stages, direct) <= kHalfSm);
     p.cta_tiles = p.tiles / ctas;
@@ -563,12 +560,17 @@ cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream
     p.chunk_magic = static_cast<unsigned>(((1ull << 32) + p.K / 16 - 1) / (p.K / 16));
     p.pad = p.pitch - p.K;
     p.box_magic = p.boxes == 1 ? 0u : static_cast<unsigned>(((1ull << 32) + p.boxes - 1) / p.boxes);
-    const int longest = ((p.cta_tiles + (p.longer ? 1 : 0)) * p.boxes + kL4Warps - 1) / kL4Warps;
-    if (longest < p.stages) p.stages = longest;  // (what an SM has left is room for the launch behind this one to start in)
-    const size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, direct);
+    // Never three CTAs on an SM: what the third takes from the others is more than its early start gives (four projections at one row 22.6 us with
+    // three, 20.1 with two, 30.6 with one).
+    size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, direct);
+    if (smem < kThirdSm) smem = kThirdSm;
     if constexpr (T <= 2)
-        if (direct) return launch_l4(&attribute[1], ctas, smem, stream, linear4_kernel<T, P, EXACT, true>, map, p);
-    return launch_l4(&attribute[0], ctas, smem, stream, linear4_kernel<T, P, EXACT, false>, map, p);
+        if (direct) {
+            CUtensorMap x_map;
+            if (make_tensor_map_2d_u8(&x_map, p.Xq, p.K, p.M, p.K, 128, 8 * T, 1)) return cudaErrorInvalidValue;
+            return launch_l4(&attribute[1], ctas, smem, stream, linear4_kernel<T, P, EXACT, true>, map, x_map, p);
+        }
+    return launch_l4(&attribute[0], ctas, smem, stream, linear4_kernel<T, P, EXACT, false>, map, map, p);
 }
 template <int T, bool EXACT>
 cudaError_t launch_rows4(const L4Params& p, const CUtensorMap& map, int P, cudaStream_t stream) {

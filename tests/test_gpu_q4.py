@@ -515,6 +515,12 @@ def test_linear4_shapes_of_the_generic_kernel(ctx, M, N, K, g, offset):
     check_linear(ctx, np.random.default_rng(M + N), M, N, K, min(g, K), 0, offset)
 
 
+@pytest.mark.parametrize("M,N,K,g", [(16, 16, 65536, 32), (33, 16, 32768, 32), (9, 40, 65536, 64), (5, 16, 131072, 128), (32, 33, 16384, 256), (7, 4800, 32, 32)])
+def test_linear4_long_rows(ctx, M, N, K, g):
+    """Scales and codes that fill shared memory, so that fewer rows go into a launch."""
+    check_linear(ctx, np.random.default_rng(K), M, N, K, g, 0)
+
+
 def test_linear4_sums_are_exact(ctx):
     """Scales of one and the largest codes: whole numbers that fp16 holds come out as they are, and a long group's sum stays exact."""
     rng = np.random.default_rng(5)
