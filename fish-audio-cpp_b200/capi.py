@@ -107,6 +107,7 @@ def load_library() -> C.CDLL:
         "w8a8_kv4_read": (I, [P, P, I, P, I, I, I, I, I, I, P, P, P]),
         "w8a8_kv4_attention_workspace_bytes": (Z, [I, I]),
         "w8a8_kv4_attention_decode": (I, [P, P, P, I, P, P, P, I, I, I, I, F, I, I, I, I, I, P, P, P]),
+        "w8a8_kv4_attention_decode_ahead": (I, [P, P, P, I, P, P, P, I, I, I, I, F, I, I, I, I, I, P, P, P]),
         "w8a8_linear4_q": (I, [P, P, P, I, P, P, P, I, I, I, I, P, P]),
         "w8a8_quantize_weight4": (I, [P, P, I, I, I, P, P, P]),
         "w8a8_unpack_weight4": (I, [P, P, I, I, P, P]),
@@ -143,7 +144,7 @@ EXPORTS = [
     "w8a8_decode_stack_timeline",
     "w8a8_pack_gate_up", "w8a8_qknorm_rope_kvwrite", "w8a8_paged_attention_decode", "w8a8_qkv_attention_decode",
     "w8a8_qkv_attention_decode_ahead", "w8a8_plan_blocks", "w8a8_kv4_cache_bytes", "w8a8_kv4_write", "w8a8_kv4_read",
-    "w8a8_kv4_attention_workspace_bytes", "w8a8_kv4_attention_decode", "w8a8_linear4_q", "w8a8_quantize_weight4", "w8a8_unpack_weight4",
+    "w8a8_kv4_attention_workspace_bytes", "w8a8_kv4_attention_decode", "w8a8_kv4_attention_decode_ahead", "w8a8_linear4_q", "w8a8_quantize_weight4", "w8a8_unpack_weight4",
     "w8a8_tp_create", "w8a8_tp_connect",
     "w8a8_tp_linear_q", "w8a8_tp_allreduce_rmsnorm_quantize", "w8a8_packed_weight_bytes", "w8a8_pack_weight", "w8a8_register_packed_weight",
     "w8a8_static_scratch_bytes", "w8a8_linear_static_scratch", "w8a8_static_scratch_check_status",
@@ -431,11 +432,12 @@ class Context:
                                            _ptr(k_out), _ptr(v_out), _stream(stream)), "w8a8_kv4_read")
 
     def kv4_attention_decode(self, q, cache, n_blocks, block_table, seq_lens, out, batch, n_heads, head_dim, max_blocks, sm_scale, layer,
-                             n_layers, n_kv, group, quant_group_size=0, Xq=None, Xs=None, stream=None):
-        self._check(self.lib.w8a8_kv4_attention_decode(self.handle, _ptr(q), _ptr(cache), n_blocks, _ptr(block_table), _ptr(seq_lens),
-                                                       _ptr(out), batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers, n_kv,
-                                                       group, quant_group_size, _ptr(Xq), _ptr(Xs), _stream(stream)),
-                    "w8a8_kv4_attention_decode")
+                             n_layers, n_kv, group, quant_group_size=0, Xq=None, Xs=None, stream=None, ahead=False):
+        """ahead=True: w8a8_kv4_attention_decode_ahead, for a caller who can make the statement it asks for."""
+        name = "w8a8_kv4_attention_decode_ahead" if ahead else "w8a8_kv4_attention_decode"
+        self._check(getattr(self.lib, name)(self.handle, _ptr(q), _ptr(cache), n_blocks, _ptr(block_table), _ptr(seq_lens),
+                                            _ptr(out), batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers, n_kv,
+                                            group, quant_group_size, _ptr(Xq), _ptr(Xs), _stream(stream)), name)
 
     def linear4_q(self, W4, w_scale, group_size, Xq, Xs, Y, M, N, K, epilogue=EPI_NONE, residual=None, stream=None):
         self._check(self.lib.w8a8_linear4_q(self.handle, _ptr(W4), _ptr(w_scale), group_size, _ptr(Xq), _ptr(Xs), _ptr(Y), M, N, K, epilogue,

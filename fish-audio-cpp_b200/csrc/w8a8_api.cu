@@ -612,9 +612,9 @@ size_t w8a8_kv4_attention_workspace_bytes(int n_heads, int n_kv_heads) {
     return kv4_attention_scratch(n_heads, n_kv_heads);
 }
 
-int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table, const int* seq_lens,
-                              void* out, int batch, int n_heads, int head_dim, int max_blocks_per_seq, float sm_scale, int layer, int n_layers,
-                              int n_kv_heads, int group_size, int quant_group_size, void* Xq, void* Xs, void* stream) {
+static int kv4_attention(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table, const int* seq_lens,
+                         void* out, int batch, int n_heads, int head_dim, int max_blocks_per_seq, float sm_scale, int layer, int n_layers,
+                         int n_kv_heads, int group_size, int quant_group_size, void* Xq, void* Xs, bool ahead, void* stream) {
     if (int rc = check_kv4(ctx, "kv4_attention_decode", cache, n_blocks, layer, n_layers, batch, n_heads, n_kv_heads, head_dim, group_size)) return rc;
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 8)
         return fail(W8A8_ERR_UNSUPPORTED, "kv4_attention_decode: %d query heads over %d kv heads (1 to 8 each are built)", n_heads, n_kv_heads);
@@ -635,7 +635,21 @@ int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, i
     return launch_kv4_attention(static_cast<const __half*>(q), cache, n_blocks, block_table, seq_lens, static_cast<__half*>(out), batch, n_heads,
                                 n_kv_heads, max_blocks_per_seq, sm_scale, layer, n_layers, group_size, quant_group_size, static_cast<int8_t*>(Xq),
                                 static_cast<float*>(Xs), reinterpret_cast<float*>(ctx->workspace), ctx->tail_counters + kTailCounterInts,
-                                ctx->device_status, static_cast<cudaStream_t>(stream));
+                                ctx->device_status, ahead, static_cast<cudaStream_t>(stream));
+}
+
+int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table, const int* seq_lens,
+                              void* out, int batch, int n_heads, int head_dim, int max_blocks_per_seq, float sm_scale, int layer, int n_layers,
+                              int n_kv_heads, int group_size, int quant_group_size, void* Xq, void* Xs, void* stream) {
+    return kv4_attention(ctx, q, cache, n_blocks, block_table, seq_lens, out, batch, n_heads, head_dim, max_blocks_per_seq, sm_scale, layer, n_layers,
+                         n_kv_heads, group_size, quant_group_size, Xq, Xs, false, stream);
+}
+
+int w8a8_kv4_attention_decode_ahead(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table, const int* seq_lens,
+                              void* out, int batch, int n_heads, int head_dim, int max_blocks_per_seq, float sm_scale, int layer, int n_layers,
+                              int n_kv_heads, int group_size, int quant_group_size, void* Xq, void* Xs, void* stream) {
+    return kv4_attention(ctx, q, cache, n_blocks, block_table, seq_lens, out, batch, n_heads, head_dim, max_blocks_per_seq, sm_scale, layer, n_layers,
+                         n_kv_heads, group_size, quant_group_size, Xq, Xs, true, stream);
 }
 
 static int check_weight4(const w8a8_ctx* ctx, const char* what, int N, int K, int group_size) {

@@ -189,7 +189,7 @@ int kv4_max_batch();
 size_t kv4_attention_scratch(int n_q, int n_kv);
 int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const int* table, const int* lens, __half* out, int batch, int n_q,
                          int n_kv, int max_blocks, float sm_scale, int layer, int n_layers, int group, int g, int8_t* Xq, float* Xs,
-                         float* scratch, int* tickets, int* status, cudaStream_t stream);
+                         float* scratch, int* tickets, int* status, bool ahead, cudaStream_t stream);
 // w8a8_linear4.cu : few rows of activation codes times 4-bit weights.
 int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t* Xq, const float* Xs, __half* Y, const __half* residual, int M, int N,
                    int K, int epilogue, int* status, cudaStream_t stream);

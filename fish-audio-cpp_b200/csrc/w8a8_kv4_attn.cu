@@ -57,6 +57,7 @@ struct Kv4Params {
     float* scratch;    // [CTAs][2] pieces
     int* tickets;      // [CTAs], zero between launches
     int* status;
+    bool ahead;  // lengths, table and all pages but each sequence's last were complete ahead of the launch ahead
 };
 
 // ---- helpers -------------------------------------------------------------------------------------------------------
@@ -256,8 +257,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         ptx::fence_proxy_async();
     }
     if (tid < 2 * W) piece_pair[tid] = -1;
-    ptx::pdl_wait();
-    ptx::pdl_launch_dependents();
+    if (!p.ahead) ptx::pdl_wait();
 
     // ---- table entries in use ahead of every sequence; each is n_kv units ----
     const int cap = p.max_blocks * kTokens;
@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     auto units_ahead = [&](int b) { return first_s[b] * p.n_kv; };
 
     const uint32_t ring = ptx::smem_u32(ring_all) + warp * (D * kPage);
-    int page_of = 0;  // the page's number in the cache of unit (i & ~31) + lane of the run
+    int page_of = 0;     // the page's number in the cache of unit (i & ~31) + lane of the run
+    bool newest = false;  // it is its sequence's last
     auto look_up = [&](int i0) {
         const int i = i0 + lane;
         if (i < n_mine) {
@@ -351,6 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             int phys = p.table[static_cast<size_t>(b) * p.max_blocks + blk];
             if (phys < 0 || phys >= p.n_blocks) phys = 0;  // (the caller's mistake; reads stay inside the cache)
             page_of = (phys * p.n_layers + p.layer) * p.n_kv + h;
+            newest = blk == blocks - 1;
         }
     };
     auto issue = [&](int i) {  // the copy of unit i of the run, by the lane that knows where it is
@@ -362,8 +364,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     };
     if (n_mine > 0) {
         look_up(0);
-        for (int i = 0; i < min(n_mine, D); ++i) issue(i);
+        if (p.ahead) {  // a sequence's last page may still be in the making
+            const uint32_t later = __ballot_sync(0xffffffffu, newest && lane < min(n_mine, D));
+            for (int i = 0; i < min(n_mine, D); ++i)
+                if (!(later >> i & 1)) issue(i);
+            ptx::pdl_wait();
+            for (uint32_t rest = later; rest; rest &= rest - 1) issue(__ffs(rest) - 1);
+        } else {
+            for (int i = 0; i < min(n_mine, D); ++i) issue(i);
+        }
+    } else if (p.ahead) {
+        ptx::pdl_wait();
     }
+    ptx::pdl_launch_dependents();
 
     // rows of no tokens: zeros
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
@@ -669,11 +682,11 @@ size_t kv4_attention_scratch(int n_q, int n_kv) {
 
 int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const int* table, const int* lens, __half* out, int batch, int n_q,
                          int n_kv, int max_blocks, float sm_scale, int layer, int n_layers, int group, int g, int8_t* Xq, float* Xs,
-                         float* scratch, int* tickets, int* status, cudaStream_t stream) {
+                         float* scratch, int* tickets, int* status, bool ahead, cudaStream_t stream) {
     if (batch == 0) return W8A8_OK;
     const int ratio = n_q / n_kv;
     Kv4Params p = {q, static_cast<const unsigned char*>(cache), table, lens, out, Xq, Xs, g, batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers,
-                   sm_scale * 1.4426950408889634f * 0x1p24f, scratch, tickets, status};
+                   sm_scale * 1.4426950408889634f * 0x1p24f, scratch, tickets, status, ahead};
     const long long most = static_cast<long long>(batch) * n_kv * max_blocks;  // units, were all sequences as long as their rows
     const int sms = device_sms() < kKv4Tickets ? device_sms() : kKv4Tickets, ctas = most < sms ? static_cast<int>(most) : sms;
     cudaError_t e;

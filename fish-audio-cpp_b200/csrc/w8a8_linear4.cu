@@ -217,7 +217,6 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
             if (x0 + i * kL4Warps * 32 < chunks) c_next[i] = ptx::ld_result_v4(p.Xq + 16ll * (x0 + i * kL4Warps * 32));
     };
     if constexpr (DIRECT) {
-        ptx::fence_proxy_async();  // (what the launch ahead wrote is read by bulk copies)
         if (lane == 0)
             for (int i = 0; i < min(p.stages, n_mine); ++i) issue_codes(i);
     } else {

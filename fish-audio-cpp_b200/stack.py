@@ -336,7 +336,7 @@ class SlowARStack:
                               q_norm_w=lw["q_norm"], k_norm_w=lw["k_norm"], eps=c.eps, freqs=self.freqs, positions=self.positions, q_out=self.q)
                 ctx.kv4_attention_decode(self.q, self.cache4, self.n_blocks, self.block_table, self.seq_lens, None, B, self.nq_l, D,
                                          self.max_blocks, sm_scale, l, c.n_layer, self.nkv_l, self.kv_group, quant_group_size=g,
-                                         Xq=self.aq, Xs=self.as_)
+                                         Xq=self.aq, Xs=self.as_, ahead=True)
             elif self.fuse_rope:
                 ctx.qkv_attention_decode(self.qkv, lw["q_norm"], lw["k_norm"], c.eps, self.freqs, self.positions,
                                          self.k_cache, self.v_cache, self.block_table, self.seq_lens, None, B, self.nq_l,

@@ -362,6 +362,15 @@ W8A8_API int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void*
                               const int* seq_lens, void* out, int batch, int n_heads, int head_dim,
                               int max_blocks_per_seq, float sm_scale, int layer, int n_layers, int n_kv_heads,
                               int group_size, int quant_group_size, void* Xq, void* Xs, void* stream);
+/* The same for a caller who states that lengths, block table and this layer's pages of all blocks but each sequence's last were written ahead
+ * of a w8a8_kv4_write call (of one token or more), or of an ordinary launch or copy, that itself lies ahead of this call on the same stream. The kernel may then
+ * read them before the launch directly ahead of it has finished: in a decode step of one new token per sequence the launch ahead is the
+ * w8a8_kv4_write of its rows. Results are the same; where the statement does not hold (a w8a8_plan_blocks directly ahead, say, or a prompt's
+ * rows, which fill other blocks too) they are undefined. */
+W8A8_API int w8a8_kv4_attention_decode_ahead(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table,
+                              const int* seq_lens, void* out, int batch, int n_heads, int head_dim,
+                              int max_blocks_per_seq, float sm_scale, int layer, int n_layers, int n_kv_heads,
+                              int group_size, int quant_group_size, void* Xq, void* Xs, void* stream);
 
 /* w8a8_linear_q over 4-bit weights: W4 uint8 [N, K / 2], row-major, two codes a byte as two's complement, the even k in the low four
  * bits; w_scale fp16 [N, G] (4-bit groups along K); Xq, Xs as there. Per group an exact int32 sum, promoted with both scales in

@@ -706,6 +706,44 @@ def test_two_contexts_on_two_streams(pkg):
         ctx.close()
 
 
+@pytest.mark.parametrize("lens", [[1], [17, 1, 33], [1000] * 8, [16, 48, 32, 0], [9000, 5]])
+def test_kv4_attention_ahead_of_the_write(ctx, lens):
+    """Layer after layer, the newest row written and attended over with nothing in between: the call that starts early gives what the
+    other gives, also where the new row opens a block, and where a sequence has none."""
+    rng = np.random.default_rng(len(lens) + lens[0])
+    n_q, n_kv, group, layers, B = 8, 2, 32, 6, len(lens)
+    width = max(lens) // 16 + 1
+    q, pages, table, n = attention_case(rng, lens, n_q, n_kv, group, layers, width)
+    slots = dev(np.array([table[b, (m - 1) // 16] * 16 + (m - 1) % 16 if m else -1 for b, m in enumerate(lens)], np.int64))
+    qkv = [dev(rng.standard_normal((B, n_q + 2 * n_kv, D)).astype(np.float16)) for _ in range(layers)]
+    dtable, dlens, blocks, side = dev(table), dev(n), len(pages), torch.cuda.Stream()
+
+    def run(cache, rows, out, ahead):
+        for l in range(layers):
+            ctx.kv4_write(qkv[l], slots, cache, blocks, l, layers, B, n_q, n_kv, D, group, q_out=rows)
+            ctx.kv4_attention_decode(rows, cache, blocks, dtable, dlens, out[l], B, n_q, D, width, 0.1, l, layers, n_kv, group, ahead=ahead)
+
+    results = []
+    for ahead in (False, True):
+        for captured in (False, True):
+            cache, rows, out = dev(pages), torch.zeros((B, n_q, D), dtype=torch.float16, device="cuda"), torch.zeros((layers, B, n_q, D), dtype=torch.float16, device="cuda")
+            with torch.cuda.stream(side):
+                side.wait_stream(torch.cuda.default_stream())
+                if captured:
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph, stream=side):
+                        run(cache, rows, out, ahead)
+                    for _ in range(3):
+                        graph.replay()
+                else:
+                    run(cache, rows, out, ahead)
+            torch.cuda.synchronize()
+            results.append((out, cache))
+    ctx.check_device_status()
+    for out, cache in results[1:]:
+        assert torch.equal(out, results[0][0]) and torch.equal(cache, results[0][1])
+
+
 def test_replays_and_eager_calls_in_turn(ctx):
     """Two graphs and eager calls of other sizes take turns on one stream: they share the context's scratch and tickets."""
     rng = np.random.default_rng(31)

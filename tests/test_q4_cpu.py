@@ -109,7 +109,8 @@ def _attention_args(**change):
     (dict(xq=P, xs=P, quant=96), UNSUPPORTED), (dict(xq=P, xs=P, quant=1024), UNSUPPORTED), (dict(xq=P + 1, xs=P, quant=64), BAD)])
 def test_kv4_attention_refuses(pkg, change, status):
     lib = pkg.load_library()
-    assert lib.w8a8_kv4_attention_decode(*_attention_args(**change)) == status and lib.w8a8_last_error()
+    for call in (lib.w8a8_kv4_attention_decode, lib.w8a8_kv4_attention_decode_ahead):
+        assert call(*_attention_args(**change)) == status and lib.w8a8_last_error()
 
 
 def _linear_args(**change):
