@@ -262,6 +262,7 @@ class SlowARStack:
         self.weight_bytes = wbytes
         kv_row = 2 * D * 2 if kv_bits == 16 else capi.kv4_cache_bytes(1, 1, 1, D, kv_group) // c.block_tokens  # k and v of a token and kv head
         self.kv_bytes_per_step = lambda ctx_len: B * ctx_len * c.n_layer * self.nkv_l * kv_row
+        torch.cuda.synchronize()  # (tables and caches are there whatever stream the steps run on)
 
     def _weight4(self, w, s):
         """A weight in 4 bits from its int8 codes and scales: what a loader does with the fp16 values of a checkpoint."""
