@@ -3,10 +3,11 @@
 //   out[b, h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(q_h . k_t sm_scale - max),  t < seq_lens[b];  zeros where seq_lens[b] is 0
 //   k_t, v_t = code * scale of the row's group; one pass with the running maximum and sum of the softmax, both fp32
 //
-// Bound: HBM and the unpacking, close to one another. A token costs 128 + 4 G bytes per kv head (K and V; G = 128 / group) instead of the fp16
-// cache's 512; a warp executes some 350 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 74 us, 61 % of
-// the measured copy rate; the copies alone, without arithmetic, take 54, the arithmetic alone, on pages that lie in L2, 71. Half of the
-// instructions go to the half-rate pipe that masks and shifts; two pages at a time, scales folded into p, and 8 or 16 warps instead of 12 changed nothing.
+// Bound: HBM and the arithmetic, close to one another. A token costs 128 + 4 G bytes per kv head (K and V; G = 128 / group) instead of the fp16
+// cache's 512; a warp executes some 340 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 77 us, 58 % of
+// the measured copy rate; the copies alone, without arithmetic, take 54, the arithmetic alone, without copies, 61 (the scores and the
+// softmax 42 of them, a chain that three warps a scheduler cannot hide). Two pages at a time, one page's scores beside the sum over the page
+// before it, scales folded into p, and 8 or 14 or 16 warps instead of 12 changed nothing or cost time.
 //
 // Split. The unit is a page: 16 tokens of one (sequence, kv head). All units of the batch, in the order sequence, head, page, are one
 // range that is cut evenly over the warps of the grid (a CTA's warps take neighbouring runs), whatever the lengths are: nobody waits
@@ -20,8 +21,9 @@
 // Arithmetic. Scores: a masked nibble is, as the bits of an fp16 number, the subnormal code * 2^-24 (or, four bits up, code * 2^-20, which
 // meets a q that was divided by 16), exact as a matrix operand: one instruction for two codes. The 8 that stored codes carry leaves with the
 // accumulator's start, -8 * sum of q over the group. Sums are fp32 per group, times the group's scale in fp32. P V: codes as fp16 numbers
-// (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p is rounded to fp16 (2^-11
-// relative, and the denominator sums the rounded values); products are summed in fp32. The reference of the exponentials is a score of the
+// (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p as two fp16 numbers, the
+// rounded one and what that left, which costs nothing here (77.3 and 77.1 us) and takes the error from 3.3e-4 of the output to 2.6e-4,
+// of which the output's own rounding is 2.1e-4; products are summed in fp32. The reference of the exponentials is a score of the
 // row that others exceed by at most 2^kLag, so that it moves, and the sums with it, a few times per row only.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
@@ -519,13 +521,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                 }
                 relative();
             }
-            const __half2 p0 = __floats2half2_rn(exp2_fast(y[0]), exp2_fast(y[1])), p1 = __floats2half2_rn(exp2_fast(y[2]), exp2_fast(y[3]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = exp2_fast(y[e]);
+            l_run[0] += y[0] + y[2];
+            l_run[1] += y[1] + y[3];
+            // as two fp16 numbers each: rounded, and what that left
+            const __half2 p0 = __floats2half2_rn(y[0], y[1]), p1 = __floats2half2_rn(y[2], y[3]);
             const float2 f0 = __half22float2(p0), f1 = __half22float2(p1);
-            l_run[0] += f0.x + f1.x;
-            l_run[1] += f0.y + f1.y;
+            const __half2 r0 = __floats2half2_rn(y[0] - f0.x, y[1] - f0.y), r1 = __floats2half2_rn(y[2] - f1.x, y[3] - f1.y);
 
             // ---- out^T += V^T P^T: rows are channels, columns heads, the contraction runs over tokens ----
-            const uint32_t pb0 = transposed(as_u32(p0)), pb1 = transposed(as_u32(p1));
+            const uint32_t pb0 = transposed(as_u32(p0)), pb1 = transposed(as_u32(p1)), rb0 = transposed(as_u32(r0)), rb1 = transposed(as_u32(r1));
 #pragma unroll
             for (int high = 0; high < 2; ++high) {
                 uint32_t a0[4], a1[4], a2[4], a3[4];
@@ -536,8 +542,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const __half2 s0 = as_half2(vs0[(4 * high + n) * G / 8]), s1 = as_half2(vs1[(4 * high + n) * G / 8]);
-                    mma_f16(o[4 * high + n], as_u32(__hmul2(as_half2(a0[n]), s0)), as_u32(__hmul2(as_half2(a1[n]), s0)),
-                            as_u32(__hmul2(as_half2(a2[n]), s1)), as_u32(__hmul2(as_half2(a3[n]), s1)), pb0, pb1);
+                    const uint32_t v[4] = {as_u32(__hmul2(as_half2(a0[n]), s0)), as_u32(__hmul2(as_half2(a1[n]), s0)), as_u32(__hmul2(as_half2(a2[n]), s1)),
+                                           as_u32(__hmul2(as_half2(a3[n]), s1))};
+                    mma_f16(o[4 * high + n], v[0], v[1], v[2], v[3], pb0, pb1);
+                    mma_f16(o[4 * high + n], v[0], v[1], v[2], v[3], rb0, rb1);
                 }
             }
 
