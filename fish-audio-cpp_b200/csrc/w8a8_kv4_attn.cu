@@ -19,7 +19,7 @@
 // pairs; nothing in the steady state synchronises warps.
 //
 // Arithmetic. Scores: a masked nibble is, as the bits of an fp16 number, the subnormal code * 2^-24 (or, four bits up, code * 2^-20, which
-// meets a q that was divided by 16), exact as a matrix operand: one instruction for two codes. The 8 that stored codes carry leaves with the
+// meets a q that was divided by 16: below 2^-10 that rounds by 2^-25), exact as a matrix operand: one instruction for two codes. The 8 that stored codes carry leaves with the
 // accumulator's start, -8 * sum of q over the group. Sums are fp32 per group, times the group's scale in fp32. P V: codes as fp16 numbers
 // (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p as two fp16 numbers, the
 // rounded one and what that left, which costs nothing here (77.3 and 77.1 us) and takes the error from 3.3e-4 of the output to 2.6e-4,
