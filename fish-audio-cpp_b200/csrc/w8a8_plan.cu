@@ -11,7 +11,8 @@
 // back and taken again in the same call is read from the row that gives it, so that nothing that is read is written by the call, but
 // for the lengths and the stack's count where the caller has them updated in place.
 //
-// Bound: latency at decode sizes (one round trip for the lengths, one for block numbers), 12 bytes written per token for prompts. One
+// Bound: latency at decode sizes (one round trip for the lengths, one for block numbers; 8 requests 4.5 us), 12 bytes written per token for prompts (512
+// requests, 200000 tokens 10.1 us). One
 // launch: a CTA per 4096 tokens, each of which makes the sums again (200000 tokens: 20.1 us when a cluster of eight shared them) and then
 // four tokens a thread. What may be updated in place is written by the CTA that comes last (a ticket, reset by that CTA). All or nothing:
 // where the blocks, the table's width, the token count or a length do not fit, no request gets anything, and `info` says why.
