@@ -6,7 +6,7 @@
 // decode step's go the same way, and rows with a negative slot (a captured step's empty rows) are left alone, their q too.
 //
 // Bound: for prompts instructions and bytes alike (2 (n_q + 2 n_kv) 128 read and 2 n_q 128 written per token), latency for a decode step.
-// 8192 tokens of 32 + 16 heads 48.3 us to write (issue slots 75 % busy; 27 for the bytes) and 10.8 to read back, a decode step's 8 tokens 3.5 for both.
+// 8192 tokens of 32 + 16 heads 43 us to write (27 for the bytes; 35 without the norm) and 10.9 to read back, a decode step's 8 tokens 3.5 for both.
 // Half a warp holds a head, eight neighbouring channels a lane: 16-byte reads and writes, a K word a lane, and of the norm's tree three levels
 // in the lane. A warp takes one token and one pair of heads after another, so that the angles are made once.
 #include "sm100_ptx.cuh"
@@ -16,7 +16,7 @@
 namespace w8a8 {
 namespace {
 
-constexpr int kStoreWarps = 4;
+constexpr int kStoreWarps = 4, kPairsAhead = 4;
 
 struct StoreParams {
     const __half* qkv;       // [tokens, (n_q + 2 n_kv) * 128]
@@ -44,6 +44,14 @@ __device__ __forceinline__ Row load_row(const __half* src, int l) {
     r.h[1] = *reinterpret_cast<const __half2*>(&v.y);
     r.h[2] = *reinterpret_cast<const __half2*>(&v.z);
     r.h[3] = *reinterpret_cast<const __half2*>(&v.w);
+    return r;
+}
+__device__ __forceinline__ Row lds_row(uint32_t addr) {
+    Row r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(*reinterpret_cast<uint32_t*>(&r.h[0])), "=r"(*reinterpret_cast<uint32_t*>(&r.h[1])), "=r"(*reinterpret_cast<uint32_t*>(&r.h[2])),
+                   "=r"(*reinterpret_cast<uint32_t*>(&r.h[3]))
+                 : "r"(addr) : "memory");
     return r;
 }
 __device__ __forceinline__ void store_row(__half* dst, int l, const Row& r) {
@@ -125,7 +133,7 @@ __device__ __forceinline__ uint32_t exchange_bytes(uint32_t w, int n) {
 __host__ __device__ inline int store_pairs(int n_q, int n_kv) { return (n_q + 1) / 2 + 2 * ((n_kv + 1) / 2); }
 
 template <int GROUPS>
-__global__ void __launch_bounds__(kStoreWarps * 32, 8) kv4_write_kernel(const __grid_constant__ StoreParams p) {
+__global__ void __launch_bounds__(kStoreWarps * 32, 10) kv4_write_kernel(const __grid_constant__ StoreParams p) {
     constexpr int kSpan = 16 / GROUPS;  // lanes of a group
     const int lane = threadIdx.x & 31, l = lane & 15, side = lane >> 4;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -145,19 +153,35 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 8) kv4_write_kernel(const __
     const long long slot = p.slots[token];
     if (slot < 0 || slot >= p.n_slots) return;
     const __half* const row = p.qkv + static_cast<size_t>(token) * (p.n_q + 2 * p.n_kv) * q4::kDim;
-    auto fetch = [&](int pair) {  // (a half without a head: its neighbour's)
-        const int kind = pair < q_pairs ? 0 : pair < q_pairs + kv_pairs ? 1 : 2;
-        const int h = 2 * (pair - (kind > 0 ? q_pairs : 0) - (kind > 1 ? kv_pairs : 0)) + side;
-        return load_row(row + ((kind > 0 ? p.n_q : 0) + (kind > 1 ? p.n_kv : 0) + min(h, (kind > 0 ? p.n_kv : p.n_q) - 1)) * q4::kDim, l);
+    // Heads lie one behind the other, q, k, v; a pair's are two neighbours, but for the last of an odd kind, whose second half reads the next kind's
+    // first (at the row's end its neighbour's) for nothing.
+    const int heads = p.n_q + 2 * p.n_kv;
+    int ahead = 2 * first - (first >= q_pairs ? p.n_q & 1 : 0) - (first >= q_pairs + kv_pairs ? p.n_kv & 1 : 0);  // the first head of the next pair to fetch
+    // Through shared memory, kPairsAhead ahead; a lane copies what it reads itself, so that it waits for nobody else. (8192 tokens, one pair ahead in
+    // registers 48 us, with the norm and without; ahead by 2, 3, 4, 8 42.6, 42.9, 43.0, 43.2 with it and 38.2, 36.1, 35.0, 34.2 without.)
+    __shared__ __align__(16) uint4 ring_s[kStoreWarps][kPairsAhead][32];
+    const uint32_t ring = ptx::smem_u32(&ring_s[warp][0][lane]);
+    int asked = first;
+    auto ask = [&] {
+        if (asked < last) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (asked - first) % kPairsAhead * 512),
+                         "l"(row + min(ahead + side, heads - 1) * q4::kDim + 8 * l)
+                         : "memory");
+            ++asked;
+            ahead += 2 - (asked == q_pairs ? p.n_q & 1 : asked == q_pairs + kv_pairs ? p.n_kv & 1 : 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    Row next = fetch(first);  // (more than one ahead gave nothing: 8192 tokens 48.3 us with one, 49.7 with two, 50.3 with three)
+#pragma unroll 1
+    for (int i = 0; i < kPairsAhead; ++i) ask();
     auto take = [&](int pair) {
-        const Row r = next;
-        if (pair + 1 < last) next = fetch(pair + 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kPairsAhead - 1) : "memory");
+        const Row r = lds_row(ring + (pair - first) % kPairsAhead * 512);
+        ask();
         return r;
     };
     // cosines and sines of the lane's four pairs; either half makes two
-    F2 c[2], s[2];
+    F2 c[2], s[2], minus_s[2];
     if (turned && first < q_pairs + kv_pairs) {
         const float pos = static_cast<float>(p.positions[token]);
         const float2 a = cos_sin(f[0] * pos), b = cos_sin(f[1] * pos);
@@ -168,6 +192,8 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 8) kv4_write_kernel(const __
         c[1] = side ? mine_c : other_c;
         s[0] = side ? other_s : mine_s;
         s[1] = side ? mine_s : other_s;
+        minus_s[0] = -s[0];
+        minus_s[1] = -s[1];
     }
     auto turn = [&](const Row& r) {  // norm and rotation of a q or k row
         const Row t = normed ? normed_row(r, w, p.eps) : r;
@@ -176,7 +202,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 8) kv4_write_kernel(const __
         Wide o;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // interleaved pairs (rope.cu:36-45), rounded as qknorm_rope_kvwrite_kernel's are
-            o.x[i] = fma2(v.x[i], c[i], -(v.y[i] * s[i]));
+            o.x[i] = fma2(v.x[i], c[i], v.y[i] * minus_s[i]);
             o.y[i] = fma2(v.y[i], c[i], v.x[i] * s[i]);
         }
         return o.halves();
@@ -211,10 +237,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 8) kv4_write_kernel(const __
 #pragma unroll
         for (int d = kSpan / 2; d > 0; d >>= 1) mx = __hmax2_nan(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const q4::Scale sc(mx);
-        uint32_t word = 0;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            word |= static_cast<uint32_t>(sc.code(__low2half(r.h[x])) + 8) << (8 * x) | static_cast<uint32_t>(sc.code(__high2half(r.h[x])) + 8) << (8 * x + 4);
+        const uint32_t word = sc.codes_plus_8(r.h);
         const int n = (l >> 1) & 3;
         const uint32_t pieces = is_v ? exchange_bytes(word, n) : 0u;
         if (head >= p.n_kv) continue;
@@ -304,8 +327,8 @@ int launch_kv4_write(const __half* qkv, const __half* q_norm_w, const __half* k_
     if (tokens == 0) return W8A8_OK;
     StoreParams p = {qkv, q_norm_w, k_norm_w, eps, freqs, positions, slots, static_cast<long long>(n_blocks) * q4::kTokens,
                      static_cast<unsigned char*>(cache), tokens, n_q, n_kv, layer, n_layers, q_out, 1};
-    // A warp takes one pair of heads while that does not fill the GPU (32 warps an SM run at once), else several, up to a token's: 48 warps an SM or
-    // more. (With 96 and 150: 613 tokens 8.6 us instead of 5.9, 2048 tokens 18.8 and 21.4 instead of 15.3, 8192 tokens 49.7 and 55.4 instead of 48.3.)
+    // A warp takes one pair of heads while that does not fill the GPU (40 warps an SM run at once), else several, up to a token's: 48 warps an SM or
+    // more. (With 32 and 96: 613 tokens 5.5 and 8.0 us instead of 6.0, 2048 tokens 16.7 and 17.3 instead of 14.9, 8192 tokens 42.6 and 44.3 instead of 42.6.)
     const int pairs = store_pairs(n_q, n_kv);
     const long long each = static_cast<long long>(tokens) * pairs / (48ll * device_sms());
     p.pairs_per_warp = each < 1 ? 1 : each < pairs ? static_cast<int>(each) : pairs;
