@@ -12,9 +12,10 @@
 // for the lengths and the stack's count where the caller has them updated in place.
 //
 // Bound: latency at decode sizes (one round trip for the lengths, one for block numbers; 8 requests 4.5 us), 12 bytes written per token for prompts (512
-// requests, 200000 tokens 10.1 us). One
+// requests, room for 200000 tokens 9.2 us). One
 // launch: a CTA per 4096 tokens, each of which makes the sums again (200000 tokens: 20.1 us when a cluster of eight shared them) and then
-// four tokens a thread. What may be updated in place is written by the CTA that comes last (a ticket, reset by that CTA). All or nothing:
+// four tokens a thread. What is updated in place is written by the CTA that comes last (a ticket, reset by that CTA; 512 requests 10.1 us with it, 9.2
+// without). All or nothing:
 // where the blocks, the table's width, the token count or a length do not fit, no request gets anything, and `info` says why.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
@@ -23,6 +24,7 @@ namespace w8a8 {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+static_assert(kPlanThreads == 32 * 32, "a warp adds up the warps' sums");
 constexpr int kPlanBlock = 16;
 constexpr int kPlanMaxBatch = 4096;
 
@@ -43,7 +45,7 @@ struct PlanParams {
     int max_tokens;
     int* info;
     int vector_stores;  // slots and positions are 16-byte aligned
-    int* ticket;        // zero between launches
+    int* ticket;        // zero between launches; null where nothing is updated in place, or by one CTA
 };
 
 struct Sums {
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
         }
     }
     // what may be an input too: when every CTA has read it
-    if (parts > 1) {
+    if (p.ticket) {
         __syncthreads();
         if (tid == 0) {
             int before;
@@ -211,6 +213,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
         }
         __syncthreads();
         if (!last_s) return;
+    } else if (part > 0) {
+        return;
     }
     for (int b = tid; b < p.batch; b += kPlanThreads) {
         const int cached = cached_s[b], was = cached < 0 ? -1 - cached : cached;
@@ -233,6 +237,7 @@ int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* tabl
                     seq_lens, first_token, max_tokens, info,
                     ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) & 15u) == 0, ticket};
     const int want = (max_tokens + 4 * kPlanThreads - 1) / (4 * kPlanThreads), sms = device_sms(), parts = want < 1 ? 1 : want < sms ? want : sms;
+    if (parts == 1 || (seq_lens != cached && free_count_out != free_count)) p.ticket = nullptr;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(parts, 1, 1);
     cfg.blockDim = dim3(kPlanThreads, 1, 1);
