@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import threading
 from pathlib import Path
 
@@ -258,6 +259,41 @@ def kv4_attention_workspace_bytes(n_heads, n_kv) -> int:
     return load_library().w8a8_kv4_attention_workspace_bytes(n_heads, n_kv)
 
 
+class _CtypesCalls:
+    """The calls of w8a8_calls where it was not built (no Python headers): the same arguments, through ctypes."""
+
+    def __init__(self, lib):
+        self._lib = lib
+
+    def __getattr__(self, name):
+        fn = getattr(self._lib, name)
+
+        def call(*args):
+            return fn(*[x if x is None or isinstance(x, (int, float)) else x.data_ptr() for x in args])
+
+        setattr(self, name, call)
+        return call
+
+
+_CALLS = None
+
+
+def _load_calls(lib):
+    """w8a8_calls (csrc/w8a8_calls.cpp), bound to the loaded library's functions."""
+    global _CALLS
+    if _CALLS is None:
+        path = Path(__file__).resolve().parent / "lib" / "w8a8_calls.so"
+        if path.exists():
+            spec = importlib.util.spec_from_file_location("w8a8_calls", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in dir(module) if n.startswith("w8a8_")})
+            _CALLS = module
+        else:
+            _CALLS = _CtypesCalls(lib)
+    return _CALLS
+
+
 class Context:
     """Owns one w8a8_ctx. Use one per stream."""
 
@@ -266,12 +302,14 @@ class Context:
         h = C.c_void_p()
         self._check(self.lib.w8a8_create(C.byref(h), device, workspace_bytes), "w8a8_create")
         self.handle = h
+        self.address = h.value
+        self.calls = _load_calls(self.lib)
         self.device = device
 
     def close(self):
         if getattr(self, "handle", None):
             self.lib.w8a8_destroy(self.handle)
-            self.handle = None
+            self.handle = self.address = None
 
     def __del__(self):
         try:
@@ -413,35 +451,42 @@ class Context:
                                             _ptr(out), batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers, n_kv,
                                             quant_group_size, _ptr(Xq), _ptr(Xs), context_splits, _stream(stream)), name)
 
+    # (these go through w8a8_calls, which takes tensors and addresses alike)
     def plan_blocks(self, cached_lens, new_lens, batch, block_table, max_blocks, free_blocks, free_capacity, free_count, slots, positions,
                     seq_lens, first_token, max_tokens, info, free_count_out=None, stream=None):
         """Block tables, slots and positions of a step from the requests' lengths. free_count_out None: free_count is updated in place."""
-        self._check(self.lib.w8a8_plan_blocks(self.handle, _ptr(cached_lens), _ptr(new_lens), batch, _ptr(block_table), max_blocks,
-                                              _ptr(free_blocks), free_capacity, _ptr(free_count),
-                                              _ptr(free_count if free_count_out is None else free_count_out), _ptr(slots), _ptr(positions),
-                                              _ptr(seq_lens), _ptr(first_token), max_tokens, _ptr(info), _stream(stream)), "w8a8_plan_blocks")
+        rc = self.calls.w8a8_plan_blocks(self.address, cached_lens, new_lens, batch, block_table, max_blocks, free_blocks, free_capacity, free_count,
+                                         free_count if free_count_out is None else free_count_out, slots, positions, seq_lens, first_token,
+                                         max_tokens, info, _stream(stream))
+        if rc:
+            self._check(rc, "w8a8_plan_blocks")
 
     def kv4_write(self, qkv, slots, cache, n_blocks, layer, n_layers, tokens, n_q, n_kv, head_dim, group, q_norm_w=None, k_norm_w=None,
                   eps=0.0, freqs=None, positions=None, q_out=None, stream=None):
-        self._check(self.lib.w8a8_kv4_write(self.handle, _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), eps, _ptr(freqs), _ptr(positions),
-                                            _ptr(slots), _ptr(cache), n_blocks, layer, n_layers, tokens, n_q, n_kv, head_dim, group,
-                                            _ptr(q_out), _stream(stream)), "w8a8_kv4_write")
+        rc = self.calls.w8a8_kv4_write(self.address, qkv, q_norm_w, k_norm_w, eps, freqs, positions, slots, cache, n_blocks, layer, n_layers,
+                                       tokens, n_q, n_kv, head_dim, group, q_out, _stream(stream))
+        if rc:
+            self._check(rc, "w8a8_kv4_write")
 
     def kv4_read(self, cache, n_blocks, slots, layer, n_layers, tokens, n_kv, head_dim, group, k_out, v_out, stream=None):
-        self._check(self.lib.w8a8_kv4_read(self.handle, _ptr(cache), n_blocks, _ptr(slots), layer, n_layers, tokens, n_kv, head_dim, group,
-                                           _ptr(k_out), _ptr(v_out), _stream(stream)), "w8a8_kv4_read")
+        rc = self.calls.w8a8_kv4_read(self.address, cache, n_blocks, slots, layer, n_layers, tokens, n_kv, head_dim, group, k_out, v_out,
+                                      _stream(stream))
+        if rc:
+            self._check(rc, "w8a8_kv4_read")
 
     def kv4_attention_decode(self, q, cache, n_blocks, block_table, seq_lens, out, batch, n_heads, head_dim, max_blocks, sm_scale, layer,
                              n_layers, n_kv, group, quant_group_size=0, Xq=None, Xs=None, stream=None, ahead=False):
         """ahead=True: w8a8_kv4_attention_decode_ahead, for a caller who can make the statement it asks for."""
-        name = "w8a8_kv4_attention_decode_ahead" if ahead else "w8a8_kv4_attention_decode"
-        self._check(getattr(self.lib, name)(self.handle, _ptr(q), _ptr(cache), n_blocks, _ptr(block_table), _ptr(seq_lens),
-                                            _ptr(out), batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers, n_kv,
-                                            group, quant_group_size, _ptr(Xq), _ptr(Xs), _stream(stream)), name)
+        call = self.calls.w8a8_kv4_attention_decode_ahead if ahead else self.calls.w8a8_kv4_attention_decode
+        rc = call(self.address, q, cache, n_blocks, block_table, seq_lens, out, batch, n_heads, head_dim, max_blocks, sm_scale, layer, n_layers,
+                  n_kv, group, quant_group_size, Xq, Xs, _stream(stream))
+        if rc:
+            self._check(rc, "w8a8_kv4_attention_decode")
 
     def linear4_q(self, W4, w_scale, group_size, Xq, Xs, Y, M, N, K, epilogue=EPI_NONE, residual=None, stream=None):
-        self._check(self.lib.w8a8_linear4_q(self.handle, _ptr(W4), _ptr(w_scale), group_size, _ptr(Xq), _ptr(Xs), _ptr(Y), M, N, K, epilogue,
-                                            _ptr(residual), _stream(stream)), "w8a8_linear4_q")
+        rc = self.calls.w8a8_linear4_q(self.address, W4, w_scale, group_size, Xq, Xs, Y, M, N, K, epilogue, residual, _stream(stream))
+        if rc:
+            self._check(rc, "w8a8_linear4_q")
 
     def quantize_weight4(self, W, N, K, group_size, W4, w_scale, stream=None):
         self._check(self.lib.w8a8_quantize_weight4(self.handle, _ptr(W), N, K, group_size, _ptr(W4), _ptr(w_scale), _stream(stream)),

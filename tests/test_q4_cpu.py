@@ -1,10 +1,12 @@
 """Host-side checks of the 4-bit decode step: the restatement agrees with itself, and calls that cannot run are refused before anything
 is launched (no device is needed for that: what is wrong with the arguments is said first)."""
 import ctypes as C
+import importlib
 import math
 
 import numpy as np
 import pytest
+import torch
 
 from oracle import q4
 
@@ -144,3 +146,54 @@ def test_sizes_of_caches_and_scratch(pkg):
     assert pkg.kv4_attention_workspace_bytes(32, 8) > 0 and pkg.kv4_attention_workspace_bytes(8, 1) > pkg.kv4_attention_workspace_bytes(4, 1)
     assert not any(pkg.kv4_attention_workspace_bytes(*a) for a in ((0, 1), (9, 1), (5, 2), (4, 0)))
     assert math.gcd(q4.page_bytes(32), q4.page_bytes(64), q4.page_bytes(128)) % 16 == 0
+
+
+def _both_call_modules(pkg):
+    capi, lib = importlib.import_module(pkg.__name__ + ".capi"), pkg.load_library()
+    made = capi._load_calls(lib)
+    return [made] if isinstance(made, capi._CtypesCalls) else [made, capi._CtypesCalls(lib)]
+
+
+def test_calls_refuse_alike_from_python(pkg):
+    for calls in _both_call_modules(pkg):
+        for name, args, changes in (("w8a8_plan_blocks", _plan_args, (dict(ctx=None), dict(batch=4097), dict(info=None))),
+                                    ("w8a8_kv4_write", _write_args, (dict(tokens=-1), dict(dim=64), dict(qkv=P + 2))),
+                                    ("w8a8_kv4_read", _read_args, (dict(k=None, v=None), dict(group=0))),
+                                    ("w8a8_kv4_attention_decode", _attention_args, (dict(heads=7), dict(out=P + 4))),
+                                    ("w8a8_kv4_attention_decode_ahead", _attention_args, (dict(heads=7), dict(out=P + 4))),
+                                    ("w8a8_linear4_q", _linear_args, (dict(K=127), dict(w=None), dict(epilogue=2, N=24)))):
+            call, plain = getattr(calls, name), getattr(pkg.load_library(), name)
+            for change in changes:
+                assert call(*args(**change)) == plain(*args(**change)) != 0
+            with pytest.raises((TypeError, C.ArgumentError)):
+                call(*args()[:-1])
+            with pytest.raises((AttributeError, TypeError, C.ArgumentError)):
+                call(*["no address" if a == P else a for a in args()])
+
+
+def test_calls_hand_over_what_they_are_given(pkg):
+    """Bound to functions that note their arguments: tensors arrive as their addresses, None as null, numbers as they are."""
+    calls, lib = _both_call_modules(pkg)[0], pkg.load_library()
+    if type(calls).__name__ == "_CtypesCalls":
+        pytest.skip("w8a8_calls is not built")
+    names, seen, kept = [n for n in dir(calls) if n.startswith("w8a8_")], [], []
+    try:
+        for n in names:
+            plain = getattr(lib, n)
+            kept.append(C.CFUNCTYPE(C.c_int, *plain.argtypes)(lambda *a: seen.append(a) or 7))
+        calls.bind({n: C.cast(f, C.c_void_p).value for n, f in zip(names, kept)})
+        for n in names:
+            types = getattr(lib, n).argtypes
+            tensors = [torch.empty(4) for _ in types]
+            args = [t if ty is C.c_void_p and i % 3 else None if ty is C.c_void_p else 0.375 if ty is C.c_float else 1000 + i
+                    for i, (ty, t) in enumerate(zip(types, tensors))]
+            args[0] = (1 << 47) - 8
+            assert getattr(calls, n)(*args) == 7
+            assert list(seen.pop()) == [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+            whole = next(i for i, ty in enumerate(types) if ty is C.c_int)
+            for wrong, error in ((1 << 31, OverflowError), (1 << 70, OverflowError), (1.5, TypeError), (None, TypeError)):
+                with pytest.raises(error):
+                    getattr(calls, n)(*args[:whole], wrong, *args[whole + 1:])
+            assert not seen
+    finally:
+        calls.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names})
