@@ -11,7 +11,7 @@
 // back and taken again in the same call is read from the row that gives it, so that nothing that is read is written by the call, but
 // for the lengths and the stack's count where the caller has them updated in place.
 //
-// Bound: latency at decode sizes (one round trip for the lengths, one for block numbers; 8 requests 4.5 us), 12 bytes written per token for prompts (512
+// Bound: latency at decode sizes (one round trip for the lengths, one for block numbers; 8 requests 3.8 us), 12 bytes written per token for prompts (512
 // requests, room for 200000 tokens 9.2 us). One
 // launch: a CTA per 4096 tokens, each of which makes the sums again (200000 tokens: 20.1 us when a cluster of eight shared them) and then
 // four tokens a thread. What is updated in place is written by the CTA that comes last (a ticket, reset by that CTA; 512 requests 10.1 us with it, 9.2
@@ -23,8 +23,9 @@
 namespace w8a8 {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-static_assert(kPlanThreads == 32 * 32, "a warp adds up the warps' sums");
+// Threads of a CTA: 1024, and 128 where that takes no more than one round (8 requests 3.8 us instead of 4.5).
+constexpr int kPlanThreads = 1024, kPlanFew = 128;
+static_assert(kPlanThreads <= 32 * 32, "a warp adds up the warps' sums");
 constexpr int kPlanBlock = 16;
 constexpr int kPlanMaxBatch = 4096;
 
@@ -56,13 +57,15 @@ __device__ __forceinline__ Sums shfl_up(Sums v, int d) {
     return {__shfl_up_sync(0xffffffffu, v.tokens, d), __shfl_up_sync(0xffffffffu, v.take, d), __shfl_up_sync(0xffffffffu, v.give, d)};
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanParams p) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) plan_blocks_kernel(const PlanParams p) {
+    constexpr int kWarps = THREADS / 32;
     extern __shared__ int plan_smem[];
     int* first_s = plan_smem;                      // [batch + 1] tokens ahead of request b
     int* take_s = first_s + p.batch + 1;           // [batch] blocks taken ahead of it
     int* give_s = take_s + p.batch;                // [batch] blocks given back ahead of it
     int* cached_s = give_s + p.batch;              // [batch]; minus one minus the length where the request ended
-    __shared__ Sums warp_s[kPlanThreads / 32];
+    __shared__ Sums warp_s[kWarps];
     __shared__ Sums run_s;
     __shared__ int bad_s, last_s;
 
@@ -76,7 +79,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
         bad_s = 8;  // the lowest status found (5 comes before all); 8: none
     }
     __syncthreads();
-    for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+    for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
         const int b = b0 + tid;
         Sums mine = {0, 0, 0};
         int cached = 0;
@@ -104,13 +107,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
         __syncthreads();
         const Sums base = run_s;
         if (warp == 0) {
-            Sums w = warp_s[lane];
+            Sums w = {0, 0, 0};
+            if (lane < kWarps) w = warp_s[lane];
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const Sums o = shfl_up(w, d);
                 if (lane >= d) w = w + o;
             }
-            warp_s[lane] = w;
+            if (lane < kWarps) warp_s[lane] = w;
         }
         __syncthreads();
         Sums at = base + inc;
@@ -121,7 +125,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
             give_s[b] = static_cast<int>(at.give - mine.give);
             cached_s[b] = ended ? -1 - cached : cached;
         }
-        if (tid == 0) run_s = base + warp_s[kPlanThreads / 32 - 1];
+        if (tid == 0) run_s = base + warp_s[kWarps - 1];
         __syncthreads();
     }
     if (tid == 0) first_s[0] = 0;
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
     const bool ok = status == 8;
 
     __syncthreads();  // (first_s[0])
-    const int threads = parts * kPlanThreads, me = part * kPlanThreads + tid;
+    const int threads = parts * THREADS, me = part * THREADS + tid;
     // the request that item x of a prefix sum belongs to: the last whose items start at or before it
     auto owner = [&](const int* ahead, int x) {
         int lo = 0, hi = p.batch - 1;
@@ -216,14 +220,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_blocks_kernel(const PlanPar
     } else if (part > 0) {
         return;
     }
-    for (int b = tid; b < p.batch; b += kPlanThreads) {
+    for (int b = tid; b < p.batch; b += THREADS) {
         const int cached = cached_s[b], was = cached < 0 ? -1 - cached : cached;
         p.seq_lens[b] = !ok ? was : cached < 0 ? 0 : cached + first_s[b + 1] - first_s[b];
     }
     if (tid == 0) *p.free_count_out = static_cast<int>(ok ? top - all.take : count);
 }
 
-SmemAttribute plan_attribute;
+SmemAttribute plan_attribute[2];
 constexpr int kPlanSmem = (4 * kPlanMaxBatch + 1) * 4;
 
 }  // namespace
@@ -238,9 +242,10 @@ int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* tabl
                     ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(positions)) & 15u) == 0, ticket};
     const int want = (max_tokens + 4 * kPlanThreads - 1) / (4 * kPlanThreads), sms = device_sms(), parts = want < 1 ? 1 : want < sms ? want : sms;
     if (parts == 1 || (seq_lens != cached && free_count_out != free_count)) p.ticket = nullptr;
+    const bool few = batch <= kPlanFew && max_tokens <= 4 * kPlanFew;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(parts, 1, 1);
-    cfg.blockDim = dim3(kPlanThreads, 1, 1);
+    cfg.blockDim = dim3(few ? kPlanFew : kPlanThreads, 1, 1);
     cfg.dynamicSmemBytes = (4 * batch + 1) * 4;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -248,7 +253,8 @@ int launch_plan_blocks(const int* cached, const int* fresh, int batch, int* tabl
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled(kPdlRow) ? 1 : 0;
-    const cudaError_t e = launch_with_smem(plan_attribute, kPlanSmem, cfg, plan_blocks_kernel, p);
+    const cudaError_t e = few ? launch_with_smem(plan_attribute[0], kPlanSmem, cfg, plan_blocks_kernel<kPlanFew>, p)
+                              : launch_with_smem(plan_attribute[1], kPlanSmem, cfg, plan_blocks_kernel<kPlanThreads>, p);
     if (e != cudaSuccess) return fail(W8A8_ERR_CUDA, "plan_blocks launch: %s", cudaGetErrorString(e));
     return W8A8_OK;
 }

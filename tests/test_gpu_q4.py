@@ -74,6 +74,12 @@ def test_plan_blocks(ctx, B, longest, prompts, prompt, ended, in_place):
     assert run_plan(ctx, *case, tokens, in_place=in_place) == want
 
 
+@pytest.mark.parametrize("B,tokens", [(128, 512), (128, 513), (129, 512), (127, 300)])
+def test_plan_blocks_around_one_round_of_few_threads(ctx, B, tokens):
+    case = plan_case(np.random.default_rng(B + tokens), B, 50, 2, 60, 5)
+    assert run_plan(ctx, *case, tokens) == q4.plan(*case, max_tokens=tokens, capacity=len(case[3]))
+
+
 def test_plan_blocks_odd_addresses_and_no_requests(ctx):
     rng = np.random.default_rng(1)
     case = plan_case(rng, 9, 90, 3, 50, 1)
