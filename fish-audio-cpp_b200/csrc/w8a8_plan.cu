@@ -12,10 +12,10 @@
 // for the lengths and the stack's count where the caller has them updated in place.
 //
 // Bound: latency at decode sizes (one round trip for the lengths, one for block numbers; 8 requests 3.8 us), 12 bytes written per token for prompts (512
-// requests, room for 200000 tokens 9.2 us). One
-// launch: a CTA per 4096 tokens, each of which makes the sums again (200000 tokens: 20.1 us when a cluster of eight shared them) and then
-// four tokens a thread. What is updated in place is written by the CTA that comes last (a ticket, reset by that CTA; 512 requests 10.1 us with it, 9.2
-// without). All or nothing:
+// requests, room for 200000 tokens 7.8 us). One
+// launch: a CTA per 2048 tokens, each of which makes the sums again (200000 tokens: 20.1 us when a cluster of eight shared them) and then
+// four tokens a thread. What is updated in place is written by the CTA that comes last (a ticket, reset by that CTA, which costs 0.9 us
+// at 512 requests). All or nothing:
 // where the blocks, the table's width, the token count or a length do not fit, no request gets anything, and `info` says why.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
@@ -23,8 +23,9 @@
 namespace w8a8 {
 namespace {
 
-// Threads of a CTA: 1024, and 128 where that takes no more than one round (8 requests 3.8 us instead of 4.5).
-constexpr int kPlanThreads = 1024, kPlanFew = 128;
+// Threads of a CTA: 512, and 128 where that takes no more than one round. With 128, 512 and 1024 for 8 requests of a token 3.8, -, 4.5 us; with 256, 512 and
+// 1024 for 64 requests with 4 prompts 6.2, 6.5, 7.1, 512 with room for 200000 tokens 8.0, 7.8, 9.2, 4000 of a token 21.5, 17.3, 16.7.
+constexpr int kPlanThreads = 512, kPlanFew = 128;
 static_assert(kPlanThreads <= 32 * 32, "a warp adds up the warps' sums");
 constexpr int kPlanBlock = 16;
 constexpr int kPlanMaxBatch = 4096;
