@@ -29,6 +29,8 @@
 #include "w8a8_internal.h"
 #include "w8a8_q4.cuh"
 
+#include <cmath>
+
 namespace w8a8 {
 namespace {
 
@@ -59,6 +61,7 @@ struct Kv4Params {
     float* scratch;    // [CTAs][2] pieces
     int* tickets;      // [CTAs], zero between launches
     int* status;
+    float over_grid;  // 1 / CTAs, rounded up
     bool ahead;  // lengths, table and all pages but each sequence's last were complete ahead of the launch ahead
 };
 
@@ -117,6 +120,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+// x / d and what is left, for quotients below 2^20 (x below 2^31): the product with the reciprocal is off by less than a quarter there, the whole
+// number below it by one at most.
+struct Quotient {
+    int q, rest;
+};
+__device__ __forceinline__ Quotient quotient(int x, int d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(static_cast<float>(d)));
+    int q = __float2int_rz(static_cast<float>(x) * r), rest = x - q * d;
+    if (rest < 0) {
+        --q;
+        rest += d;
+    } else if (rest >= d) {
+        ++q;
+        rest -= d;
+    }
+    return {q, rest};
 }
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
@@ -229,6 +250,61 @@ __device__ __noinline__ void merge_pieces(const Kv4Params& p, const float* base,
         finish<R>(p, s, b, kvh, p.n_q / p.n_kv, lane);
 }
 
+// Heads h0 .. h0 + E - 1 of pieces base[i], i in `which`, added and finished, or to the piece `to`. E is one, or the heads of a group of codes. Lane i
+// sees to piece i's weights, so that the loop over the pieces has no chain but its sums. (Four heads by a warp each: 8 x 1024 tokens 11.5 us; all by one
+// warp, piece by piece, 12.0.)
+template <int R, int E>
+__device__ __noinline__ void merge_share(const Kv4Params& p, const float* base, uint32_t which, float* to, int b, int kvh, int h0) {
+    constexpr int kPiece = piece_floats(R);
+    const int lane = threadIdx.x & 31;
+    const bool there = which >> lane & 1;
+    const float* const mine = base + (there ? lane : __ffs(which) - 1) * kPiece + R * kDim + h0;
+    Merged<E> s;
+    s.clear();
+    float w[E];
+#pragma unroll
+    for (int h = 0; h < E; ++h) {
+        const float top_mine = there ? mine[h] : kNoScore, sum = there ? mine[R + h] : 0.0f;
+        float top = top_mine;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        w[h] = exp2_fast(top_mine - top);
+        float part = there ? sum * w[h] : 0.0f;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+        s.l[h] = part;
+        s.m[h] = top;
+    }
+#pragma unroll 4
+    for (; which; which &= which - 1) {
+        const int i = __ffs(which) - 1;
+        const float* const from = base + i * kPiece + h0 * kDim + 4 * lane;
+#pragma unroll
+        for (int h = 0; h < E; ++h) {
+            const float4 a = *reinterpret_cast<const float4*>(from + h * kDim);
+            const float x = __shfl_sync(0xffffffffu, w[h], i);
+            s.acc[h] = {fmaf(a.x, x, s.acc[h].x), fmaf(a.y, x, s.acc[h].y), fmaf(a.z, x, s.acc[h].z), fmaf(a.w, x, s.acc[h].w)};
+        }
+    }
+    const int heads = p.n_q / p.n_kv;
+    if (!to) return finish<E>(p, s, b, (kvh * heads + h0) / E, E, lane);
+#pragma unroll
+    for (int h = 0; h < E; ++h) {
+        reinterpret_cast<float4*>(to + (h0 + h) * kDim)[lane] = s.acc[h];
+        if (lane == 0) {
+            to[R * kDim + h0 + h] = s.m[h];
+            to[R * kDim + R + h0 + h] = s.l[h];
+        }
+    }
+}
+template <int R>
+__device__ __forceinline__ void merge_share(const Kv4Params& p, int each, const float* base, uint32_t which, float* to, int b, int kvh, int share) {
+    if (each == 1) return merge_share<R, 1>(p, base, which, to, b, kvh, share);
+    if (each == 2) return merge_share<R, 2>(p, base, which, to, b, kvh, 2 * share);
+    if (each == 4) return merge_share<R, 4>(p, base, which, to, b, kvh, 4 * share);
+    if constexpr (R == 8) merge_share<R, 8>(p, base, which, to, b, kvh, 8 * share);
+}
+
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 // G groups per head; R the most query heads per kv head (4 or 8); W warps.
 // Twelve warps of 168 registers: with sixteen of 128 the long cases take the same (64 x 4000 tokens 74 us) and the short ones more (8 x 1024 tokens
@@ -300,7 +376,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     // The range is cut by cost: a pair counts kPairCost pages more than it has (its q, its piece, its output; a run of many short pairs would
     // else last longest). Cost v of the range is cost v - of pairs ahead - kPairCost pages into its pair, none where that is negative.
     const int costs = units + kPairCost * p.batch * p.n_kv;
-    const int cta_cost = max(static_cast<int>((costs + gridDim.x - 1) / gridDim.x), 1);
+    const int grid = gridDim.x;
+    int cta_cost = __float2int_ru(__fmul_ru(__int2float_ru(costs), p.over_grid));  // costs / grid or, of many, a few more
+    if (static_cast<long long>(cta_cost - 1) * grid >= costs) --cta_cost;
+    cta_cost = max(cta_cost, 1);
     auto cost_ahead = [&](int b) { return (first_s[b] + kPairCost * b) * p.n_kv; };
     auto last_at = [&](auto ahead, int v) {  // the last sequence b with ahead(b) <= v
         int a = 0, z = p.batch - 1;
@@ -315,8 +394,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         int b, h, in, of;  // cost `in` of `of` of the pair (b, h)
     };
     auto place_of = [&](int v) {
-        const int b = last_at(cost_ahead, v), of = first_s[b + 1] - first_s[b] + kPairCost, rest = v - cost_ahead(b), h = rest / of;
-        return Place{b, h, rest - h * of, of};
+        const int b = last_at(cost_ahead, v), of = first_s[b + 1] - first_s[b] + kPairCost, rest = v - cost_ahead(b);
+        const Quotient x = quotient(rest, of);
+        return Place{b, x.q, x.rest, of};
     };
     // Lanes 0, 1: where the CTA's run begins and ends; lanes 2, 3: the warp's. A CTA's borders are at multiples of cta_cost, but not inside a
     // pair of few pages, which goes to one side or the other as a whole.
@@ -350,7 +430,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         const int i = i0 + lane;
         if (i < n_mine) {
             const int u = lo + i, b = last_at(units_ahead, u);  // (the last of those that start at or before u: empty ones in front of it start there too)
-            const int blocks = first_s[b + 1] - first_s[b], rest = u - units_ahead(b), h = rest / blocks, blk = rest - h * blocks;
+            const int blocks = first_s[b + 1] - first_s[b], rest = u - units_ahead(b);
+            const Quotient x = quotient(rest, blocks);
+            const int h = x.q, blk = x.rest;
             int phys = p.table[static_cast<size_t>(b) * p.max_blocks + blk];
             if (phys < 0 || phys >= p.n_blocks) phys = 0;  // (the caller's mistake; reads stay inside the cache)
             page_of = (phys * p.n_layers + p.layer) * p.n_kv + h;
@@ -364,7 +446,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             bulk_load(ring + (i & (D - 1)) * kPage, p.cache + static_cast<size_t>(static_cast<uint32_t>(page_of)) * kPage, kPage, bar);
         }
     };
+    // the pair at hand, and its q: asked for ahead of the pages, of a later pair ahead of the piece of the one before it
+    const int g8 = lane >> 2, j4 = lane & 3, heads = p.n_q / p.n_kv;
+    int b = n_mine > 0 ? last_at(units_ahead, lo) : 0, blocks = 1, kvh = 0, blk0 = 0;
+    uint4 q_raw[4];
+    auto ask_q = [&](int u) {
+        while (units_ahead(b + 1) <= u) ++b;
+        blocks = first_s[b + 1] - first_s[b];
+        const Quotient x = quotient(u - units_ahead(b), blocks);
+        kvh = x.q;
+        blk0 = x.rest;
+#pragma unroll
+        for (int run = 0; run < 4; ++run) {
+            q_raw[run] = {0, 0, 0, 0};
+            if (g8 < heads) q_raw[run] = ptx::ld_result_v4(p.q + (static_cast<size_t>(b) * p.n_q + kvh * heads + g8) * kDim + 32 * run + 8 * j4);
+        }
+    };
     if (n_mine > 0) {
+        if (!p.ahead) ask_q(lo);
         look_up(0);
         if (p.ahead) {  // a sequence's last page may still be in the making
             const uint32_t later = __ballot_sync(0xffffffffu, newest && lane < min(n_mine, D));
@@ -372,6 +471,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                 if (!(later >> i & 1)) issue(i);
             ptx::pdl_wait();
             for (uint32_t rest = later; rest; rest &= rest - 1) issue(__ffs(rest) - 1);
+            ask_q(lo);
         } else {
             for (int i = 0; i < min(n_mine, D); ++i) issue(i);
         }
@@ -385,14 +485,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         if (first_s[b] == first_s[b + 1])
             for (int h = warp; h < p.n_kv; h += W) merge_pieces<R>(p, pieces, 0u, nullptr, b, h);
 
-    const int g8 = lane >> 2, j4 = lane & 3;
     bool failed = false;
-    int b = n_mine > 0 ? last_at(units_ahead, lo) : 0;
     for (int i = 0; i < n_mine;) {
         // ---- the next pair of the run ----
         const int u0 = lo + i;
-        while (units_ahead(b + 1) <= u0) ++b;
-        const int blocks = first_s[b + 1] - first_s[b], rest = u0 - units_ahead(b), kvh = rest / blocks, blk0 = rest - kvh * blocks;
         const int i_end = min(n_mine, i + blocks - blk0);
         int tokens = min(max(p.lens[b], 0), cap) - blk0 * kTokens;  // from the page's first on
 
@@ -400,14 +496,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         uint32_t qb[4][4];  // [run][channels 0, 4; 1, 5; 2, 6; 3, 7 of the lane's eight]; the odd ones over 16
         float start[G][4];  // of heads 2 j4, 2 j4 + 1, for the tokens of either half
         {
-            const int heads = p.n_q / p.n_kv;
             float sum[G];
 #pragma unroll
             for (int x = 0; x < G; ++x) sum[x] = 0.0f;
 #pragma unroll
             for (int run = 0; run < 4; ++run) {
-                uint4 w = {0, 0, 0, 0};
-                if (g8 < heads) w = ptx::ld_result_v4(p.q + (static_cast<size_t>(b) * p.n_q + kvh * heads + g8) * kDim + 32 * run + 8 * j4);
+                const uint4 w = q_raw[run];
                 const __half2 over16 = as_half2(0x2c002c00u);
                 qb[run][0] = __byte_perm(w.x, w.z, 0x5410);
                 qb[run][1] = as_u32(__hmul2(as_half2(__byte_perm(w.x, w.z, 0x7632)), over16));
@@ -560,7 +654,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         }
 
         // ---- the pair's piece: of a pair that began in front of this run, or that begins in it ----
-        const bool head = blk0 > 0;
+        const bool head = blk0 > 0, whole = !head && lo + i - u0 == blocks;
+        const int this_b = b, this_kvh = kvh;
+        if (i < n_mine) ask_q(lo + i);
         float* const piece = pieces + (2 * warp + (head ? 0 : 1)) * kPiece;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -580,20 +676,23 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             }
         }
         __syncwarp();
-        if (!head && lo + i - u0 == blocks) {  // all of the pair
-            merge_pieces<R>(p, piece, 1u, nullptr, b, kvh);
+        if (whole) {
+            merge_pieces<R>(p, piece, 1u, nullptr, this_b, this_kvh);
             __syncwarp();
         } else if (lane == 0) {
-            piece_pair[2 * warp + (head ? 0 : 1)] = b * p.n_kv + kvh;
+            piece_pair[2 * warp + (head ? 0 : 1)] = this_b * p.n_kv + this_kvh;
         }
     }
     __syncthreads();
 
-    // ---- pieces that meet in the CTA: chains of neighbours of one pair; a warp a chain ----
+    // ---- pieces that meet in the CTA: chains of neighbours of one pair; a warp takes a head of a chain, or the heads of a group of codes ----
+    const int each = p.Xq && p.g > kDim ? p.g / kDim : 1, shares = heads / each;
     auto pair_units = [&](int pair, int& from, int& to) {
-        const int pb = pair / p.n_kv, blocks = first_s[pb + 1] - first_s[pb];
-        from = units_ahead(pb) + (pair - pb * p.n_kv) * blocks;
-        to = from + blocks;
+        const Quotient x = quotient(pair, p.n_kv);
+        const int pages = first_s[x.q + 1] - first_s[x.q];
+        from = units_ahead(x.q) + x.rest * pages;
+        to = from + pages;
+        return x;
     };
     // (lane x of every warp looks at piece x; a chain starts where the piece in front of it is another pair's)
     const int pair_x = lane < 2 * W ? piece_pair[lane] : -1;
@@ -602,20 +701,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     const int pair_before = __shfl_sync(0xffffffffu, pair_x, in_front ? 31 - __clz(in_front) : 0);
     const uint32_t starts = __ballot_sync(0xffffffffu, pair_x >= 0 && (!in_front || pair_before != pair_x));
     int open[2] = {-1, -1};  // pairs that go on in other CTAs: one that began ahead of this CTA's run, one that ends behind it
-    int chain = 0;
+    int task = warp;  // of (chain, share), counted from the chain at hand: this warp's next
 #pragma unroll 1
-    for (uint32_t todo = starts; todo; todo &= todo - 1, ++chain) {
+    for (uint32_t todo = starts; todo; todo &= todo - 1, task -= shares) {
         const int x = __ffs(todo) - 1;
         const uint32_t later = todo & (todo - 1);
         const uint32_t mine = there & (0xffffffffu << x) & (later ? (1u << (__ffs(later) - 1)) - 1 : 0xffffffffu);
         const int pair = __shfl_sync(0xffffffffu, pair_x, x);
         int from, to;
-        pair_units(pair, from, to);
+        const Quotient x_pair = pair_units(pair, from, to);
         const bool whole = from >= cta_lo && to <= cta_hi, before = from < cta_lo;
         if (!whole) open[before ? 0 : 1] = pair;
-        if (chain % W != warp) continue;
-        merge_pieces<R>(p, pieces, mine, whole ? nullptr : p.scratch + (2ll * blockIdx.x + (before ? 0 : 1)) * kPiece,
-                        pair / p.n_kv, pair % p.n_kv);
+        for (; task < shares; task += W)
+            merge_share<R>(p, each, pieces, mine, whole ? nullptr : p.scratch + (2ll * blockIdx.x + (before ? 0 : 1)) * kPiece, x_pair.q, x_pair.rest,
+                                  task);
     }
 
     // ---- pairs that lie in several CTAs: the last of them to come here adds their pieces; half of the warps see to either open pair ----
@@ -627,9 +726,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         const int pair = open[side];
         if (pair >= 0) {
             int from, to;
-            pair_units(pair, from, to);
+            const Quotient x_pair = pair_units(pair, from, to);
             const int first_cost = from + kPairCost * (pair + 1);  // of the pair's first page
-            const int c0 = first_cost / cta_cost, c1 = (first_cost + (to - from) - 1) / cta_cost, n = c1 - c0 + 1;
+            const int c0 = quotient(first_cost, cta_cost).q, c1 = quotient(first_cost + (to - from) - 1, cta_cost).q, n = c1 - c0 + 1;
             auto half_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + side), "n"(kHalf * 32) : "memory"); };
             if (w == 0 && lane == 0) {  // (releases what the CTA's warps stored ahead of the barrier, acquires what the others' released)
                 int before;
@@ -641,7 +740,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             if (last_s[side]) {
                 // pieces in the order of the pages: warp w a run of them, the runs then in order
                 const int run = (n + kHalf - 1) / kHalf, x0 = min(n, w * run), x1 = min(n, x0 + run);
-                float* const mine = pieces + warp * kPiece;
+                float* const sums = pieces + side * kHalf * kPiece;
                 Merged<R> s;
                 s.clear();
                 for (int k = x0; k < x1; ++k) {
@@ -650,10 +749,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                     for (int h = 0; h < R; ++h)
                         s.add(h, __ldcg(reinterpret_cast<const float4*>(piece + h * kDim) + lane), __ldcg(piece + R * kDim + h), __ldcg(piece + R * kDim + R + h));
                 }
-                if (x0 < x1) s.store(mine, lane);
+                if (x0 < x1) s.store(sums + w * kPiece, lane);
                 half_barrier();
-                if (w == 0)
-                    merge_pieces<R>(p, mine, (1u << ((n + run - 1) / run)) - 1, nullptr, pair / p.n_kv, pair % p.n_kv);
+                for (int x = w; x < shares; x += kHalf)
+                    merge_share<R>(p, each, sums, (1u << ((n + run - 1) / run)) - 1, nullptr, x_pair.q, x_pair.rest, x);
             }
         }
     }
@@ -694,9 +793,10 @@ int launch_kv4_attention(const __half* q, const void* cache, int n_blocks, const
     if (batch == 0) return W8A8_OK;
     const int ratio = n_q / n_kv;
     Kv4Params p = {q, static_cast<const unsigned char*>(cache), table, lens, out, Xq, Xs, g, batch, n_q, n_kv, max_blocks, n_blocks, layer, n_layers,
-                   sm_scale * 1.4426950408889634f * 0x1p24f, scratch, tickets, status, ahead};
+                   sm_scale * 1.4426950408889634f * 0x1p24f, scratch, tickets, status, 0.0f, ahead};
     const long long most = static_cast<long long>(batch) * n_kv * max_blocks;  // units, were all sequences as long as their rows
     const int sms = device_sms() < kKv4Tickets ? device_sms() : kKv4Tickets, ctas = most < sms ? static_cast<int>(most) : sms;
+    p.over_grid = std::nextafter(1.0f / static_cast<float>(ctas > 0 ? ctas : 1), 1.0f);
     cudaError_t e;
     if (ratio <= 4)
         e = group == 32 ? launch_kv4<4, 4>(p, ctas, stream) : group == 64 ? launch_kv4<2, 4>(p, ctas, stream) : launch_kv4<1, 4>(p, ctas, stream);
