@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     };
     // Lanes 0, 1: where the CTA's run begins and ends; lanes 2, 3: the warp's. A CTA's borders are at multiples of cta_cost, but not inside a
     // pair of few pages, which goes to one side or the other as a whole.
-    int at_border;
+    int at_border, b_border;  // in pages; the sequence (or one of no pages in front of it)
     {
         const int whole_pages = min(kWholePages, 4 * cta_cost);
         const long long nominal = static_cast<long long>(blockIdx.x + (lane & 1)) * cta_cost;
@@ -414,6 +414,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                 const int from = __shfl_sync(0xffffffffu, v, 0), to = __shfl_sync(0xffffffffu, v, 1);
                 if (lane & 2) v = min(to, from + (warp + (lane & 1)) * ((to - from + W - 1) / W));
             } else {
+                b_border = x.b;
                 v = v < costs ? first_s[x.b] * p.n_kv + x.h * (x.of - kPairCost) + max(0, x.in - kPairCost) : units;
             }
         }
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     };
     // the pair at hand, and its q: asked for ahead of the pages, of a later pair ahead of the piece of the one before it
     const int g8 = lane >> 2, j4 = lane & 3, heads = p.n_q / p.n_kv;
-    int b = n_mine > 0 ? last_at(units_ahead, lo) : 0, blocks = 1, kvh = 0, blk0 = 0;
+    int b = __shfl_sync(0xffffffffu, b_border, 2), blocks = 1, kvh = 0, blk0 = 0;
     uint4 q_raw[4];
     auto ask_q = [&](int u) {
         while (units_ahead(b + 1) <= u) ++b;
@@ -467,12 +468,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         look_up(0);
         if (p.ahead) {  // a sequence's last page may still be in the making
             const uint32_t later = __ballot_sync(0xffffffffu, newest && lane < min(n_mine, D));
+#pragma unroll 1
             for (int i = 0; i < min(n_mine, D); ++i)
                 if (!(later >> i & 1)) issue(i);
             ptx::pdl_wait();
+#pragma unroll 1
             for (uint32_t rest = later; rest; rest &= rest - 1) issue(__ffs(rest) - 1);
             ask_q(lo);
         } else {
+#pragma unroll 1  // (code size: it runs cold)
             for (int i = 0; i < min(n_mine, D); ++i) issue(i);
         }
     } else if (p.ahead) {
