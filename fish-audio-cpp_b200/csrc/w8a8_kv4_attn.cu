@@ -4,7 +4,7 @@
 //   k_t, v_t = code * scale of the row's group; one pass with the running maximum and sum of the softmax, both fp32
 //
 // Bound: HBM and the arithmetic, close to one another. A token costs 128 + 4 G bytes per kv head (K and V; G = 128 / group) instead of the fp16
-// cache's 512; a warp executes some 340 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 77 us, 58 % of
+// cache's 512; a warp executes some 340 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 74 us, 60 % of
 // the measured copy rate; the copies alone, without arithmetic, take 54, the arithmetic alone, without copies, 61 (the scores and the
 // softmax 42 of them, a chain that three warps a scheduler cannot hide). Two pages at a time, one page's scores beside the sum over the page
 // before it, scales folded into p, and 8 or 14 or 16 warps instead of 12 changed nothing or cost time.
@@ -39,9 +39,10 @@ using q4::kTokens;
 
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
-// Pairs of at most so many pages (and at most four times a CTA's share) are not cut between CTAs: a join costs what a warp's six to eight pages
-// cost. us with 32, 96 and 256: 8 x 1024 tokens 13.5, 12.4, 12.4; 64 x 1024 31, 29, 29; 64 x 4000 73, 73, 79; 1 x 1024 10.4 where cut, 11.6 whole.
-constexpr int kWholePages = 96;
+// Pairs of at most kFewPages, and of at most twice a CTA's share up to kWholePages, are not cut between CTAs: a join costs what a warp's two or three
+// pages cost. us whole and cut: 1 x 400 tokens 7.3 and 8.3, 8 x 400 8.0 and 9.5, 16 x 1024 11.5 and 13.1; 8 x 1024 11.3 and 11.0, 8 x 1500 13.8 and
+// 12.0 (more than twice a share); 64 x 4000 79 and 73 (whole up to 256 pages, and up to 96).
+constexpr int kFewPages = 32, kWholePages = 96;
 // Pages that a pair counts for beyond its own. us with 0, 2, 4 and 8: 48 ragged sequences up to 8000 tokens 34, 23.5, 23.2, 23.4; 200 up to 2000
 // tokens 50, 31.7, 32.1, 35.1; 64 x 512 20.5, 21.1, 21.3, 22.0.
 constexpr int kPairCost = 3;
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     // pair of few pages, which goes to one side or the other as a whole.
     int at_border, b_border;  // in pages; the sequence (or one of no pages in front of it)
     {
-        const int whole_pages = min(kWholePages, 4 * cta_cost);
+        const int whole_pages = min(kWholePages, max(2 * cta_cost, kFewPages));
         const long long nominal = static_cast<long long>(blockIdx.x + (lane & 1)) * cta_cost;
         int v = static_cast<int>(min(nominal, static_cast<long long>(costs)));
 #pragma unroll 1
