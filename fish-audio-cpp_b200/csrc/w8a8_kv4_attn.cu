@@ -39,9 +39,9 @@ using q4::kTokens;
 
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
-// Pairs of at most kFewPages, and of at most twice a CTA's share up to kWholePages, are not cut between CTAs: a join costs what a warp's two or three
-// pages cost. us whole and cut: 1 x 400 tokens 7.3 and 8.3, 8 x 400 8.0 and 9.5, 16 x 1024 11.5 and 13.1; 8 x 1024 11.3 and 11.0, 8 x 1500 13.8 and
-// 12.0 (more than twice a share); 64 x 4000 79 and 73 (whole up to 256 pages, and up to 96).
+// Pairs of at most kFewPages, and of at most twice a CTA's share (with eight heads, whose pieces are twice as long, four times) up to kWholePages, are not
+// cut between CTAs: a join costs what a warp's two or three pages cost. us whole and cut: 1 x 400 tokens 7.3 and 8.3, 8 x 400 8.0 and 9.5, 16 x 1024 11.5 and 13.1; 8 x 1024 11.3 and 11.0, 8 x 1500 13.8 and
+// 12.0 (more than twice a share), with eight heads 8 x 1024 11.7 and 13.1; 64 x 4000 79 and 73 (whole up to 256 pages, and up to 96).
 constexpr int kFewPages = 32, kWholePages = 96;
 // Pages that a pair counts for beyond its own. us with 0, 2, 4 and 8: 48 ragged sequences up to 8000 tokens 34, 23.5, 23.2, 23.4; 200 up to 2000
 // tokens 50, 31.7, 32.1, 35.1; 64 x 512 20.5, 21.1, 21.3, 22.0.
@@ -382,8 +382,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     if (static_cast<long long>(cta_cost - 1) * grid >= costs) --cta_cost;
     cta_cost = max(cta_cost, 1);
     auto cost_ahead = [&](int b) { return (first_s[b] + kPairCost * b) * p.n_kv; };
-    auto last_at = [&](auto ahead, int v) {  // the last sequence b with ahead(b) <= v
-        int a = 0, z = p.batch - 1;
+    auto last_at = [&](auto ahead, int v, int a) {  // the last sequence b >= a with ahead(b) <= v, where a is one: most often a
+        int z = p.batch - 1;
+        if (ahead(min(a + 1, z)) > v) z = a;
 #pragma unroll 1
         while (a < z) {
             const int mid = (a + z + 1) >> 1;
@@ -394,8 +395,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     struct Place {
         int b, h, in, of;  // cost `in` of `of` of the pair (b, h)
     };
-    auto place_of = [&](int v) {
-        const int b = last_at(cost_ahead, v), of = first_s[b + 1] - first_s[b] + kPairCost, rest = v - cost_ahead(b);
+    auto place_of = [&](int v, int a) {
+        const int b = last_at(cost_ahead, v, a), of = first_s[b + 1] - first_s[b] + kPairCost, rest = v - cost_ahead(b);
         const Quotient x = quotient(rest, of);
         return Place{b, x.q, x.rest, of};
     };
@@ -403,16 +404,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     // pair of few pages, which goes to one side or the other as a whole.
     int at_border, b_border;  // in pages; the sequence (or one of no pages in front of it)
     {
-        const int whole_pages = min(kWholePages, max(2 * cta_cost, kFewPages));
+        const int whole_pages = min(kWholePages, max(R / 2 * cta_cost, kFewPages));
         const long long nominal = static_cast<long long>(blockIdx.x + (lane & 1)) * cta_cost;
-        int v = static_cast<int>(min(nominal, static_cast<long long>(costs)));
+        int v = static_cast<int>(min(nominal, static_cast<long long>(costs))), a = 0;
 #pragma unroll 1
         for (int step = 0; step < 2; ++step) {  // (two rounds through one copy of the code: the CTA's borders, then all four in pages)
             Place x = {0, 0, 0, kPairCost};
-            if (v < costs) x = place_of(v);
+            if (v < costs) x = place_of(v, a);
             if (step == 0) {
                 if (v < costs && x.of - kPairCost <= whole_pages) v += 2 * x.in < x.of ? -x.in : x.of - x.in;
                 const int from = __shfl_sync(0xffffffffu, v, 0), to = __shfl_sync(0xffffffffu, v, 1);
+                a = __shfl_sync(0xffffffffu, x.b, 0);  // (no border of the CTA's lies in front of its first one's sequence)
                 if (lane & 2) v = min(to, from + (warp + (lane & 1)) * ((to - from + W - 1) / W));
             } else {
                 b_border = x.b;
@@ -426,12 +428,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     auto units_ahead = [&](int b) { return first_s[b] * p.n_kv; };
 
     const uint32_t ring = ptx::smem_u32(ring_all) + warp * (D * kPage);
+    const int first_b = __shfl_sync(0xffffffffu, b_border, 2);  // at or in front of the run's first sequence
     int page_of = 0;     // the page's number in the cache of unit (i & ~31) + lane of the run
     bool newest = false;  // it is its sequence's last
     auto look_up = [&](int i0) {
         const int i = i0 + lane;
         if (i < n_mine) {
-            const int u = lo + i, b = last_at(units_ahead, u);  // (the last of those that start at or before u: empty ones in front of it start there too)
+            const int u = lo + i, b = last_at(units_ahead, u, first_b);  // (the last of those that start at or before u: empty ones in front of it start there too)
             const int blocks = first_s[b + 1] - first_s[b], rest = u - units_ahead(b);
             const Quotient x = quotient(rest, blocks);
             const int h = x.q, blk = x.rest;
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     };
     // the pair at hand, and its q: asked for ahead of the pages, of a later pair ahead of the piece of the one before it
     const int g8 = lane >> 2, j4 = lane & 3, heads = p.n_q / p.n_kv;
-    int b = __shfl_sync(0xffffffffu, b_border, 2), blocks = 1, kvh = 0, blk0 = 0;
+    int b = first_b, blocks = 1, kvh = 0, blk0 = 0;
     uint4 q_raw[4];
     auto ask_q = [&](int u) {
         while (units_ahead(b + 1) <= u) ++b;
