@@ -384,9 +384,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     auto cost_ahead = [&](int b) { return (first_s[b] + kPairCost * b) * p.n_kv; };
     auto last_at = [&](auto ahead, int v, int a) {  // the last sequence b >= a with ahead(b) <= v, where a is one: most often a
         int z = p.batch - 1;
-        if (ahead(min(a + 1, z)) > v) z = a;
+        if (a >= z || ahead(a + 1) > v) return a;
 #pragma unroll 1
-        while (a < z) {
+        for (++a; a < z;) {
             const int mid = (a + z + 1) >> 1;
             if (ahead(mid) <= v) a = mid; else z = mid - 1;
         }
