@@ -233,22 +233,20 @@ __device__ __forceinline__ void finish(const Kv4Params& p, const Merged<R>& s, i
     }
 }
 
-// Pieces base[i] (in shared memory), i in `which`, added in order: to `to`, or finished. One copy of this code: it runs cold.
+// A pair that is one piece, or none (no tokens). One copy of this code: it runs cold.
 template <int R>
-__device__ __noinline__ void merge_pieces(const Kv4Params& p, const float* base, uint32_t which, float* to, int b, int kvh) {
+__device__ __noinline__ void finish_whole(const Kv4Params& p, const float* piece, int b, int kvh) {
     const int lane = threadIdx.x & 31;
     Merged<R> s;
     s.clear();
-#pragma unroll 1
-    for (; which; which &= which - 1) {
-        const float* piece = base + (__ffs(which) - 1) * piece_floats(R);
+    if (piece) {
 #pragma unroll
-        for (int h = 0; h < R; ++h) s.add(h, reinterpret_cast<const float4*>(piece + h * kDim)[lane], piece[R * kDim + h], piece[R * kDim + R + h]);
+        for (int h = 0; h < R; ++h) {
+            s.acc[h] = reinterpret_cast<const float4*>(piece + h * kDim)[lane];
+            s.l[h] = piece[R * kDim + R + h];
+        }
     }
-    if (to)
-        s.store(to, lane);
-    else
-        finish<R>(p, s, b, kvh, p.n_q / p.n_kv, lane);
+    finish<R>(p, s, b, kvh, p.n_q / p.n_kv, lane);
 }
 
 // Heads h0 .. h0 + E - 1 of pieces base[i], i in `which`, added and finished, or to the piece `to`. E is one, or the heads of a group of codes. Lane i
@@ -491,7 +489,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
     // rows of no tokens: zeros
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
         if (first_s[b] == first_s[b + 1])
-            for (int h = warp; h < p.n_kv; h += W) merge_pieces<R>(p, pieces, 0u, nullptr, b, h);
+            for (int h = warp; h < p.n_kv; h += W) finish_whole<R>(p, nullptr, b, h);
 
     bool failed = false;
     for (int i = 0; i < n_mine;) {
@@ -685,7 +683,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         }
         __syncwarp();
         if (whole) {
-            merge_pieces<R>(p, piece, 1u, nullptr, this_b, this_kvh);
+            finish_whole<R>(p, piece, this_b, this_kvh);
             __syncwarp();
         } else if (lane == 0) {
             piece_pair[2 * warp + (head ? 0 : 1)] = this_b * p.n_kv + this_kvh;
