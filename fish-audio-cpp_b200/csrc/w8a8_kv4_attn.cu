@@ -23,8 +23,8 @@
 // accumulator's start, -8 * sum of q over the group. Sums are fp32 per group, times the group's scale in fp32. P V: codes as fp16 numbers
 // (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p as two fp16 numbers, the
 // rounded one and what that left, which costs nothing here (77.3 and 77.1 us) and takes the error from 3.3e-4 of the output to 2.6e-4,
-// of which the output's own rounding is 2.1e-4; products are summed in fp32. The reference of the exponentials is a score of the
-// row that others exceed by at most 2^kLag, so that it moves, and the sums with it, a few times per row only.
+// of which the output's own rounding is 2.1e-4; products are summed in fp32. The reference of the exponentials lies below the row's largest score and moves, and the
+// sums with it, when a weight passes 2^kTop: a few times per row only.
 #include "sm100_ptx.cuh"
 #include "w8a8_internal.h"
 #include "w8a8_q4.cuh"
@@ -46,7 +46,11 @@ constexpr int kFewPages = 32, kWholePages = 96;
 // Pages that a pair counts for beyond its own. us with 0, 2, 4 and 8: 48 ragged sequences up to 8000 tokens 34, 23.5, 23.2, 23.4; 200 up to 2000
 // tokens 50, 31.7, 32.1, 35.1; 64 x 512 20.5, 21.1, 21.3, 22.0.
 constexpr int kPairCost = 3;
-constexpr float kLag = 8.0f;  // p is at most 2^8: it keeps its precision in fp16
+// The largest weight of a warp's pages so far stands between 2^kAt and 2^kTop, at the upper end of fp16: what a weight as two fp16 numbers loses is 2^-22 of itself
+// or 2^-25, so a key that takes nearly all the weight leaves the others what they have down to 2^-36 of it. (With weights of up to one, others below
+// 2^-25 were gone, which is all of the output where that key's value is small.) us for 2 x 131000 tokens and 64 heads over 8 x 1024 with kAt = 7, 10, 12, 13:
+// 74.1, 74.1, 74.3, 74.5 and 11.3, 11.4, 11.5, 11.6.
+constexpr float kTop = 15.0f, kAt = 11.0f;
 
 struct Kv4Params {
     const __half* q;  // [batch, n_q, 128]
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                 for (int e = 0; e < 4; ++e) y[e] = g8 + 4 * (e & 2) < tokens ? fmaf(sc[e], p.scale_log2, -m_run[e & 1]) : -INFINITY;
             };
             relative();
-            if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kLag)) {
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kTop)) {
                 const float before[2] = {m_run[0], m_run[1]};
                 m_run[0] = m_run[1] = 0.0f;
                 relative();
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
                     float mx = fmaxf(y[e], y[2 + e]);
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    m_run[e] = fmaxf(before[e], mx);
+                    m_run[e] = fmaxf(before[e], mx - kAt);
                     const float corr = exp2_fast(before[e] - m_run[e]);
                     l_run[e] *= corr;
 #pragma unroll

@@ -355,8 +355,8 @@ W8A8_API int w8a8_kv4_read(w8a8_ctx* ctx, const void* cache, int n_blocks, const
 /* w8a8_paged_attention_decode over this cache: q fp16 [batch, n_heads, head_dim], 1 to 8 query heads per kv head, batch <= 4096, any
  * mix of lengths (a row of length 0 gives zeros). Lengths are cut at 16 * max_blocks_per_seq; a block number outside the cache reads
  * block 0. out fp16 [batch, n_heads, head_dim] and / or its codes Xq and scales Xs as there, quant_group_size a power of two from 4 up
- * that divides (n_heads / n_kv_heads) * head_dim. Sums are fp32; code * scale of V is rounded to fp16. Results do not depend on
- * timing. Needs w8a8_kv4_attention_workspace_bytes of the context's workspace. */
+ * that divides (n_heads / n_kv_heads) * head_dim. Sums are fp32; code * scale of V is rounded to fp16; the weights of the softmax
+ * are held to 2^-22 of themselves or 2^-36 of the row's largest. Results do not depend on timing. Needs w8a8_kv4_attention_workspace_bytes of the context's workspace. */
 W8A8_API size_t w8a8_kv4_attention_workspace_bytes(int n_heads, int n_kv_heads);
 W8A8_API int w8a8_kv4_attention_decode(w8a8_ctx* ctx, const void* q, const void* cache, int n_blocks, const int* block_table,
                               const int* seq_lens, void* out, int batch, int n_heads, int head_dim,

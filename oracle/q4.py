@@ -106,6 +106,55 @@ def attention(q, pages, table, lens, layer, sm_scale, g):
     return out, tol
 
 
+# A weight of the softmax is held as two fp16 numbers relative to a reference that leaves the largest weight of a run of pages at 2^11 or more.
+WEIGHTS_AT = 2.0**11
+
+
+def attention_bound(q, pages, table, lens, layer, sm_scale, g, sms=148):
+    """The same output with a bound for every element, from the row's own weights. With w_t = exp(s_t - max), D = sum w_t:
+
+    * a score moves by at most d_t = 136 2^-24 sum |q k| sm + 2^-21 (1 + max |s|) (128 products and four scaled group sums in fp32, the scaling, the
+      exponential), and with it its weight in numerator and denominator: sum w_t (e^d_t - 1) (|v_t| + |out|);
+    * the denominator adds up the fp32 weights, the numerator takes them as two fp16 numbers: 2^-22 relative, or half a subnormal step where
+      the largest weight is 2^11: sum max(2^-22 w_t, 2^-36) |v_t|;
+    * code * scale of V is rounded to fp16: sum w_t (2^-11 |v_t| + 2^-25);
+    * fp32 sums: two multiplies a page of a warp's run, each off by at most 2^-21 of what it adds up (seventeen terms, cut at the last place of the
+      largest), and less than 64 sums where pieces meet, for the numerator; one sum a page and those, 2^-23 each, for the denominator. A run is at most a
+      twelfth of a CTA's share of all pages, each pair counting three more, and of a pair of 96 pages kept whole;
+    * the quotient and its rounding: (2^-22 + 2^-11) |out| + 2^-25.
+    All of it over D but the last, and a hundredth more for products of these."""
+    B, H, _ = q.shape
+    n_kv = pages.shape[2]
+    ratio = H // n_kv
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    q64 = q.astype(np.float64)
+    in_use = [(max(int(n), 0) + 15) // 16 for n in lens]
+    share = (sum(in_use) + 3 * B) * n_kv / sms
+    for b in range(B):
+        n = int(lens[b])
+        if n <= 0:
+            continue
+        run = min(in_use[b], (share + 97) / 12 + 2)
+        K, V = open_pages(pages[table[b, :in_use[b]], layer], g)  # [blocks, n_kv, 16, 128]
+        K = K.transpose(1, 0, 2, 3).reshape(n_kv, -1, DIM)[:, :n]
+        V = V.transpose(1, 0, 2, 3).reshape(n_kv, -1, DIM)[:, :n]
+        for h in range(H):
+            k, v = K[h // ratio], V[h // ratio]
+            s = k @ q64[b, h] * sm_scale
+            w = np.exp(s - s.max())
+            total, size = w.sum(), np.abs(v)
+            out[b, h] = w @ v / total
+            d = 136 * 2.0**-24 * (np.abs(k) @ np.abs(q64[b, h])) * abs(sm_scale) + 2.0**-21 * (1 + np.abs(s).max())
+            moved = w * np.expm1(d)
+            weighted = w @ size
+            e = moved @ size + moved.sum() * np.abs(out[b, h])
+            e += np.maximum(2.0**-22 * w, 2.0**-25 / WEIGHTS_AT) @ size
+            e += 2.0**-11 * weighted + 2.0**-25 * total
+            e += (2 * run + 64) * 2.0**-21 * weighted + (run + 64) * 2.0**-23 * total * np.abs(out[b, h])
+            tol[b, h] = 1.01 * (e / total + (2.0**-22 + 2.0**-11) * (np.abs(out[b, h]) + e / total)) + 2.0**-25
+    return out, tol
+
+
 # ---- the step plan ----
 def plan(cached, new, table, free, count, max_tokens, capacity):
     """What w8a8_plan_blocks leaves, from Python lists: a dict of lists."""

@@ -1,0 +1,74 @@
+"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import q4
+
+pytestmark = pytest.mark.gpu
+
+D, BS = 128, 16
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------
+
+
+def paged(rng, rows_k, rows_v, group):
+    """fp16 rows [tokens, n_kv, 128] of every sequence -> (pages with one layer in a shuffled order, table, lengths)."""
+    lens = [len(k) for k in rows_k]
+    used = [(n + BS - 1) // BS for n in lens]
+    n_kv = rows_k[0].shape[1]
+    perm = rng.permutation(sum(used) + 3)
+    pages = np.full((len(perm), 1, n_kv, q4.page_bytes(group)), 255, np.uint8)
+    table = np.full((len(lens), max(max(used), 1)), -1, np.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        table[b, :used[b]] = perm[at:at + used[b]]
+        at += used[b]
+        padded = [np.zeros((used[b] * BS, n_kv, D), np.float16) for _ in range(2)]
+        for x, rows in zip(padded, (rows_k[b], rows_v[b])):
+            x[:n] = rows
+        if n:
+            pages[table[b, :used[b]], 0] = q4.fill_pages(*(x.reshape(-1, BS, n_kv, D).transpose(0, 2, 1, 3) for x in padded), group)
+    return pages, table, np.array(lens, np.int32)
+
+
+def run_attention(ctx, q, pages, table, lens, group, sm):
+    B, n_q, _ = q.shape
+    out = torch.full((B, n_q, D), 9.0, dtype=torch.float16, device="cuda")
+    ctx.kv4_attention_decode(dev(q), dev(pages), len(pages), dev(table), dev(lens), out, B, n_q, D, table.shape[1], sm, 0, 1, pages.shape[2], group)
+    torch.cuda.synchronize()
+    ctx.check_device_status()
+    return out.cpu().numpy().astype(np.float64)
+
+
+def check_attention(ctx, q, pages, table, lens, group, sm):
+    want, tol = q4.attention_bound(q, pages, table, lens, 0, sm, group)
+    got = run_attention(ctx, q, pages, table, lens, group, sm)
+    assert np.isfinite(got).all()
+    worst = (np.abs(got - want) / (tol + 2.0**-40)).max()
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("below", [20.3, 23.5, 25.2, 27.0, 29.5])
+@pytest.mark.parametrize("n,B", [(40000, 1), (3000, 1), (12000, 24)])
+def test_kv4_attention_keeps_the_tail_behind_one_dominant_key(ctx, n, B, below):
+    """One key takes the weight and has a value of zero; all others weigh 2^-below of it and have values of one: together they are the output.
+    The warp that holds that key holds more of the pages the more sequences there are."""
+    rng = np.random.default_rng(n)
+    group, sm = 32, 1 / math.sqrt(D)
+    for at in (0, 17, n - 1):
+        K, V = np.zeros((n, 1, D), np.float16), np.ones((n, 1, D), np.float16)
+        K[at, 0, 0] = 4.0
+        V[at] = 0
+        q = np.zeros((B, 4, D), np.float16)
+        q[:, :, 0] = below * math.log(2) / (4 * sm)
+        q[:, 2, 0] *= 0.75
+        pages, table, lens = paged(rng, [K], [V], group)
+        check_attention(ctx, q, pages, np.repeat(table, B, 0), np.repeat(lens, B), group, sm)  # (the sequences share their pages)
