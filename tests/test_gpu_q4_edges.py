@@ -1,4 +1,4 @@
-"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest."""
+"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, pages that must not be lost."""
 import math
 
 import numpy as np
@@ -72,3 +72,32 @@ def test_kv4_attention_keeps_the_tail_behind_one_dominant_key(ctx, n, B, below):
         q[:, 2, 0] *= 0.75
         pages, table, lens = paged(rng, [K], [V], group)
         check_attention(ctx, q, pages, np.repeat(table, B, 0), np.repeat(lens, B), group, sm)  # (the sequences share their pages)
+
+
+def pages_in_channels(n, n_kv):
+    """Values that show which pages were added up: page i is one in channel 128 i / pages (times a sign per kv head), zero elsewhere."""
+    V = np.zeros((n, n_kv, D), np.float16)
+    pages = (n + BS - 1) // BS
+    V[np.arange(n), :, np.arange(n) // BS * D // pages] = 1 - 2 * (np.arange(n_kv) % 2)
+    return V
+
+
+@pytest.mark.parametrize("n_q,n_kv,lens,group", [(4, 1, [40000], 64), (8, 1, [9000, 20000], 32), (16, 4, [12345, 1, 0, 30000], 128), (4, 4, [17000], 32),
+                                                 (32, 8, [1024] * 8, 32), (32, 8, [1500, 40, 700], 64), (64, 8, [1024] * 8, 32)])
+def test_kv4_attention_adds_up_every_page(ctx, n_q, n_kv, lens, group):
+    rng = np.random.default_rng(n_q + lens[0])
+    rows_k = [rng.standard_normal((n, n_kv, D)).astype(np.float16) for n in lens]
+    q = rng.standard_normal((len(lens), n_q, D)).astype(np.float16)
+    pages, table, n = paged(rng, rows_k, [pages_in_channels(m, n_kv) for m in lens], group)
+    for _ in range(2):
+        check_attention(ctx, q, pages, table, n, group, 1 / math.sqrt(D))
+
+
+@pytest.mark.parametrize("n_q,n_kv,lens,group", [(4, 1, [40000], 64), (8, 2, [5, 300, 0, 1000, 16, 31], 32), (16, 4, [12345, 1, 30000], 128), (32, 8, [1024] * 4, 32)])
+def test_kv4_attention_within_what_the_weights_allow(ctx, n_q, n_kv, lens, group):
+    rng = np.random.default_rng(n_q + lens[0] + 1)
+    gain = np.where(rng.random(D) < 0.06, 4.0, 1.0)
+    rows_k = [(rng.standard_normal((n, n_kv, D)) * gain).astype(np.float16) for n in lens]
+    rows_v = [rng.standard_normal((n, n_kv, D)).astype(np.float16) for n in lens]
+    q = rng.standard_normal((len(lens), n_q, D)).astype(np.float16)
+    check_attention(ctx, q, *paged(rng, rows_k, rows_v, group), group, 1 / math.sqrt(D))
