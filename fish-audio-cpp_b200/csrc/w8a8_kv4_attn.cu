@@ -19,7 +19,8 @@
 // pairs; nothing in the steady state synchronises warps.
 //
 // Arithmetic. Scores: a masked nibble is, as the bits of an fp16 number, the subnormal code * 2^-24 (or, four bits up, code * 2^-20, which
-// meets a q that was divided by 16: below 2^-10 that rounds by 2^-25), exact as a matrix operand: one instruction for two codes. The 8 that stored codes carry leaves with the
+// meets a q of a sixteenth), exact as a matrix operand: one instruction for two codes. Where a head's q stays below 512 the other channels take it sixteen times instead, so
+// that nothing of a small q is lost; above, what a sixteenth rounds by is 2^-21 beside a q of 2^9. The 8 that stored codes carry leaves with the
 // accumulator's start, -8 * sum of q over the group. Sums are fp32 per group, times the group's scale in fp32. P V: codes as fp16 numbers
 // (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p as two fp16 numbers, the
 // rounded one and what that left, which costs nothing here (77.3 and 77.1 us) and takes the error from 3.3e-4 of the output to 2.6e-4,
@@ -503,20 +504,29 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
         int tokens = min(max(p.lens[b], 0), cap) - blk0 * kTokens;  // from the page's first on
 
         // q of head g8 (nothing in columns without a head), the channels in the order of the K words; the start of the sums
-        uint32_t qb[4][4];  // [run][channels 0, 4; 1, 5; 2, 6; 3, 7 of the lane's eight]; the odd ones over 16
+        uint32_t qb[4][4];  // [run][channels 0, 4; 1, 5; 2, 6; 3, 7 of the lane's eight]; the odd ones a sixteenth of the even ones
         float start[G][4];  // of heads 2 j4, 2 j4 + 1, for the tokens of either half
+        float to_log2[2];   // of these heads: what takes their raw scores to powers of two
         {
+            uint32_t both = 0;  // bits 14 and 30: the two highest bits of a channel's exponent are set, it is 512 or more (or no number)
+#pragma unroll
+            for (int run = 0; run < 4; ++run)
+                both |= (q_raw[run].x & q_raw[run].x << 1) | (q_raw[run].y & q_raw[run].y << 1) | (q_raw[run].z & q_raw[run].z << 1) | (q_raw[run].w & q_raw[run].w << 1);
+            const uint32_t large = __ballot_sync(0xffffffffu, (both & 0x40004000u) != 0);
+            const bool mine = (large >> (lane & 28) & 15) != 0;
+            const __half2 even_by = as_half2(mine ? 0x3c003c00u : 0x4c004c00u), odd_by = as_half2(mine ? 0x2c002c00u : 0x3c003c00u);  // 1 or 16; 1 / 16 or 1
+#pragma unroll
+            for (int e = 0; e < 2; ++e) to_log2[e] = p.scale_log2 * ((large >> (8 * j4 + 4 * e) & 15) != 0 ? 1.0f : 0.0625f);
             float sum[G];
 #pragma unroll
             for (int x = 0; x < G; ++x) sum[x] = 0.0f;
 #pragma unroll
             for (int run = 0; run < 4; ++run) {
                 const uint4 w = q_raw[run];
-                const __half2 over16 = as_half2(0x2c002c00u);
-                qb[run][0] = __byte_perm(w.x, w.z, 0x5410);
-                qb[run][1] = as_u32(__hmul2(as_half2(__byte_perm(w.x, w.z, 0x7632)), over16));
-                qb[run][2] = __byte_perm(w.y, w.w, 0x5410);
-                qb[run][3] = as_u32(__hmul2(as_half2(__byte_perm(w.y, w.w, 0x7632)), over16));
+                qb[run][0] = as_u32(__hmul2(as_half2(__byte_perm(w.x, w.z, 0x5410)), even_by));
+                qb[run][1] = as_u32(__hmul2(as_half2(__byte_perm(w.x, w.z, 0x7632)), odd_by));
+                qb[run][2] = as_u32(__hmul2(as_half2(__byte_perm(w.y, w.w, 0x5410)), even_by));
+                qb[run][3] = as_u32(__hmul2(as_half2(__byte_perm(w.y, w.w, 0x7632)), odd_by));
                 float even = 0.0f, odd = 0.0f;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             const uint32_t page = ring + (i & (D - 1)) * kPage;
 
             // ---- scores: tokens g8, g8 + 8 of heads 2 j4, 2 j4 + 1 ----
-            float sc[4];  // raw: times scale_log2 they are in powers of two
+            float sc[4];  // raw: times to_log2 they are in powers of two
             {
                 uint32_t k0[4], k1[4], s0[G], s1[G];
                 lds_words<4>(k0, page + g8 * 64 + j4 * 16);
@@ -602,7 +612,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) kv4_attention_kernel(const __g
             float y[4];
             auto relative = [&] {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = g8 + 4 * (e & 2) < tokens ? fmaf(sc[e], p.scale_log2, -m_run[e & 1]) : -INFINITY;
+                for (int e = 0; e < 4; ++e) y[e] = g8 + 4 * (e & 2) < tokens ? fmaf(sc[e], to_log2[e & 1], -m_run[e & 1]) : -INFINITY;
             };
             relative();
             if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kTop)) {

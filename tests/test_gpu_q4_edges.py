@@ -1,4 +1,4 @@
-"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, pages that must not be lost."""
+"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost."""
 import math
 
 import numpy as np
@@ -72,6 +72,19 @@ def test_kv4_attention_keeps_the_tail_behind_one_dominant_key(ctx, n, B, below):
         q[:, 2, 0] *= 0.75
         pages, table, lens = paged(rng, [K], [V], group)
         check_attention(ctx, q, pages, np.repeat(table, B, 0), np.repeat(lens, B), group, sm)  # (the sequences share their pages)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("size", [2.0**-24, 2.0**-17, 2.0**-13, 2.0**-9, 1.0, 2.0**9, 2.0**12])
+def test_kv4_attention_queries_of_any_size(ctx, size, group):
+    """The scale of the scores takes out what q is multiplied by, so that they are alike; heads of other sizes beside them."""
+    rng = np.random.default_rng(group)
+    lens = [900, 33, 1]
+    rows = [[rng.standard_normal((n, 2, D)).astype(np.float16) for n in lens] for _ in range(2)]
+    q = np.clip(rng.standard_normal((3, 8, D)) * size, -65504, 65504)
+    q[:, 1] *= 2.0**-3
+    q[:, 6] *= 2.0**2
+    check_attention(ctx, np.clip(q, -65504, 65504).astype(np.float16), *paged(rng, *rows, group), group, 0.1 / size)
 
 
 def pages_in_channels(n, n_kv):
