@@ -1,4 +1,4 @@
-"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost."""
+"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost, several tiles a CTA."""
 import math
 
 import numpy as np
@@ -114,3 +114,55 @@ def test_kv4_attention_within_what_the_weights_allow(ctx, n_q, n_kv, lens, group
     rows_v = [rng.standard_normal((n, n_kv, D)).astype(np.float16) for n in lens]
     q = rng.standard_normal((len(lens), n_q, D)).astype(np.float16)
     check_attention(ctx, q, *paged(rng, rows_k, rows_v, group), group, 1 / math.sqrt(D))
+
+
+# ---- linear --------------------------------------------------------------------------------------------------------
+
+
+def part_of(g):
+    """Channels that are promoted together: 256, 128, 64 or 32, the largest that divides the group's size."""
+    return next(p for p in (256, 128, 64, 32) if g % p == 0)
+
+
+@pytest.mark.parametrize("M", [1, 8, 16, 32])
+@pytest.mark.parametrize("N,K,g", [(4752, 512, 64), (4760, 2560, 256), (9736, 2592, 32), (9728, 2560, 128), (9736, 1056, 96), (19456, 2560, 64), (19456, 512, 256),
+                                   (40000, 2560, 256), (40000, 544, 544)])
+def test_linear4_several_tiles_a_cta(ctx, M, N, K, g):
+    """Two and many tiles a CTA, of several boxes each: runs that cross tiles, tiles that several warps share, with each epilogue. Sums of fp32 parts: (parts + 16
+    warps + 3) 2^-24 of the magnitudes; every rounding to fp16 2^-11; silu' is at most 1.1."""
+    gen = torch.Generator(device="cuda").manual_seed(M + N + K + g)
+    G = (K + g - 1) // g
+    codes = torch.randint(-8, 8, (N, K), generator=gen, device="cuda", dtype=torch.int8)
+    scale = (torch.rand((N, G), generator=gen, device="cuda") * 4e-3 + 1e-3).half()
+    x = torch.randint(-127, 128, (M, K), generator=gen, device="cuda", dtype=torch.int8)
+    xs = torch.rand((M, G), generator=gen, device="cuda") * 0.045 + 0.005
+    W = (codes[:, 0::2] & 15 | codes[:, 1::2] << 4).view(torch.uint8).contiguous()
+    y, mag = (torch.zeros((M, N), dtype=torch.float64, device="cuda") for _ in range(2))
+    starts = range(0, K, part_of(g))
+    for k in starts:
+        at, i = slice(k, min(K, k + part_of(g))), k // g
+        term = x[:, at].double() @ codes[:, at].double().T * scale[:, i].double() * xs[:, i:i + 1].double()  # (whole numbers below 2^53: exact)
+        y, mag = y + term, mag + term.abs()
+    err, half = (len(starts) + 19) * 2.0**-24 * mag, 2.0**-11
+    residual = torch.randn((M, N), generator=gen, device="cuda").half()
+    for epilogue in (0, 1, 2):
+        if epilogue == 2 and N % 16:
+            continue
+        out = torch.full((M + 1, N // 2 if epilogue == 2 else N), 7.0, dtype=torch.float16, device="cuda")
+        ctx.linear4_q(W, scale, g, x, xs, out, M, N, K, epilogue=epilogue, residual=residual if epilogue == 1 else None)
+        torch.cuda.synchronize()
+        assert (out[M] == 7).all()
+        if epilogue == 2:
+            (gate, up), (eg, eu) = (a.view(M, -1, 2, 8).unbind(2) for a in (y, err))
+            s = gate / (1 + torch.exp(-gate))
+            ds = 1.1 * (eg + half * gate.abs()) + half * s.abs() + 2.0**-22
+            want = s * up
+            tol = (s.abs() + ds) * (eu + half * up.abs()) + up.abs() * ds
+            want, tol = want.reshape(M, -1), (tol + half * (want.abs() + tol)).reshape(M, -1)
+        else:
+            want, tol = y, err + half * (y.abs() + err)
+            if epilogue == 1:
+                want = y + residual.double()
+                tol = tol + half * (want.abs() + tol)
+        worst = ((out[:M].double() - want).abs() / (tol + 2.0**-24)).max().item()
+        assert worst <= 1, (epilogue, worst)
