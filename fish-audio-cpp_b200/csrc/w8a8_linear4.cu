@@ -54,6 +54,9 @@ struct L4Params {
     unsigned chunk_magic;   // the same for K / 16
     int pad;                // pitch - K
     int* status;
+    int parts;            // of a row, what is promoted together: 256 / P channels
+    unsigned part_magic;  // 2^31 over the parts of a group, rounded up
+    int xs_rows;          // of the activation scales in shared memory: G where EXACT, else one more
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -107,7 +110,7 @@ __device__ __noinline__ bool l4_wait_long(uint64_t* bar, uint32_t phase, int* st
 // T token tiles of 8; P promotes per box (256 / P channels each, all in one group); EXACT: groups of 256 / P channels, K in whole boxes and
 // the scales of a box in one aligned read; DIRECT: the codes that meet a box come through the ring behind it (two boxes of 128 channels), by the
 // warp that uses them.
-// Shared memory: rings [warps][stages][box, codes]; pieces fp32 [warps][16][8 T + 1]; activation scales over 16, fp32 [G][8 T]; not DIRECT: codes
+// Shared memory: rings [warps][stages][box, codes]; pieces fp32 [warps][16][8 T + 1]; activation scales over 16, fp32 [xs_rows][8 T]; not DIRECT: codes
 // [M][pitch], a pitch at which the rows that lanes read together lie in different banks. A run's last piece goes where its ring was.
 // (reads run on to the end of the last box: what lies behind K meets weights of zero)
 inline int l4_pitch(int K, int P) { return (K + 127) / 128 * 128 + (P <= 2 ? 16 : P == 4 ? 64 : 32); }
@@ -118,8 +121,8 @@ __host__ __device__ constexpr int l4_stage_bytes(bool direct) { return kBox + (d
 template <int T>
 constexpr int kDirectStages = T == 1 ? 3 : 2;
 template <int T>
-size_t l4_smem(int M, int K, int G, int stages, bool direct) {
-    return 1024 + static_cast<size_t>(kL4Warps) * stages * l4_stage_bytes<T>(direct) + kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(G) * 8 * T * 4 +
+size_t l4_smem(int M, int K, int xs_rows, int stages, bool direct) {
+    return 1024 + static_cast<size_t>(kL4Warps) * stages * l4_stage_bytes<T>(direct) + kL4Warps * l4_piece_floats<T>() * 4 + static_cast<size_t>(xs_rows) * 8 * T * 4 +
            (direct ? 0 : static_cast<size_t>(l4_pitch(K, 4)) * M + kBoxK);
 }
 
@@ -133,7 +136,8 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     float* const piece_s = reinterpret_cast<float*>(base + kL4Warps * p.stages * kStage);
     float* const xs_s = piece_s + kL4Warps * kPiece;
     auto end_piece = [&](int w) { return reinterpret_cast<float*>(base + w * p.stages * kStage); };  // of a finished run, in its ring
-    unsigned char* const codes_s = reinterpret_cast<unsigned char*>(xs_s + p.G * 8 * T);
+    const int xs_rows = EXACT ? p.G : p.G + 1;  // (one of zeros behind the last group)
+    unsigned char* const codes_s = reinterpret_cast<unsigned char*>(xs_s + xs_rows * 8 * T);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g8 = lane >> 2, j4 = lane & 3;
     const int row8 = (g8 & 1) << 2 | (g8 & 2) | g8 >> 2;  // the row of the tile that this lane's fragment row is (and + 8)
     // tiles [t0, t0 + nt) of this CTA, units [u0, u0 + n_mine) of this warp: the boxes of the CTA's tiles, one tile after the other
@@ -172,7 +176,9 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         for (int i = 0; i < min(p.stages, n_mine); ++i) issue(i);
     // weight scales of the box that comes next, rows row8 and row8 + 8
     __half2 ws_next[P > 1 ? P : 1];  // EXACT, P > 1: [row half][P / 2 pairs of groups]; else one {row, row + 8} pair per promote
-    auto group_of = [&](int bx, int pr) { return EXACT ? bx * P + pr : min(p.G - 1, (bx * kBoxK + pr * (kBoxK / P)) / p.g); };
+    // (a part behind K has no channels and takes two scales of zero: its sum of zero times an infinite one would be no number)
+    auto missing = [&](int part) { return !EXACT && P > 1 && part >= p.parts; };
+    auto group_of = [&](int part) { return EXACT ? part : missing(part) ? p.G : static_cast<int>(__umulhi(2u * part, p.part_magic)); };
     const __half *ws_row0 = nullptr, *ws_row1 = nullptr;  // of the tile that the next box belongs to
     auto scale_rows = [&](int tl) {
         ws_row0 = p.w_scale + static_cast<size_t>(min(tl * 16 + row8, p.N - 1)) * p.G;
@@ -195,8 +201,9 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
         } else {
 #pragma unroll
             for (int pr = 0; pr < P; ++pr) {
-                const int gr = group_of(bx, pr);
-                ws_next[pr] = __halves2half2(ws_row0[gr], ws_row1[gr]);
+                const int gr = min(p.G - 1, group_of(bx * P + pr));
+                const __half2 w = __halves2half2(ws_row0[gr], ws_row1[gr]);
+                ws_next[pr] = missing(bx * P + pr) ? __halves2half2(__ushort_as_half(0), __ushort_as_half(0)) : w;
             }
         }
     };
@@ -224,9 +231,9 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
     } else {
         ask(tid);
     }
-    for (int x = tid; x < p.G * 8 * T; x += kL4Warps * 32) {
+    for (int x = tid; x < xs_rows * 8 * T; x += kL4Warps * 32) {
         const int group = x / (8 * T), m = x % (8 * T);
-        xs_s[x] = m < p.M ? 0.0625f * ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
+        xs_s[x] = m < p.M && (EXACT || group < p.G) ? 0.0625f * ptx::ld_result_f32(p.Xs + static_cast<size_t>(m) * p.G + group) : 0.0f;
     }
     if constexpr (!DIRECT) {
 #pragma unroll 1
@@ -347,7 +354,7 @@ __global__ void __launch_bounds__(kL4Warps * 32, 2) linear4_kernel(const __grid_
                             ws0 = __low2float(ws[pr]);
                             ws1 = __high2float(ws[pr]);
                         }
-                        const uint32_t xg = xs_at + group_of(box, pr) * (8 * T * 4);
+                        const uint32_t xg = xs_at + group_of(box * P + pr) * (8 * T * 4);
 #pragma unroll
                         for (int t = 0; t < T; ++t) {
                             const uint2 xx = lds64(xg + t * 32);
@@ -535,16 +542,16 @@ cudaError_t launch_l4(SmemAttribute* attribute, int ctas, size_t smem, cudaStrea
 // least two: in the end the ring holds a piece of up to 2112 bytes.)
 constexpr size_t kHalfSm = 112 * 1024, kThirdSm = 76 * 1024;
 template <int T>
-int l4_stages(int M, int K, int G, bool direct) {
-    if (direct) return l4_smem<T>(M, K, G, kDirectStages<T>, true) <= kL4MaxSmem ? kDirectStages<T> : 0;
+int l4_stages(int M, int K, int xs_rows, bool direct) {
+    if (direct) return l4_smem<T>(M, K, xs_rows, kDirectStages<T>, true) <= kL4MaxSmem ? kDirectStages<T> : 0;
     for (int stages = 4; stages >= 2; --stages)
-        if (l4_smem<T>(M, K, G, stages, direct) <= kHalfSm) return stages;
+        if (l4_smem<T>(M, K, xs_rows, stages, direct) <= kHalfSm) return stages;
     for (int stages = 8; stages >= 2; --stages)
-        if (l4_smem<T>(M, K, G, stages, direct) <= kL4MaxSmem) return stages;
+        if (l4_smem<T>(M, K, xs_rows, stages, direct) <= kL4MaxSmem) return stages;
     return 0;
 }
-int l4_stages(int M, int K, int G, bool direct) {
-    return M > 16 ? l4_stages<4>(M, K, G, direct) : M > 8 ? l4_stages<2>(M, K, G, direct) : l4_stages<1>(M, K, G, direct);
+int l4_stages(int M, int K, int xs_rows, bool direct) {
+    return M > 16 ? l4_stages<4>(M, K, xs_rows, direct) : M > 8 ? l4_stages<2>(M, K, xs_rows, direct) : l4_stages<1>(M, K, xs_rows, direct);
 }
 
 // DIRECT where every CTA has one tile, so that a code is read once either way, and there are rows enough: eight rows of 4096 channels on 160 tiles
@@ -553,17 +560,20 @@ int l4_stages(int M, int K, int G, bool direct) {
 template <int T, int P, bool EXACT>
 cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream) {
     static SmemAttribute attribute[2] = {SmemAttribute(true), SmemAttribute(true)};
-    const bool direct = T <= 2 && ((p.M > 4 && p.tiles <= 2 * device_sms()) || l4_smem<T>(p.M, p.K, p.G, 2, false) > kHalfSm);
-    p.stages = l4_stages<T>(p.M, p.K, p.G, direct);
-    const int ctas = gemv_packed_ctas(p.tiles, device_sms(), l4_smem<T>(p.M, p.K, p.G, p.stages, direct) <= kHalfSm);
+    const bool direct = T <= 2 && ((p.M > 4 && p.tiles <= 2 * device_sms()) || l4_smem<T>(p.M, p.K, p.xs_rows, 2, false) > kHalfSm);
+    p.stages = l4_stages<T>(p.M, p.K, p.xs_rows, direct);
+    const int ctas = gemv_packed_ctas(p.tiles, device_sms(), l4_smem<T>(p.M, p.K, p.xs_rows, p.stages, direct) <= kHalfSm);
     p.cta_tiles = p.tiles / ctas;
     p.longer = p.tiles - p.cta_tiles * ctas;
     p.chunk_magic = static_cast<unsigned>(((1ull << 32) + p.K / 16 - 1) / (p.K / 16));
     p.pad = p.pitch - p.K;
+    p.parts = (p.K + kBoxK / P - 1) / (kBoxK / P);
+    const int group_parts = (p.g + kBoxK / P - 1) / (kBoxK / P);
+    p.part_magic = static_cast<unsigned>(((1ull << 31) + group_parts - 1) / group_parts);
     p.box_magic = p.boxes == 1 ? 0u : static_cast<unsigned>(((1ull << 32) + p.boxes - 1) / p.boxes);
     // Never three CTAs on an SM: what the third takes from the others is more than its early start gives (four projections at one row 22.6 us with
     // three, 20.1 with two, 30.6 with one).
-    size_t smem = l4_smem<T>(p.M, p.K, p.G, p.stages, direct);
+    size_t smem = l4_smem<T>(p.M, p.K, p.xs_rows, p.stages, direct);
     if (smem < kThirdSm) smem = kThirdSm;
     if constexpr (T <= 2)
         if (direct) {
@@ -592,10 +602,11 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
     const int P = g % 256 == 0 ? 1 : g % 128 == 0 ? 2 : g % 64 == 0 ? 4 : 8;
     const bool exact = g == kBoxK / P && K % kBoxK == 0 && (reinterpret_cast<uintptr_t>(w_scale) & (2 * P - 1)) == 0;
     // rows of a launch: as many as fit shared memory; the weights are streamed once per launch
+    const int xs_rows = G + (exact ? 0 : 1);
     int rows = 32;
-    while (rows > 1 && l4_stages(rows, K, G, rows <= 16) == 0) rows /= 2;
+    while (rows > 1 && l4_stages(rows, K, xs_rows, rows <= 16) == 0) rows /= 2;
     const bool fast = K % 32 == 0 && g % 32 == 0 && ((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(Xq)) & 15u) == 0 &&
-                      l4_stages(rows, K, G, rows <= 16) > 0 &&
+                      l4_stages(rows, K, xs_rows, rows <= 16) > 0 &&
                       // the kernel's 32-bit arithmetic
                       (static_cast<unsigned long long>((N + 15) / 16) / device_sms() + 2) * ((K + kBoxK - 1) / kBoxK) * ((K + kBoxK - 1) / kBoxK) < (1ull << 28);
     CUtensorMap map;
@@ -605,7 +616,7 @@ int launch_linear4(const void* W, const __half* w_scale, int group, const int8_t
         const int m = fast ? (M - m0 < rows ? M - m0 : rows) : M;
         L4Params p = {static_cast<const uint8_t*>(W), w_scale, Xq + static_cast<size_t>(m0) * K, Xs + static_cast<size_t>(m0) * G,
                       Y + static_cast<size_t>(m0) * columns, residual ? residual + static_cast<size_t>(m0) * N : nullptr, m, N, K, g, G, epilogue,
-                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), 0, 0, 0, 0, 0, status};
+                      (N + 15) / 16, (K + kBoxK - 1) / kBoxK, 0, l4_pitch(K, P), 0, 0, 0, 0, 0, status, 0, 0, xs_rows};
         cudaError_t e;
         if (fast) {
             if (exact)

@@ -1,4 +1,4 @@
-"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost, several tiles a CTA."""
+"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost, several tiles a CTA, infinite scales."""
 import math
 
 import numpy as np
@@ -166,3 +166,26 @@ def test_linear4_several_tiles_a_cta(ctx, M, N, K, g):
                 tol = tol + half * (want.abs() + tol)
         worst = ((out[:M].double() - want).abs() / (tol + 2.0**-24)).max().item()
         assert worst <= 1, (epilogue, worst)
+
+
+@pytest.mark.parametrize("M", [1, 7, 16, 20])
+@pytest.mark.parametrize("N,K,g", [(32, 160, 32), (48, 288, 96), (16, 320, 64), (160, 2592, 32), (40, 66, 22), (32, 384, 128), (16, 544, 544)])
+def test_linear4_infinite_scales(ctx, M, N, K, g):
+    """Codes and activations of one: every group's sum is positive, so an infinite scale gives infinity in its row or token and nowhere else."""
+    G = (K + g - 1) // g
+    W = dev(q4.pack_codes(np.ones((N, K), np.int64)))
+    x = torch.ones((M, K), dtype=torch.int8, device="cuda")
+    for group in {0, G // 2, G - 1}:
+        scale, xs = np.full((N, G), 2.0**-7, np.float16), np.full((M, G), 2.0**-3, np.float32)
+        scale[3, group], scale[N - 1, group], xs[M // 2, group] = np.inf, -np.inf, np.inf
+        want = np.full((M, N), K * 2.0**-10)
+        want[M // 2] = np.inf
+        want[:, 3], want[:, N - 1] = np.inf, -np.inf
+        out = torch.empty((M, N), dtype=torch.float16, device="cuda")
+        ctx.linear4_q(W, dev(scale), g, x, dev(xs), out, M, N, K)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy().astype(np.float64)
+        assert np.array_equal(np.isinf(got), np.isinf(want)) and not np.isnan(got).any(), (group, got[:, :8])
+        assert np.array_equal(np.sign(got), np.sign(want))
+        finite = np.isfinite(want)
+        assert (np.abs(got[finite] - want[finite]) <= 2.0**-11 * want[finite]).all()
