@@ -29,6 +29,7 @@ constexpr int kPlanThreads = 512, kPlanFew = 128;
 static_assert(kPlanThreads <= 32 * 32, "a warp adds up the warps' sums");
 constexpr int kPlanBlock = 16;
 constexpr int kPlanMaxBatch = 4096;
+constexpr int kPlanMaxBlocks = 0x7fffffff / kPlanBlock;  // of a request: its tokens, and their number rounded up to whole blocks, fit 32 bits
 
 struct PlanParams {
     const int* cached;
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(THREADS) plan_blocks_kernel(const PlanParams p
             }
             const long long have = (static_cast<long long>(cached) + kPlanBlock - 1) / kPlanBlock;
             const long long all = ended ? have : (static_cast<long long>(cached) + fresh + kPlanBlock - 1) / kPlanBlock;
-            if (all > p.max_blocks) atomicMin(&bad_s, 2);
+            if (all > min(p.max_blocks, kPlanMaxBlocks)) atomicMin(&bad_s, 2);
             mine = {ended ? 0 : fresh, all - have, ended ? have : 0};
         }
         Sums inc = mine;

@@ -320,7 +320,7 @@ W8A8_API int w8a8_qkv_attention_decode_ahead(w8a8_ctx* ctx, const void* qkv, con
  *   info        int32 [4]  {status, new tokens, blocks taken, blocks left}
  * All or nothing. Where status is not 0, no table row and no free block has changed, every slot is -1, first_token is 0 and seq_lens holds
  * the cached lengths (an ended request's too): 5 free_count out of range (with what is given back); else the lowest of 1 not enough free
- * blocks, 2 a request longer than its table row, 3 more than max_tokens new tokens, 4 a negative cached length (taken as 0). Rows of ended requests are left as they were.
+ * blocks, 2 a request longer than its table row (or 2^31 - 16 tokens), 3 more than max_tokens new tokens, 4 a negative cached length (taken as 0). Rows of ended requests are left as they were.
  * batch <= 4096. One launch. */
 W8A8_API int w8a8_plan_blocks(w8a8_ctx* ctx, const int* cached_lens, const int* new_lens, int batch, int* block_table,
                      int max_blocks_per_seq, int* free_blocks, int free_capacity, const int* free_count, int* free_count_out,

@@ -158,7 +158,7 @@ def attention_bound(q, pages, table, lens, layer, sm_scale, g, sms=148):
 # ---- the step plan ----
 def plan(cached, new, table, free, count, max_tokens, capacity):
     """What w8a8_plan_blocks leaves, from Python lists: a dict of lists."""
-    B, width = len(cached), len(table[0]) if table else 0
+    B, width = len(cached), min(len(table[0]) if table else 0, 2**27 - 1)
     table, free = [list(r) for r in table], list(free)
     blocks = lambda n: (n + 15) // 16
     give = sum(blocks(c) for c, n in zip(cached, new) if n < 0 and c >= 0)

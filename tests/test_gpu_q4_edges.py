@@ -1,4 +1,4 @@
-"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost, several tiles a CTA, infinite scales."""
+"""The decode step in 4 bits where a small mistake would be a large one: weights far below the largest, small and large queries, pages that must not be lost, several tiles a CTA, infinite scales, lengths near 2^31."""
 import math
 
 import numpy as np
@@ -189,3 +189,28 @@ def test_linear4_infinite_scales(ctx, M, N, K, g):
         assert np.array_equal(np.sign(got), np.sign(want))
         finite = np.isfinite(want)
         assert (np.abs(got[finite] - want[finite]) <= 2.0**-11 * want[finite]).all()
+
+
+# ---- the step plan -------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cached,new,status", [(2**31 - 5, 1, 2), (2**31 - 17, 2, 2), (2**31 - 1, 0, 2), (2**31 - 1, -1, 5), (0, 2**31 - 1, 1), (2**31 - 1, 2**31 - 1, 1),
+                                               (2**31 - 17, 1, 0), (2**31 - 16, 0, 0)])
+def test_plan_blocks_lengths_near_the_end_of_32_bits(ctx, cached, new, status):
+    """A table row as wide as numbers go: tokens beyond 2^31 - 16 are refused like a row that is too short (after what comes ahead of that: blocks given
+    back that the stack has no room for, blocks that it does not have)."""
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    width = 2**27
+    table = torch.full((width,), 3, dtype=torch.int32, device="cuda")
+    free, count, left = i32(8, 9), i32(2), i32(-7)
+    slots, positions = torch.full((5,), -7, dtype=torch.int64, device="cuda"), i32(*[-7] * 5)
+    lens, first, info = i32(-7), i32(-7, -7), i32(*[-7] * 4)
+    ctx.plan_blocks(i32(cached), i32(new), 1, table, width, free, 2, count, slots, positions, lens, first, 5, info, free_count_out=left)
+    torch.cuda.synchronize()
+    assert (table == 3).all() and free.tolist() == [8, 9] and left.item() == 2
+    if status:
+        assert info.tolist() == [status, 0, 0, 2] and slots.tolist() == [-1] * 5 and positions.tolist() == [0] * 5 and lens.item() == cached
+    else:
+        assert info.tolist() == [0, new, 0, 2] and lens.item() == cached + new
+        assert positions.tolist() == [cached] * new + [0] * (5 - new)
+        assert slots.tolist() == [3 * 16 + cached % 16] * new + [-1] * (5 - new)
