@@ -558,7 +558,8 @@ static int check_kv4(const w8a8_ctx* ctx, const char* what, const void* cache, i
 }
 
 size_t w8a8_kv4_cache_bytes(int n_blocks, int n_layers, int n_kv_heads, int head_dim, int group_size) {
-    if (n_blocks <= 0 || n_layers <= 0 || n_kv_heads <= 0 || head_dim != 128) return 0;
+    if (n_blocks <= 0 || n_layers <= 0 || n_kv_heads <= 0 || n_kv_heads > 65536 || head_dim != 128) return 0;
+    if (static_cast<long long>(n_blocks) * n_layers > 0x7fffffffll / n_kv_heads) return 0;  // (no call takes it; the bytes may not fit either)
     return static_cast<size_t>(n_blocks) * n_layers * n_kv_heads * kv4_page_bytes(group_size);
 }
 

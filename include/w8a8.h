@@ -333,7 +333,7 @@ W8A8_API int w8a8_plan_blocks(w8a8_ctx* ctx, const int* cached_lens, const int* 
  *   [1024, 2048)  V: tokens 2 p and 2 p + 1 at 128 p; the word 4 r + 2 half + high holds channels 64 high + 16 n + 8 half + r,
  *                 n = 0 .. 3, of token 2 p as nibbles 0 .. 3 and of token 2 p + 1 as nibbles 4 .. 7
  *   then fp16 scales of K [8 pairs of tokens][128 / group][2], and of V the same
- * The buffer is 16-byte aligned and w8a8_kv4_cache_bytes long (0: bad arguments); it needs no initialisation. */
+ * The buffer is 16-byte aligned and w8a8_kv4_cache_bytes long (0: bad arguments, or 2^31 pages and more); it needs no initialisation. */
 W8A8_API size_t w8a8_kv4_cache_bytes(int n_blocks, int n_layers, int n_kv_heads, int head_dim, int group_size);
 
 /* w8a8_qknorm_rope_kvwrite for this cache, tokens named by slots (w8a8_plan_blocks): a prompt's rows as well as a decode step's. qkv
