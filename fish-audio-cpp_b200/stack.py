@@ -147,6 +147,11 @@ def synthetic_kv(torch, cfg: SlowARConfig, batch: int, context: int, max_new: in
     return caches[0], caches[1], perm.view(batch, max_blocks).contiguous(), max_blocks
 
 
+# what w8a8_plan_blocks may refuse
+PLAN_STATUS = {1: "not enough free blocks", 2: "a sequence longer than its table row", 3: "too many new tokens", 4: "a negative length",
+               5: "the number of free blocks is out of range"}
+
+
 class SlowARStack:
     def __init__(self, torch, ctx: capi.Context, cfg: SlowARConfig, batch: int, context: int, max_new: int = 256,
                  tp_rank: int = 0, tp_size: int = 1, seed: int = 0, all_reduce=None, pack: bool = True,
@@ -295,7 +300,9 @@ class SlowARStack:
         self.seq_lens.fill_(context)  # tokens in the cache; a step's plan adds its own
         self.slots = torch.empty((B,), dtype=torch.int64, device=dev)
         self.first_token = torch.empty((B + 1,), dtype=torch.int32, device=dev)
-        self.plan_info = torch.empty((4,), dtype=torch.int32, device=dev)
+        self.plan_info = torch.zeros((4,), dtype=torch.int32, device=dev)
+        self.room = self.max_blocks * c.block_tokens - context  # steps for which there are blocks
+        self._steps = 0
 
     def _linear(self, w, s, xq, xs, y, n, k, epilogue=capi.EPI_NONE):
         (self.ctx.linear4_q if self.weight_bits == 4 else self.ctx.linear_q)(w, s, self.cfg.group, xq, xs, y, self.B, n, k, epilogue=epilogue)
@@ -303,11 +310,18 @@ class SlowARStack:
     # ------------------------------------------------------------------------------------------
     def decode_step(self, x_in=None):
         """One token for every sequence. x_in fp16 [B, dim] (the embedding of the new token); returns
-        the final-normed hidden state in self.out. All launches go to the current stream. The first layer's attention
+        the final-normed hidden state in self.out. With a 4-bit cache a step for which there are no blocks left raises RuntimeError. Replays
+        of a captured step are not counted for that: where the plan on the GPU refuses one (and a step behind it) the cache stays as it is and self.out has no
+        meaning, which check_plan() tells. All launches go to the current stream. The first layer's attention
         waits for all that is ahead on the stream (positions, lengths, cache rows of earlier steps), so the other layers'
         may read those before the kernels directly ahead of them have finished."""
         c, ctx, B, g = self.cfg, self.ctx, self.B, self.cfg.group
         D = c.head_dim
+        if self.kv_bits == 4:
+            if not self.torch.cuda.is_current_stream_capturing():
+                if self._steps >= self.room:
+                    raise RuntimeError(f"decode_step: the sequences fill their {self.max_blocks} blocks ({self.context0} tokens of context, {self.room} of steps)")
+                self._steps += 1
         if x_in is not None:
             self.x.copy_(x_in, non_blocking=True)
         sm_scale = 1.0 / math.sqrt(D)
@@ -474,10 +488,19 @@ class SlowARStack:
             self.ctx.register_packed_weight(W, None)
         self._registered = []
 
+    def check_plan(self):
+        """Raises RuntimeError where the newest step of a 4-bit cache was refused by its plan (so is every step after it). Waits for the current stream."""
+        if self.kv_bits == 4:
+            status, _, _, left = self.plan_info.tolist()
+            if status:
+                raise RuntimeError(f"the step plan refused the last step (status {status}: {PLAN_STATUS.get(status, '?')}; {left} blocks are free)")
+
     def reset_positions(self):
         if self.kv_bits == 4:  # (the blocks taken since go back on the stack, where the next steps find them in the same order)
             self.seq_lens.fill_(self.context0)
             self.free_count.fill_(self.free0)
+            self.plan_info.zero_()
+            self._steps = 0
             return
         self.positions.fill_(self.context0)
         self.seq_lens.fill_(self.context0 + 1)
