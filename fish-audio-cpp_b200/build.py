@@ -1,7 +1,7 @@
 """Builds libw8a8.so in-tree with nvcc for sm_100a.
 
 Every .cu under csrc/ is compiled to an object in _build/ (only when it or a header is
-newer than the object) and linked into lib/libw8a8.so; csrc/w8a8_calls.cpp becomes lib/w8a8_calls.so. No JIT cache is involved, so the
+newer than the object) and linked into lib/libw8a8.so; csrc/w8a8_calls.cpp becomes lib/w8a8_calls<the interpreter's suffix>. No JIT cache is involved, so the
 built library travels with the source tree.
 """
 from __future__ import annotations
@@ -84,16 +84,18 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False, 
 
 
 def build_calls(force: bool = False) -> Path | None:
-    """lib/w8a8_calls.so, the Python side of the decode step's calls; None where there are no Python headers (the binding then uses ctypes)."""
-    src, out, headers = CSRC / "w8a8_calls.cpp", LIB.parent / "w8a8_calls.so", sysconfig.get_paths()["include"]
+    """The Python side of the decode step's calls, lib/w8a8_calls with the interpreter's suffix (an extension of one interpreter is none of another's).
+    None where there are no Python headers or no compiler that takes it: the binding then uses ctypes."""
+    src, out, headers = CSRC / "w8a8_calls.cpp", LIB.parent / ("w8a8_calls" + sysconfig.get_config_var("EXT_SUFFIX")), sysconfig.get_paths()["include"]
     if not Path(headers, "Python.h").exists() or not shutil.which("g++"):
         return None
     if force or not out.exists() or out.stat().st_mtime < max(src.stat().st_mtime, (INCLUDE / "w8a8.h").stat().st_mtime):
         cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-I{headers}", f"-I{INCLUDE}", str(src), "-o", str(out)]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError("g++ failed on w8a8_calls.cpp")
+            out.unlink(missing_ok=True)
+            sys.stderr.write(f"{r.stdout}{r.stderr}w8a8_calls.cpp was not built; its calls go through ctypes\n")
+            return None
     return out
 
 

@@ -3,7 +3,9 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
+import sysconfig
 import threading
+import warnings
 from pathlib import Path
 
 ACT_PER_TOKEN_GROUP, ACT_PER_TOKEN = 0, 1
@@ -260,7 +262,7 @@ def kv4_attention_workspace_bytes(n_heads, n_kv) -> int:
 
 
 class _CtypesCalls:
-    """The calls of w8a8_calls where it was not built (no Python headers): the same arguments, through ctypes."""
+    """The calls of w8a8_calls where there is none for this interpreter: the same arguments, through ctypes."""
 
     def __init__(self, lib):
         self._lib = lib
@@ -278,18 +280,25 @@ class _CtypesCalls:
 _CALLS = None
 
 
+def _calls_path() -> Path:
+    return Path(__file__).resolve().parent / "lib" / ("w8a8_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
 def _load_calls(lib):
-    """w8a8_calls (csrc/w8a8_calls.cpp), bound to the loaded library's functions."""
+    """w8a8_calls (csrc/w8a8_calls.cpp), bound to the loaded library's functions; ctypes where it was not built for this interpreter or cannot be loaded."""
     global _CALLS
     if _CALLS is None:
-        path = Path(__file__).resolve().parent / "lib" / "w8a8_calls.so"
+        path = _calls_path()
         if path.exists():
-            spec = importlib.util.spec_from_file_location("w8a8_calls", path)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
-            module.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in dir(module) if n.startswith("w8a8_")})
-            _CALLS = module
-        else:
+            try:
+                spec = importlib.util.spec_from_file_location("w8a8_calls", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in dir(module) if n.startswith("w8a8_")})
+                _CALLS = module
+            except (ImportError, AttributeError, KeyError) as e:
+                warnings.warn(f"{path.name} cannot be used ({e}); its calls go through ctypes", RuntimeWarning)
+        if _CALLS is None:
             _CALLS = _CtypesCalls(lib)
     return _CALLS
 
