@@ -4,7 +4,7 @@
 //   k_t, v_t = code * scale of the row's group; one pass with the running maximum and sum of the softmax, both fp32
 //
 // Bound: HBM and the arithmetic, close to one another. A token costs 128 + 4 G bytes per kv head (K and V; G = 128 / group) instead of the fp16
-// cache's 512; a warp executes some 340 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 74 us, 60 % of
+// cache's 512; a warp executes some 325 instructions for the 2304 bytes of 16 tokens at groups of 32. 2 x 131000 tokens: 75 us, 60 % of
 // the measured copy rate; the copies alone, without arithmetic, take 54, the arithmetic alone, without copies, 61 (the scores and the
 // softmax 42 of them, a chain that three warps a scheduler cannot hide). Two pages at a time, one page's scores beside the sum over the page
 // before it, scales folded into p, and 8 or 14 or 16 warps instead of 12 changed nothing or cost time.
@@ -23,7 +23,7 @@
 // that nothing of a small q is lost; above, what a sixteenth rounds by is 2^-21 beside a q of 2^9. The 8 that stored codes carry leaves with the
 // accumulator's start, -8 * sum of q over the group. Sums are fp32 per group, times the group's scale in fp32. P V: codes as fp16 numbers
 // (1024 + code, less 1032), times the scale, rounded to fp16 (2^-11 relative; what w8a8_kv4_read returns); p as two fp16 numbers, the
-// rounded one and what that left, which costs nothing here (77.3 and 77.1 us) and takes the error from 3.3e-4 of the output to 2.6e-4,
+// rounded one and what that left, which costs nothing here and takes the error from 3.3e-4 of the output to 2.6e-4,
 // of which the output's own rounding is 2.1e-4; products are summed in fp32. The reference of the exponentials lies below the row's largest score and moves, and the
 // sums with it, when a weight passes 2^kTop: a few times per row only.
 #include "sm100_ptx.cuh"
@@ -41,10 +41,10 @@ using q4::kTokens;
 constexpr int kMaxBatch = 4096;
 constexpr float kNoScore = -1e30f;
 // Pairs of at most kFewPages, and of at most twice a CTA's share (with eight heads, whose pieces are twice as long, four times) up to kWholePages, are not
-// cut between CTAs: a join costs what a warp's two or three pages cost. us whole and cut: 1 x 400 tokens 7.3 and 8.3, 8 x 400 8.0 and 9.5, 16 x 1024 11.5 and 13.1; 8 x 1024 11.3 and 11.0, 8 x 1500 13.8 and
+// cut between CTAs: a join costs what a warp's two or three pages cost. us whole and cut, when the rule was made: 1 x 400 tokens 7.3 and 8.3, 8 x 400 8.0 and 9.5, 16 x 1024 11.5 and 13.1; 8 x 1024 11.3 and 11.0, 8 x 1500 13.8 and
 // 12.0 (more than twice a share), with eight heads 8 x 1024 11.7 and 13.1; 64 x 4000 79 and 73 (whole up to 256 pages, and up to 96).
 constexpr int kFewPages = 32, kWholePages = 96;
-// Pages that a pair counts for beyond its own. us with 0, 2, 4 and 8: 48 ragged sequences up to 8000 tokens 34, 23.5, 23.2, 23.4; 200 up to 2000
+// Pages that a pair counts for beyond its own. us with 0, 2, 4 and 8, when it was chosen: 48 ragged sequences up to 8000 tokens 34, 23.5, 23.2, 23.4; 200 up to 2000
 // tokens 50, 31.7, 32.1, 35.1; 64 x 512 20.5, 21.1, 21.3, 22.0.
 constexpr int kPairCost = 3;
 // The largest weight of a warp's pages so far stands between 2^kAt and 2^kTop, at the upper end of fp16: what a weight as two fp16 numbers loses is 2^-22 of itself
@@ -88,7 +88,7 @@ __device__ __forceinline__ void unpack8_tiny(uint32_t w, uint32_t (&h)[4]) {
     h[2] = up & 0x000f000fu;
     h[3] = up & 0x00f000f0u;
 }
-// The eight codes themselves.
+// The eight codes themselves: nibbles set into the mantissa of 1024 (Kim, Henry, Fahim and Awadalla, "Who says elephants can't run", 2022), the upper ones over 16.
 __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&h)[4]) {
     const __half2 off = as_half2(0x64086408u);                                        // 1024 + 8
     const __half2 sixteenth = as_half2(0x2c002c00u), off16 = as_half2(0xd480d480u);  // 1 / 16; -(64 + 8)
@@ -255,8 +255,8 @@ __device__ __noinline__ void finish_whole(const Kv4Params& p, const float* piece
 }
 
 // Heads h0 .. h0 + E - 1 of pieces base[i], i in `which`, added and finished, or to the piece `to`. E is one, or the heads of a group of codes. Lane i
-// sees to piece i's weights, so that the loop over the pieces has no chain but its sums. (Four heads by a warp each: 8 x 1024 tokens 11.5 us; all by one
-// warp, piece by piece, 12.0.)
+// sees to piece i's weights, so that the loop over the pieces has no chain but its sums. (Four heads by a warp each take half a microsecond less over
+// 8 x 1024 tokens than all by one warp, piece by piece.)
 template <int R, int E>
 __device__ __noinline__ void merge_share(const Kv4Params& p, const float* base, uint32_t which, float* to, int b, int kvh, int h0) {
     constexpr int kPiece = piece_floats(R);
@@ -311,8 +311,8 @@ __device__ __forceinline__ void merge_share(const Kv4Params& p, int each, const 
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 // G groups per head; R the most query heads per kv head (4 or 8); W warps.
-// Twelve warps of 168 registers: with sixteen of 128 the long cases take the same (64 x 4000 tokens 74 us) and the short ones more (8 x 1024 tokens
-// 12.5 us instead of 12.0, 1 x 8192 13.0 instead of 12.2); with eight the long ones more (91). Four stages are 9 KB a warp on their way.
+// Twelve warps of 168 registers: with sixteen of 128 the long cases take the same (64 x 4000 tokens) and the short ones more (8 x 1024 tokens
+// 0.5 us, 1 x 8192 0.8); with eight the long ones a fifth more. Four stages are 9 KB a warp on their way.
 constexpr int kWarps = 12, kStages = 4;
 template <int G, int R>
 constexpr int kv4_smem(int batch) {

@@ -6,7 +6,7 @@
 // decode step's go the same way, and rows with a negative slot (a captured step's empty rows) are left alone, their q too.
 //
 // Bound: for prompts instructions and bytes alike (2 (n_q + 2 n_kv) 128 read and 2 n_q 128 written per token), latency for a decode step.
-// 8192 tokens of 32 + 16 heads 43 us to write (27 for the bytes; 35 without the norm) and 10.9 to read back, a decode step's 8 tokens 3.5 for both.
+// 8192 tokens of 32 + 16 heads 43 us to write (27 for the bytes; 35 without the norm) and 10.9 to read back, a decode step's 8 tokens 3.6 for both.
 // Half a warp holds a head, eight neighbouring channels a lane: 16-byte reads and writes, a K word a lane, and of the norm's tree three levels
 // in the lane. A warp takes one token and one pair of heads after another, so that the angles are made once.
 #include "sm100_ptx.cuh"

@@ -6,8 +6,8 @@
 // int32, each group is promoted with both scales in fp32. W4 is row-major, two codes a byte (two's complement, the even k in the low
 // four bits): a checkpoint's rows as they are, no packing step.
 //
-// Bound: the weights' bytes from HBM (N K / 2 + 2 N G): 155776 x 2560 at 16 rows in groups of 256 39.1 us, 81 % of the measured copy rate; at decode
-// sizes latency: 19456 x 2560 with SwiGLU at 8 rows in groups of 64 8.2 us (3.9 for the bytes; 6.1 without activations and arithmetic), 6144 x 2560 at
+// Bound: the weights' bytes from HBM (N K / 2 + 2 N G): 155776 x 2560 at 16 rows in groups of 256 39.3 us in bursts, 81 % of the measured copy rate
+// (41 to 44 in longer loops, at the card's power limit); at decode sizes latency: 19456 x 2560 with SwiGLU at 8 rows in groups of 64 8.2 us (3.9 for the bytes; 6.1 without activations and arithmetic), 6144 x 2560 at
 // one row 3.6.
 //
 // A word of eight codes becomes two operand registers of mma.m16n8k32.s8 by a shift and two masks: w << 4 and w, both & 0xf0f0f0f0, are
@@ -555,7 +555,7 @@ int l4_stages(int M, int K, int xs_rows, bool direct) {
 }
 
 // DIRECT where every CTA has one tile, so that a code is read once either way, and there are rows enough: eight rows of 4096 channels on 160 tiles
-// in a run of launches 3.9 us, through shared memory 4.2; sixteen 4.7 and 5.7; one row 5.0 and 3.5; eight rows of 2560 on 1216 tiles 8.3 and 7.7.
+// in a run of launches 3.9 us, through shared memory 4.2; sixteen 4.7 and 5.7; one row 5.0 and 3.5 (between them the rule has not been measured); eight rows of 2560 on 1216 tiles 8.3 and 7.7.
 // And where a CTA's codes leave no room for two CTAs on an SM (eight rows of 9728 channels: 10.7 us with one of them).
 template <int T, int P, bool EXACT>
 cudaError_t launch_boxes(L4Params p, const CUtensorMap& map, cudaStream_t stream) {
